@@ -625,6 +625,220 @@ hipError_t rf_gemv_qkv_q4_k_q6_k_v_rmsnorm_launch(const void* w_q, const void* w
                                                   float* out_k, float* out_v, int n_rows, int n_q, int n_kv,
                                                   hipStream_t stream);
 
+/* ---- Several requests on a paged cache (no reference counterpart) -------
+ * The reference and the launchers above run one sequence over a contiguous
+ * cache.  These run a step of a batch: each of num_seqs requests adds
+ * new_lens[b] >= 0 tokens (a piece of its prompt, or one token of decode) to a
+ * cache whose rows lie in pages that any request may own.  Token rows of all
+ * requests stand one behind the other ([rows][...]); request b owns rows
+ * [q_start[b], q_start[b + 1]), rows past q_start[num_seqs] are padding.
+ *
+ *   rf_paged_plan_launch       once a step: pages for the new tokens, block
+ *                              tables, row ranges, positions and slots
+ *   rf_paged_rope_write_launch per layer: per-head norms, RoPE, fp16 q, and k
+ *                              and v into the rows' slots
+ *   rf_paged_attention_launch  per layer: the new rows over their requests' pages
+ *   rf_logits_rules_launch     before a token is picked
+ *   rf_paged_release_launch    the pages of ended requests back to the free ones
+ *
+ * Arguments come as a struct (a caller keeps one per layer and step shape);
+ * it is read during the call only.  Lengths, positions and tables are device
+ * memory, so captured steps replay with the values they then hold.  The
+ * current device must be the stream's.  The launchers allocate nothing, do not
+ * synchronise, return hipErrorInvalidValue on a rejected argument and are
+ * otherwise as those above.  Zero rows or requests: success, nothing written. */
+
+/* K and V pages of one layer, fp16 bits.  Position t of a request, head h, dim
+ * i: k[page * page_stride + (t % page_size) * row_stride + h * head_stride + i]
+ * with page = the request's block table entry t / page_size; v alike.  Strides
+ * in elements, > 0 and multiples of 8; k and v 16-byte aligned; head_dim 64,
+ * 128 or 256; page_size a power of two, 8 to 1024; num_pages * page_size <
+ * 2^31. */
+typedef struct rf_paged_cache {
+    uint16_t* k;
+    uint16_t* v;
+    int64_t page_stride;
+    int64_t row_stride;
+    int64_t head_stride;
+    int32_t num_pages;
+    int32_t page_size;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+} rf_paged_cache;
+
+/* The plan of a step.  Requests are served in order: request b needs
+ * ceil((ctx + new) / page_size) - ceil(ctx / page_size) pages beside the ones
+ * it has (ctx = ctx_in[b] cached positions).  It is refused when new_lens[b] or
+ * ctx is negative, when its rows would pass max_rows or its pages max_blocks,
+ * or when it needs pages and its needs and those of the requests before it
+ * (refused for want of pages or not) exceed the free ones; a request that needs
+ * none is never refused for want of pages.  Pages come off the top of the
+ * stack free_pages[0 .. free_in[0]) in request order.
+ * Written: block_tables[b * max_blocks + ..] for the new pages; q_start[0 ..
+ * num_seqs] (a refused request keeps its rows, all clipped to max_rows);
+ * kv_lens[b] = ctx + new, or 0 when refused; ctx_out[b] = ctx + new, or ctx
+ * when refused; free_out[0] = free pages left; for every row below max_rows
+ * positions[r] = ctx + its index in the request and slots[r] = page *
+ * page_size + position % page_size -- rows of refused requests and padding
+ * rows get position 0 and slot -1.  ctx_out may be ctx_in and free_out may be
+ * free_in; no other buffers may overlap.  free_pages holds num_pages entries;
+ * a free_in outside [0, num_pages] is taken as the nearer end. */
+typedef struct rf_paged_plan {
+    const int32_t* new_lens;
+    const int32_t* ctx_in;
+    int32_t* ctx_out;
+    const int32_t* free_pages;
+    const int32_t* free_in;
+    int32_t* free_out;
+    int32_t* block_tables;
+    int32_t* q_start;
+    int32_t* kv_lens;
+    int32_t* positions;
+    int32_t* slots;
+    int32_t num_seqs;
+    int32_t max_blocks;
+    int32_t page_size;
+    int32_t max_rows;
+    int32_t num_pages;
+} rf_paged_plan;
+hipError_t rf_paged_plan_launch(const rf_paged_plan* plan, hipStream_t stream);
+
+/* Requests b with ended[b] != 0 give their ceil(ctx_lens[b] / page_size) pages
+ * back, in order, onto the stack free_pages[0 .. free_count[0]), and their
+ * ctx_lens[b] becomes 0.  All in place.  A request whose pages would take the
+ * stack past num_pages entries keeps them (a page was handed back twice). */
+hipError_t rf_paged_release_launch(const int32_t* ended, int32_t* ctx_lens, const int32_t* block_tables,
+                                   int32_t* free_pages, int32_t* free_count, int num_seqs, int max_blocks,
+                                   int page_size, int num_pages, hipStream_t stream);
+
+/* d_turns[i], i < rot_dim / 2: the part of a full turn by which one position
+ * turns pair i, theta_i / 2 pi in 64 bits, with theta_i = theta_base^(-2 i /
+ * rot_dim), divided by freq_scale[i] when given, and stretched for contexts
+ * longer than the model was trained on:
+ *   RF_ROPE_PLAIN   theta_i
+ *   RF_ROPE_LINEAR  theta_i / factor
+ *   RF_ROPE_YARN    theta_i (1 - r_i) + theta_i / factor r_i, r_i rising from 0
+ *                   to 1 between the pairs that make beta_fast and beta_slow
+ *                   turns over orig_positions: pair(beta) = rot_dim ln(orig_positions
+ *                   / (2 pi beta)) / (2 ln theta_base), the lower end rounded down
+ *                   and at least 0, the upper up and at most rot_dim - 1
+ * rot_dim even, 2 to 256; theta_base > 1, factor > 0, and for YaRN
+ * orig_positions > 0 and beta_fast >= beta_slow > 0. */
+enum { RF_ROPE_PLAIN = 0, RF_ROPE_LINEAR = 1, RF_ROPE_YARN = 2 };
+hipError_t rf_rope_turns_table(double* d_turns, int rot_dim, double theta_base, int mode, double factor,
+                               double orig_positions, double beta_fast, double beta_slow, const float* d_freq_scale,
+                               hipStream_t stream);
+
+/* The rotary step into the pages.  Rows r with a slot in [0, num_pages *
+ * page_size): q heads [r * ld_q + h * head_dim ..], k and v heads alike (fp32)
+ * are normed per head (q_norm, k_norm [head_dim]; either may be null to skip),
+ * dims [0, rot_dim) of q and k are turned by positions[r] * turns[i] turns
+ * (neox != 0: pairs (i, i + rot_dim / 2), else (2 i, 2 i + 1)), cosine and sine
+ * taken of the angle reduced in 64 bits and scaled by attn_factor (YaRN's 0.1 ln
+ * factor + 1, else 1); q goes to q16[r * ld_q16 + ..] and k and v to the slot,
+ * rounded to fp16 once.  Other rows are skipped: their q16 stays.  The slots of
+ * one call are distinct.  rot_dim a multiple of 8, 0 to head_dim; fp32 buffers and
+ * q16 16-byte aligned; ld_q, ld_k, ld_v multiples of 4, ld_q16 of 8; rows <=
+ * 2^23; outputs overlap nothing. */
+typedef struct rf_paged_rope {
+    const float* q;
+    const float* k;
+    const float* v;
+    const float* q_norm;
+    const float* k_norm;
+    uint16_t* q16;
+    const int32_t* positions;
+    const int32_t* slots;
+    const double* turns;
+    int64_t ld_q;
+    int64_t ld_k;
+    int64_t ld_v;
+    int64_t ld_q16;
+    int32_t rows;
+    int32_t num_heads;
+    int32_t rot_dim;
+    int32_t neox;
+    float eps;
+    float attn_factor;
+} rf_paged_rope;
+hipError_t rf_paged_rope_write_launch(const rf_paged_rope* step, const rf_paged_cache* cache, hipStream_t stream);
+
+/* Causal GQA attention of the new rows over the paged cache.  Row i of request
+ * b (n = q_start[b + 1] - q_start[b] rows, kv = kv_lens[b] positions with the
+ * new ones) stands at position p = kv - n + i and sees positions max(0, p -
+ * window + 1) .. p (window 0: all up to p): out = sum_j softmax_j(scale q . k_j)
+ * v_j, query head h on KV head h / (num_heads / num_kv_heads).  A row that sees
+ * nothing (p < 0) gets zeros; rows past q_start[num_seqs] are left as they were.
+ * What lies in the cache behind a row's position, or in front of its window,
+ * does not enter, whatever it holds.  q fp16 bits [row][ld_q], out fp16 bits
+ * (rounded once from fp32) or fp32 (out_f32 != 0) [row][ld_out].  The weights are
+ * rounded to fp16 before they meet V; scores, maxima, sums and outputs are held
+ * in fp32.  max_new is a hint, the largest n of the step, that picks the
+ * kernels; results hold for any.  kv_lens beyond max_blocks * page_size are
+ * clipped, q_start beyond rows too; rows of a request whose table names a page
+ * outside [0, num_pages) in the positions that it sees may get NaN, and nothing
+ * outside the cache is read.  workspace: rf_paged_attention_workspace_bytes
+ * bytes, 16-byte aligned (launches that share one must be stream-ordered).
+ * q, out 16-byte aligned, ld_q, ld_out multiples of 8; scale finite; window >= 0;
+ * num_heads a multiple of num_kv_heads, at most 64 of them a KV head. */
+typedef struct rf_paged_attention {
+    const uint16_t* q;
+    void* out;
+    const int32_t* block_tables;
+    const int32_t* q_start;
+    const int32_t* kv_lens;
+    void* workspace;
+    size_t workspace_bytes;
+    int64_t ld_q;
+    int64_t ld_out;
+    int32_t num_seqs;
+    int32_t max_blocks;
+    int32_t rows;
+    int32_t num_heads;
+    int32_t max_new;
+    int32_t window;
+    int32_t out_f32;
+    float scale;
+} rf_paged_attention;
+size_t rf_paged_attention_workspace_bytes(int num_heads, int num_kv_heads, int head_dim);
+hipError_t rf_paged_attention_launch(const rf_paged_attention* step, const rf_paged_cache* cache, hipStream_t stream);
+
+/* Rules on the logits of each row before a token is picked.  With the row's
+ * history history[r * ld_history + i], i < total_lens[r], of which the first
+ * prompt_lens[r] are prompt: for every token v
+ *   x = logits[r * ld_logits + v];
+ *   v in the history:            x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   c of the others are v:       x = (x - frequency[r] * c) - (c > 0 ? presence[r] : 0)
+ *   entries bias_start[r] .. bias_start[r + 1] that name v: x = x + their values' sum, in list order
+ *   bit v % 32 of allowed[r * ld_allowed + v / 32] clear: x = -inf
+ * into out[r * ld_out + v].  repetition, frequency and presence (any null: that
+ * rule is off), the bias triple (all null) and allowed (null) are optional, the
+ * history when none of the three penalties is given.  Tokens outside [0, vocab)
+ * in history or bias are skipped; total_lens is clipped to [0, ld_history].
+ * out may be logits itself (with ld_out = ld_logits), else they do not overlap.
+ * rows <= 65535. */
+typedef struct rf_logits_rules {
+    const float* logits;
+    float* out;
+    int64_t ld_logits;
+    int64_t ld_out;
+    const int32_t* history;
+    int64_t ld_history;
+    const int32_t* prompt_lens;
+    const int32_t* total_lens;
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const int32_t* bias_start;
+    const int32_t* bias_ids;
+    const float* bias_values;
+    const uint32_t* allowed;
+    int64_t ld_allowed;
+    int32_t rows;
+    int32_t vocab;
+} rf_logits_rules;
+hipError_t rf_logits_rules_launch(const rf_logits_rules* rules, hipStream_t stream);
+
 /* ---- Parity probes (no reference counterpart) ---------------------------
  * Expose the intermediate integers of the Q8-inline path so tests can check
  * them bit-exactly.  They run the same device code as the GEMV. */

@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "librocmforge_cdna4.so"
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+_d = ctypes.c_double
 _sz = ctypes.c_size_t
 
 # name -> argtypes (all return hipError_t as int)
@@ -98,6 +99,12 @@ SIGNATURES = {
     "convert_f32_to_f16": [_vp, _vp, _i, _vp],
     "wmma_attention_prefill_gqa_causal_launch": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp],
     "rf_attention_prefill_gqa_causal_f16_launch": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp],
+    "rf_paged_plan_launch": [_vp, _vp],
+    "rf_paged_release_launch": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp],
+    "rf_rope_turns_table": [_vp, _i, _d, _i, _d, _d, _d, _d, _vp, _vp],
+    "rf_paged_rope_write_launch": [_vp, _vp, _vp],
+    "rf_paged_attention_launch": [_vp, _vp, _vp],
+    "rf_logits_rules_launch": [_vp, _vp],
     "rf_q8_0_quantize_launch": [_vp, _vp, _vp, _vp, _i, _vp],
     "rf_q4_k_q8_int_dots_launch": [_vp, _vp, _vp, _i, _i, _vp],
     "rf_mfma_peak_launch": [_vp, _vp, _i, _i, _vp],
@@ -129,5 +136,7 @@ def load() -> ctypes.CDLL:
     lib.rf_library_version.restype = ctypes.c_char_p
     lib.rf_flash_attn_decode_workspace_bytes.argtypes = [_i, _i]
     lib.rf_flash_attn_decode_workspace_bytes.restype = _sz
+    lib.rf_paged_attention_workspace_bytes.argtypes = [_i, _i, _i]
+    lib.rf_paged_attention_workspace_bytes.restype = _sz
     _LIB = lib
     return lib
