@@ -651,7 +651,7 @@ hipError_t rf_gemv_qkv_q4_k_q6_k_v_rmsnorm_launch(const void* w_q, const void* w
 /* K and V pages of one layer, fp16 bits.  Position t of a request, head h, dim
  * i: k[page * page_stride + (t % page_size) * row_stride + h * head_stride + i]
  * with page = the request's block table entry t / page_size; v alike.  Strides
- * in elements, > 0 and multiples of 8; k and v 16-byte aligned; head_dim 64,
+ * in elements, > 0 and multiples of 8, row_stride <= 2^26; k and v 16-byte aligned; head_dim 64,
  * 128 or 256; page_size a power of two, 8 to 1024; num_pages * page_size <
  * 2^31. */
 typedef struct rf_paged_cache {
@@ -774,7 +774,7 @@ hipError_t rf_paged_rope_write_launch(const rf_paged_rope* step, const rf_paged_
  * (rounded once from fp32) or fp32 (out_f32 != 0) [row][ld_out].  The weights are
  * rounded to fp16 before they meet V; scores, maxima, sums and outputs are held
  * in fp32.  max_new is a hint, the largest n of the step, that picks the
- * kernels; results hold for any.  kv_lens beyond max_blocks * page_size are
+ * kernels; results hold for any.  kv_lens beyond max_blocks * page_size (< 2^31) are
  * clipped, q_start beyond rows too; rows of a request whose table names a page
  * outside [0, num_pages) in the positions that it sees may get NaN, and nothing
  * outside the cache is read.  workspace: rf_paged_attention_workspace_bytes

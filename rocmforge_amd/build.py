@@ -27,10 +27,11 @@ FLAGS = [
 ]
 
 
-# Per-source extras.  model_ops.hip: the prefill attention (its only MFMA
-# kernel) rescales and reads its accumulators with VALU every key tile; with
+# Per-source extras.  model_ops.hip, paged_attn.hip: the prefill attention (the
+# only MFMA kernels there) rescales and reads its accumulators with VALU every key tile; with
 # them in AGPRs each tile paid ~350 accvgpr moves, in VGPRs none.
-EXTRA = {"model_ops.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+EXTRA = {"model_ops.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _run(cmd: list[str]) -> None:

@@ -2,8 +2,26 @@
 // paged fp16 cache (rf_paged_attention_launch; the header states what it
 // computes).  No counterpart in the reference, which runs one sequence over a
 // contiguous cache.
+//
+// A request's rows are packed with the heads of a KV head's group: packed row
+// r = token * group + head of the group, n * group of them a request and KV
+// head, in tiles that share what they read of K and V.  Two kernels:
+//   narrow  tiles of 16 packed rows, for requests of few rows (decode): each
+//           wave streams its own pieces of K and V.  Memory-bound.
+//   wide    tiles of 32 packed rows a wave, for pieces of prompt: the waves of
+//           a workgroup share K and V.  MFMA-bound.
+// Both compute S^T = K Q^T, so that a lane holds scores of one packed row and
+// the weights in its accumulator registers are the B operand of O^T = V^T P^T
+// as they are; V is transposed by its LDS reads.  K and V come by LDS DMA from
+// the pages, 2 to 8 rows an instruction (never across a page).
+//
+// A tile's positions are cut into parts for several workgroups where that is
+// needed to fill the chip or to even out long and short requests; a second
+// kernel joins the parts' (m, l, O).  Lengths are in device memory, so every
+// workgroup works its item out from them: a few loads and wave scans.
 #include <hip/hip_fp16.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -12,87 +30,681 @@
 
 namespace rf {
 
-// One workgroup a row and head.  D / 8 lanes hold a position, 8 dims a lane; a
-// wave takes every fourth group of 512 / D positions with a running maximum,
-// sum and output, and the waves' states are joined through LDS.
-template <int D>
-__global__ __launch_bounds__(256) void rf_paged_attn_rows_kernel(const rf_paged_attention a, const rf_paged_cache c) {
-    constexpr int LPP = D / 8, PW = 64 / LPP, W = 4;
-    __shared__ float part[W * PW][D + 2];
-    const int r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (r >= a.q_start[a.num_seqs]) return;
-    int lo = 0, hi = a.num_seqs;                 // q_start[lo] <= r < q_start[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.q_start[mid] <= r)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    const int n = a.q_start[lo + 1] - a.q_start[lo], i = r - a.q_start[lo];
-    const int kv = (int)min((int64_t)max(a.kv_lens[lo], 0), (int64_t)a.max_blocks * c.page_size);
-    const int p = kv - n + i, from = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    const int sub = lane % LPP, slot = wave * PW + lane / LPP;
-    const int kvh = h / (a.num_heads / c.num_kv_heads);
-    const int* table = a.block_tables + (int64_t)lo * a.max_blocks;
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) const h8* lds_h8;
+typedef __attribute__((address_space(3))) s4* lds_s4;
+typedef __attribute__((address_space(3))) const h4* lds_h4;
 
-    float q[8], o[8] = {0, 0, 0, 0, 0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-    auto load8 = [](const uint16_t* s, float v[8]) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(s);
+constexpr float kNone = -3.0e+38f;               // the maximum of no scores
+constexpr float kLog2e = 1.4426950408889634f;
+
+constexpr int kNarrowRows = 16, kNarrowKeys = 32;
+constexpr int kWideKeys = 64;
+// Parts aimed at over the chip, and the least positions of one, in units of
+// keys.  A tile is cut only where its share is longer than total / parts, so at
+// most twice as many parts are written to the workspace.
+constexpr int kNarrowParts = 512, kNarrowLeast = 4;
+constexpr int kWideParts = 256, kWideLeast = 8;
+constexpr int kMergeRows = 16;
+
+// ---- which part of which request a workgroup does ---------------------------------------
+
+struct Share {
+    int b, q0, n, kv;            // the request, its first row, rows and positions
+    int tiles, tile;             // of its packed rows
+    int parts, part;             // of the tile's positions
+    int slot;                    // workspace slot of part 0 of tile 0 (per KV head; parts > 1)
+};
+
+// What the host knows of a launch.
+struct Plan {
+    int group;
+    int from_rows, to_rows;      // requests of from_rows < packed rows <= to_rows are this kernel's
+    int parts, least;
+    int64_t items;               // at least as many as there are
+};
+
+struct Request {
+    int q0, n, kv, tiles, units;
+};
+
+template <int ROWS, int KEYS>
+__device__ __forceinline__ Request request_of(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& p, int b) {
+    Request r = {0, 0, 0, 0, 0};
+    if (b >= a.num_seqs) return r;
+    r.q0 = min(max(a.q_start[b], 0), a.rows);
+    r.n = max(min(a.q_start[b + 1], a.rows) - r.q0, 0);
+    r.kv = (int)min((int64_t)max(a.kv_lens[b], 0), (int64_t)a.max_blocks * c.page_size);
+    const int rows = r.n * p.group;
+    if (rows <= p.from_rows || rows > p.to_rows) return r;
+    r.tiles = (rows + ROWS - 1) / ROWS;
+    // (a window's first tile of keys is entered in the middle)
+    const int seen = a.window > 0 ? (int)min((int64_t)r.kv, (int64_t)a.window + ROWS / p.group + KEYS) : r.kv;
+    r.units = (seen + KEYS - 1) / KEYS;
+    return r;
+}
+
+__device__ __forceinline__ int wave_scan(int v) {        // inclusive
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            v[2 * k] = half_bits_to_float(w[k] & 0xffffu);
-            v[2 * k + 1] = half_bits_to_float(w[k] >> 16);
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// Item j: the j-th (part, tile) over the requests, or (merge) the j-th tile of
+// more than one part.  False where there is none.  Wave-uniform.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool find_share(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& p, int j,
+                                           bool merge, Share& s) {
+    const int lane = threadIdx.x & 63;
+    const Request first = request_of<ROWS, KEYS>(a, c, p, lane);
+    float total = (float)first.tiles * (float)first.units;
+    for (int b0 = 64; b0 < a.num_seqs; b0 += 64) {
+        const Request r = request_of<ROWS, KEYS>(a, c, p, b0 + lane);
+        total += (float)r.tiles * (float)r.units;
+    }
+    // units a part: total / parts rounded up (1.0001: the sum's own roundings)
+    total = xor_sum64(total) * ((float)c.num_kv_heads * 1.0001f);
+    const int share = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(ceilf(total / (float)p.parts), (float)p.least), 1e9f));
+    int items_before = 0, slots_before = 0;
+    for (int b0 = 0; b0 < a.num_seqs; b0 += 64) {
+        const Request r = b0 == 0 ? first : request_of<ROWS, KEYS>(a, c, p, b0 + lane);
+        const int parts = max((int)(((unsigned)r.units + share - 1) / (unsigned)share), 1);
+        const int items = merge ? (parts > 1 ? r.tiles : 0) : r.tiles * parts;
+        const int slots = parts > 1 ? r.tiles * parts : 0;
+        const int items_end = items_before + wave_scan(items), slots_end = slots_before + wave_scan(slots);
+        const uint64_t past = __ballot(items_end > j);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            auto get = [l](int v) { return __builtin_amdgcn_readlane(v, l); };
+            s.b = b0 + l;
+            s.q0 = get(r.q0);
+            s.n = get(r.n);
+            s.kv = get(r.kv);
+            s.tiles = get(r.tiles);
+            s.parts = get(parts);
+            s.slot = get(slots_end - slots);
+            const int at = j - get(items_end - items);
+            // the tiles of a part one after the other (they share K and V), the longest first
+            s.part = at / s.tiles;
+            s.tile = s.tiles - 1 - (at - s.part * s.tiles);
+            return true;
         }
-    };
-    load8(a.q + r * a.ld_q + (int64_t)h * D + 8 * sub, q);
-    for (int t0 = from; t0 <= p; t0 += W * PW) {
-        const int t = t0 + slot;
-        const int page = t <= p ? table[t / c.page_size] : 0;
-        const bool bad = page < 0 || page >= c.num_pages;
-        const int64_t at = (int64_t)(bad ? 0 : page) * c.page_stride + (t % c.page_size) * c.row_stride +
-                           kvh * c.head_stride + 8 * sub;
-        float k[8] = {}, v[8] = {};
-        if (t <= p) {
-            load8(c.k + at, k);
-            load8(c.v + at, v);
+        items_before = __builtin_amdgcn_readlane(items_end, 63);
+        slots_before = __builtin_amdgcn_readlane(slots_end, 63);
+    }
+    return false;
+}
+
+// Positions of a tile's packed rows [r0, r1]: keys [lo, hi) are seen by some of them.
+struct Span {
+    int first, last;             // positions of the first and the last row
+    int lo, hi;
+};
+__device__ __forceinline__ Span span_of(const Share& s, int r0, int r1, int group, int window) {
+    Span t;
+    t.first = s.kv - s.n + r0 / group;
+    t.last = s.kv - s.n + r1 / group;
+    t.hi = max(t.last + 1, 0);
+    t.lo = window > 0 ? (int)max((int64_t)t.first - window + 1, (int64_t)0) : 0;
+    return t;
+}
+
+// The workspace slot of a part: O [ROWS][D], then m [ROWS], l [ROWS].
+template <int ROWS, int D>
+__device__ __forceinline__ float* slot_of(float* ws, const Share& s, int part, int kvh, int nkv) {
+    const int64_t i = (int64_t)(s.slot + part * s.tiles + s.tile) * nkv + kvh;
+    return ws + i * (ROWS * (D + 2));
+}
+
+__device__ __forceinline__ void store4(const rf_paged_attention& a, int64_t at, f4 v) {
+    if (a.out_f32) {
+        *reinterpret_cast<f4*>(static_cast<float*>(a.out) + at) = v;
+    } else {
+        const uint32_t x = (uint32_t)f16_bits_rn(v[0]) | ((uint32_t)f16_bits_rn(v[1]) << 16);
+        const uint32_t y = (uint32_t)f16_bits_rn(v[2]) | ((uint32_t)f16_bits_rn(v[3]) << 16);
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = u32x2{x, y};
+    }
+}
+
+// Rows of K and V in LDS lie as in memory; a row's 16-byte pieces are permuted
+// so that no read of the MFMA operands meets a bank twice: K's 16 lanes read one
+// piece of 16 rows, V's transposing reads 32 (or 64) bytes of 4 (or 8) rows.
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+template <int D>
+__device__ __forceinline__ int v_swizzle(int row) {
+    return (D == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3)) ^ (2 * ((row >> 2) & 1));
+}
+
+// LDS DMA of a group of rows of one page: its lanes' row and piece.
+template <int D>
+struct Dma {
+    static constexpr int LPR = D / 8, RPI = 64 / LPR;     // lanes a row, rows an instruction
+};
+
+// One LDS read of four keys of one dim: 16 lanes read 4 rows of 32 bytes (lane i
+// row i / 4, 8-byte piece i % 4) and receive dim i's four keys.
+__device__ __forceinline__ h4 read_tr(uint32_t at) {
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at));
+}
+
+__device__ __forceinline__ h8 join(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// Whether any of the values is an infinity or NaN: 0 * x is then not 0.
+struct Finite {
+    h8 acc = {0, 0, 0, 0, 0, 0, 0, 0};
+    __device__ __forceinline__ void take(h8 v) { acc += v * (_Float16)0; }
+    __device__ __forceinline__ bool all() const {
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ok = ok && acc[i] == (_Float16)0;
+        return __ballot(!ok) == 0;
+    }
+};
+__device__ __forceinline__ h8 finite_or_zero(h8 v) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (!(v[i] - v[i] == (_Float16)0)) v[i] = 0;
+    return v;
+}
+
+// ---- few rows -------------------------------------------------------------------------
+//
+// W waves; wave w takes the pieces of 32 positions w, w + W, .. of the part,
+// each through its own S-stage ring in LDS (no barrier in the loop): S^T by
+// 16x16x32 MFMAs, lane (row lane % 16, keys 4 (lane / 16) ..), and O^T alike.
+// The waves' (m, l, O) are joined through LDS at the end.  16 KB of K and V a
+// piece (head_dim 128), 64 KB and more in flight a CU.
+template <int D, int W, int S>
+__global__ __launch_bounds__(64 * W) void rf_paged_attn_narrow_kernel(const rf_paged_attention a, const rf_paged_cache c,
+                                                                      const Plan plan) {
+    constexpr int ROWB = 2 * D, MAT = kNarrowKeys * ROWB, STAGE = 2 * MAT;
+    constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = kNarrowKeys / RPI;   // instructions a matrix
+    constexpr int KS = D / 32, NB = D / 16;
+    constexpr int PADD = D + 4;                          // floats a row of the join
+    static_assert(W * kNarrowRows * (PADD + 2) * 4 <= W * S * STAGE, "the join fits the ring");
+    __shared__ __align__(1024) uint8_t lds[W * S * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const int nkv = c.num_kv_heads, psh = __ffs(c.page_size) - 1, pmask = c.page_size - 1;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    const uint32_t ring = lds0 + (uint32_t)wave * (S * STAGE);
+    const int dr = lane / LPR, ds = lane % LPR;
+
+    for (int64_t item = blockIdx.x; item < plan.items; item += gridDim.x) {
+        Share s;
+        const int kvh = (int)(item % nkv);
+        if (!find_share<kNarrowRows, kNarrowKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
+        const int rows = s.n * plan.group, r0 = kNarrowRows * s.tile;
+        const Span t = span_of(s, r0, min(r0 + kNarrowRows, rows) - 1, plan.group, a.window);
+        // the part's pieces
+        const int p0 = t.lo / kNarrowKeys, p1 = (t.hi + kNarrowKeys - 1) / kNarrowKeys;
+        const int each = (max(p1 - p0, 0) + s.parts - 1) / s.parts;
+        const int begin = p0 + s.part * each, end = min(begin + each, p1);
+        const int steps = max((end - begin - wave + W - 1) / W, 0);
+        // this lane's packed row
+        const int r = r0 + col, token = min(r, rows - 1) / plan.group, head = min(r, rows - 1) - token * plan.group;
+        const int pos = s.kv - s.n + token;
+        const int* table = a.block_tables + (int64_t)s.b * a.max_blocks;
+        const uint16_t* kc = c.k + kvh * c.head_stride;
+        const uint16_t* vc = c.v + kvh * c.head_stride;
+
+        // page ids of 64 / ppp pieces to come, lane (step, page of the piece)
+        const int ppp = c.page_size >= kNarrowKeys ? 1 : kNarrowKeys >> psh, window = 64 / ppp;
+        int ids = 0, ids_step = 0;
+        bool bad = false;
+        auto load_ids = [&](int step) {
+            const int piece = begin + wave + W * (step + lane / ppp);
+            const int page = min(max((piece * kNarrowKeys >> psh) + lane % ppp, t.lo >> psh), (t.hi - 1) >> psh);
+            ids = table[page];
+            const bool out = (unsigned)ids >= (unsigned)c.num_pages;
+            bad = bad || __ballot(out) != 0;
+            ids = out ? 0 : ids;
+            ids_step = step;
+        };
+        auto stage = [&](int step) {
+            if (step >= steps) return;
+            if (step - ids_step >= window) load_ids(step);
+            const int k0 = kNarrowKeys * (begin + wave + W * step);
+            const uint32_t dst = ring + (uint32_t)(step % S) * STAGE;
+            const bool whole = k0 >= t.lo && k0 + kNarrowKeys <= t.hi;
+            // the ring's last readers are done
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                // positions that no row sees are taken from the nearest one that some row sees
+                const int at = whole ? k0 + RPI * i
+                                     : max(min(k0 + RPI * i, (t.hi - 1) & ~(RPI - 1)), t.lo & ~(RPI - 1));
+                const int back = whole ? dr : min(max(at + dr, t.lo), t.hi - 1) - at;
+                const int page = __builtin_amdgcn_readlane(ids, (step - ids_step) * ppp + ((at >> psh) - (k0 >> psh)));
+                const int64_t off = (int64_t)page * c.page_stride + (int64_t)(at & pmask) * c.row_stride;
+                const uint32_t row = (uint32_t)back * (uint32_t)(2 * c.row_stride);
+                const int lr = RPI * i + dr;
+                lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * i), row + 16u * (uint32_t)(ds ^ k_swizzle<D>(lr)),
+                          reinterpret_cast<const uint8_t*>(kc + off));
+                lds_dma16(__builtin_amdgcn_readfirstlane(dst + MAT + 1024u * i),
+                          row + 16u * (uint32_t)(ds ^ v_swizzle<D>(lr)), reinterpret_cast<const uint8_t*>(vc + off));
+            }
+        };
+        h8 q[KS];
+        const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * quad;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const h8*>(qrow + 32 * k);
+        if (steps > 0) load_ids(0);
+        // (q has arrived before the DMAs start, so that none but theirs are counted below)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) stage(i);
+
+        // operand addresses: 4 k + quad = 4 k ^ quad and so on, so one base and an xor each
+        const uint32_t ka = ring + (uint32_t)col * ROWB + 16u * (uint32_t)(quad ^ k_swizzle<D>(col));
+        const int vr = 4 * quad + (col >> 2);
+        const uint32_t va = ring + MAT + (uint32_t)vr * ROWB + 16u * (uint32_t)(((col >> 1) & 1) ^ v_swizzle<D>(vr)) +
+                            8u * (uint32_t)(col & 1);
+
+        const float scale = a.scale * kLog2e;
+        f4 o[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) o[i] = f4{0, 0, 0, 0};
+        float m = kNone, l = 0.0f;
+        for (int step = 0; step < steps; ++step) {
+            stage(step + S - 1);
+            if (step + S <= steps)
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * 2 * NI) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const int k0 = kNarrowKeys * (begin + wave + W * step);
+            const uint32_t at = (uint32_t)(step % S) * STAGE;
+            f4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    x[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(lds_h8)((ka ^ (64u * k)) + at + 16u * b * ROWB), q[k],
+                                                                  x[b], 0, 0, 0);
+            const bool masked = k0 + kNarrowKeys - 1 > t.first || (a.window > 0 && k0 <= t.last - a.window);
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[b][e] *= scale;
+                    if (masked) {
+                        const int key = k0 + 16 * b + 4 * quad + e;
+                        if (key > pos || (a.window > 0 && key <= pos - a.window)) x[b][e] = -INFINITY;
+                    }
+                    top = fmaxf(top, x[b][e]);
+                }
+            top = xor_max<32, 16>(top);
+            if (__ballot(top > m)) {
+                const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) o[i] *= f;
+            }
+            h8 p;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float w = __builtin_amdgcn_exp2f(x[b][e] - m);
+                    l += w;
+                    p[4 * b + e] = (_Float16)w;
+                }
+            // V^T: lane (dim 16 i + col) takes keys 4 quad + {0 .. 3, 16 .. 19}, as p holds them
+            auto v_frag = [&](int i) {
+                const uint32_t v = (va ^ (32u * i)) + at;
+                return join(read_tr(v), read_tr(v + 16u * ROWB));
+            };
+            bool clean = true;
+            if (masked) {
+                Finite fin;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) fin.take(v_frag(i));
+                clean = fin.all();
+                asm volatile("" ::: "memory");   // (read again: kept, they would crowd the registers)
+            }
+            if (clean) {
+#pragma unroll
+                for (int i = 0; i < NB; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_frag(i), p, o[i], 0, 0, 0);
+            } else {
+                // infinities or NaN among values that some rows do not see: they reach the
+                // others by an addition
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(finite_or_zero(v_frag(i)), p, o[i], 0, 0, 0);
+                    for (int j = 0; j < kNarrowKeys; ++j) {
+                        const int key = k0 + j;
+                        if (key > pos || (a.window > 0 && key <= pos - a.window)) continue;
+                        const int piece = 2 * i + (quad >> 1);
+                        const h4 v = *(lds_h4)(ring + at + MAT + (uint32_t)j * ROWB +
+                                               16u * (uint32_t)(piece ^ v_swizzle<D>(j)) + 8u * (uint32_t)(quad & 1));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (!(v[e] - v[e] == (_Float16)0)) o[i][e] += (float)v[e];
+                    }
+                }
+            }
         }
-        float s = 0.0f;
+        l = xor_sum<32, 16>(l);
+        if (bad) l = NAN;
+        // the waves' states
+        float* join_o = reinterpret_cast<float*>(lds);
+        float* join_m = join_o + W * kNarrowRows * PADD;
+        float* join_l = join_m + W * kNarrowRows;
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = __fmaf_rn(q[e], k[e], s);
-        s = xor_sum<LPP / 2, 1>(s) * a.scale;
-        if (bad) s = NAN;
-        if (t <= p) {
-            const float mn = fmaxf(m, s), f = m == mn ? 1.0f : expf(m - mn), w = expf(s - mn);
-            m = mn;
-            l = l * f + w;
+        for (int i = 0; i < NB; ++i)
+            *reinterpret_cast<f4*>(join_o + (wave * kNarrowRows + col) * PADD + 16 * i + 4 * quad) = o[i];
+        if (quad == 0) {
+            join_m[wave * kNarrowRows + col] = m;
+            join_l[wave * kNarrowRows + col] = l;
+        }
+        __syncthreads();
+        const int live = min(rows - r0, kNarrowRows);
+        float* part = slot_of<kNarrowRows, D>(static_cast<float*>(a.workspace), s, s.part, kvh, nkv);
+        for (int i = threadIdx.x; i < live * (D / 4); i += 64 * W) {
+            const int row = i / (D / 4), d = 4 * (i % (D / 4));
+            float mx = kNone, sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = o[e] * f + w * v[e];
+            for (int w = 0; w < W; ++w) mx = fmaxf(mx, join_m[w * kNarrowRows + row]);
+            f4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float f = __builtin_amdgcn_exp2f(join_m[w * kNarrowRows + row] - mx);
+                sum += join_l[w * kNarrowRows + row] * f;
+                acc += *reinterpret_cast<f4*>(join_o + (w * kNarrowRows + row) * PADD + d) * f;
+            }
+            if (s.parts > 1) {
+                *reinterpret_cast<f4*>(part + row * D + d) = acc;
+                if (d == 0) {
+                    part[kNarrowRows * D + row] = mx;
+                    part[kNarrowRows * (D + 1) + row] = sum;
+                }
+            } else {
+                const int tk = (r0 + row) / plan.group, hd = r0 + row - tk * plan.group;
+                store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d,
+                       sum == 0.0f ? f4{0, 0, 0, 0} : acc * (1.0f / sum));
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- pieces of prompt -------------------------------------------------------------------
+//
+// NW waves of 32 packed rows each over tiles of 64 positions, K and V by LDS
+// DMA, double buffered, one barrier a tile: S^T by 32x32x16 MFMAs (two blocks of
+// 32 keys), lane (row lane % 32, keys 8 (e / 4) + 4 (lane / 32) + e % 4).
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4)))
+void rf_paged_attn_wide_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan plan) {
+    constexpr int ROWB = 2 * D, MAT = kWideKeys * ROWB, STAGE = 2 * MAT, ROWS = 32 * NW;
+    constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = kWideKeys / (RPI * NW);   // a wave's instructions a matrix
+    constexpr int KS = D / 16, NB = D / 32;
+    static_assert(NI >= 1, "every wave has rows to fetch");
+    __shared__ __align__(1024) uint8_t lds[2 * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, hi = lane >> 5;
+    const int nkv = c.num_kv_heads, psh = __ffs(c.page_size) - 1, pmask = c.page_size - 1;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    const int dr = lane / LPR, ds = lane % LPR;
+
+    for (int64_t item = blockIdx.x; item < plan.items; item += gridDim.x) {
+        Share s;
+        const int kvh = (int)(item % nkv);
+        if (!find_share<ROWS, kWideKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
+        const int rows = s.n * plan.group, r0 = ROWS * s.tile;
+        const Span t = span_of(s, r0, min(r0 + ROWS, rows) - 1, plan.group, a.window);
+        const int w0 = r0 + 32 * wave;
+        const bool active = w0 < rows;
+        const Span u = span_of(s, min(w0, rows - 1), min(w0 + 32, rows) - 1, plan.group, a.window);
+        const int p0 = t.lo / kWideKeys, p1 = (t.hi + kWideKeys - 1) / kWideKeys;
+        const int each = (max(p1 - p0, 0) + s.parts - 1) / s.parts;
+        const int begin = p0 + s.part * each, end = min(begin + each, p1);
+        const int r = min(w0 + col, rows - 1), token = r / plan.group, head = r - token * plan.group;
+        const int pos = s.kv - s.n + token;
+        const int* table = a.block_tables + (int64_t)s.b * a.max_blocks;
+        const uint16_t* kc = c.k + kvh * c.head_stride;
+        const uint16_t* vc = c.v + kvh * c.head_stride;
+
+        // page ids, 64 at a time (a tile's pages never straddle), the next ones ahead
+        bool bad = false;
+        int ids = 0, next = 0, ids_at = -1;
+        auto load_ids = [&](int at) { return table[min(max(at + lane, t.lo >> psh), (t.hi - 1) >> psh)]; };
+        auto stage = [&](int tile) {
+            const int k0 = kWideKeys * tile, at64 = (k0 >> psh) & ~63;
+            if (at64 != ids_at) {
+                ids = next;
+                const bool out = (unsigned)ids >= (unsigned)c.num_pages;
+                bad = bad || __ballot(out) != 0;
+                ids = out ? 0 : ids;
+                ids_at = at64;
+                next = load_ids(at64 + 64);
+            }
+            const uint32_t dst = lds0 + (uint32_t)(tile & 1) * STAGE;
+            const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int g = NW * i + wave, lr = RPI * g + dr;
+                // positions that no row sees are taken from the nearest one that some row sees
+                const int at = whole ? k0 + RPI * g
+                                     : max(min(k0 + RPI * g, (t.hi - 1) & ~(RPI - 1)), t.lo & ~(RPI - 1));
+                const int back = whole ? dr : min(max(at + dr, t.lo), t.hi - 1) - at;
+                const int page = __builtin_amdgcn_readlane(ids, (at >> psh) - ids_at);
+                const int64_t off = (int64_t)page * c.page_stride + (int64_t)(at & pmask) * c.row_stride;
+                const uint32_t row = (uint32_t)back * (uint32_t)(2 * c.row_stride);
+                lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * g), row + 16u * (uint32_t)(ds ^ k_swizzle<D>(lr)),
+                          reinterpret_cast<const uint8_t*>(kc + off));
+                lds_dma16(__builtin_amdgcn_readfirstlane(dst + MAT + 1024u * g),
+                          row + 16u * (uint32_t)(ds ^ v_swizzle<D>(lr)), reinterpret_cast<const uint8_t*>(vc + off));
+            }
+        };
+        if (begin < end) {
+            next = load_ids((kWideKeys * begin >> psh) & ~63);
+            stage(begin);
+        }
+        // a negative scale moves its sign to Q (exact), so that the largest S has the largest weight
+        const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+        const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+        h8 q[KS];
+        const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * hi;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) q[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qrow + 16 * k) ^ sign);
+        // operand addresses: 2 k + hi = 2 k ^ hi and so on, so one base and an xor each
+        const int i16 = lane & 15, vr = 4 * hi + (i16 >> 2);
+        const uint32_t ka = lds0 + (uint32_t)col * ROWB + 16u * (uint32_t)(hi ^ k_swizzle<D>(col));
+        const uint32_t va = lds0 + MAT + (uint32_t)vr * ROWB +
+                            16u * (uint32_t)((2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ v_swizzle<D>(vr)) +
+                            8u * (uint32_t)(i16 & 1);
+        f16v o[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+        float m = kNone, l = 0.0f;
+        bool far = false;
+
+        for (int tile = begin; tile < end; ++tile) {
+            // this wave's share of the tile has landed; past the barrier everyone's has, and
+            // the other buffer's reads are done
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            lds_barrier();
+            if (tile + 1 < end) stage(tile + 1);
+            const int k0 = kWideKeys * tile;
+            if (!active || k0 > u.last || (a.window > 0 && k0 + kWideKeys - 1 <= u.first - a.window)) continue;
+            const uint32_t at = (uint32_t)(tile & 1) * STAGE;
+            f16v x[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[b][e] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(lds_h8)((ka ^ (32u * k)) + at + 32u * b * ROWB), q[k],
+                                                                  x[b], 0, 0, 0);
+            // V^T (k-step j, dims 32 i ..): lane (dim 32 i + col) takes keys 16 j + 4 hi + {0 .. 3, 8 .. 11}, as
+            // the weights' registers hold them
+            auto v_frag = [&](int j, int i) {
+                const uint32_t v = (va ^ (64u * i)) + at + 16u * j * ROWB;
+                return join(read_tr(v), read_tr(v + 8u * ROWB));
+            };
+            const bool masked = k0 + kWideKeys - 1 > u.first || (a.window > 0 && k0 <= u.last - a.window);
+            if (masked) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = k0 + 32 * b + 8 * (e >> 2) + 4 * hi + (e & 3);
+                        if (key > pos || (a.window > 0 && key <= pos - a.window)) x[b][e] = -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[b][e]);
+            top = xor_max<32, 32>(top) * scale;
+            // exp(x - m) as 2^(x scale - m), one fma: m is a rounded product and the fma's is not, so
+            // a row's weights are off by one common factor of 2^(half a step of m).  Far from zero
+            // (2^7) scores are rounded as m is, lest the factor leave fp16's range.
+            float mul = scale;
+            if (__ballot(top > m) || far) {
+                const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[i][e] *= f;
+                far = __ballot(fabsf(m) >= 128.0f && m != kNone) != 0;
+                if (far) {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[b][e] = __fmul_rn(x[b][e], scale);
+                    mul = 1.0f;
+                }
+            }
+            h8 p[4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], mul, -m));
+                    l += w;
+                    p[2 * b + (e >> 3)][e & 7] = (_Float16)w;
+                }
+            bool clean = true;
+            if (masked) {
+                Finite fin;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) fin.take(v_frag(j, i));
+                clean = fin.all();
+                asm volatile("" ::: "memory");   // (read again: kept, they would crowd the registers)
+            }
+            if (clean) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i)
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(j, i), p[j], o[i], 0, 0, 0);
+            } else {
+                // infinities or NaN among values that some rows do not see: they reach the
+                // others by an addition
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_or_zero(v_frag(j, i)), p[j], o[i], 0, 0, 0);
+                    for (int j = 0; j < kWideKeys; ++j) {
+                        const int key = k0 + j;
+                        if (key > pos || (a.window > 0 && key <= pos - a.window)) continue;
+#pragma unroll
+                        for (int e4 = 0; e4 < 4; ++e4) {
+                            const h4 v = *(lds_h4)(lds0 + at + MAT + (uint32_t)j * ROWB +
+                                                   16u * (uint32_t)((4 * i + e4) ^ v_swizzle<D>(j)) + 8u * (uint32_t)hi);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (!(v[e] - v[e] == (_Float16)0)) o[i][4 * e4 + e] += (float)v[e];
+                        }
+                    }
+                }
+            }
+        }
+        lds_barrier();                           // the last tile's reads are done before another item's DMAs
+        if (active && w0 + col < rows) {
+            l += lane_xor<32>(l);
+            if (bad) l = NAN;
+            if (s.parts > 1) {
+                float* part = slot_of<ROWS, D>(static_cast<float*>(a.workspace), s, s.part, kvh, nkv);
+                const int row = 32 * wave + col;
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int e4 = 0; e4 < 4; ++e4)
+                        *reinterpret_cast<f4*>(part + row * D + 32 * i + 8 * e4 + 4 * hi) =
+                            f4{o[i][4 * e4], o[i][4 * e4 + 1], o[i][4 * e4 + 2], o[i][4 * e4 + 3]};
+                if (hi == 0) {
+                    part[ROWS * D + row] = m;
+                    part[ROWS * (D + 1) + row] = l;
+                }
+            } else {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const int64_t at = (int64_t)(s.q0 + token) * a.ld_out + (int64_t)(kvh * plan.group + head) * D + 4 * hi;
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int e4 = 0; e4 < 4; ++e4)
+                        store4(a, at + 32 * i + 8 * e4,
+                               f4{o[i][4 * e4], o[i][4 * e4 + 1], o[i][4 * e4 + 2], o[i][4 * e4 + 3]} * inv);
+            }
         }
     }
-    float* mine = part[slot];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mine[8 * sub + e] = o[e];
-    if (sub == 0) {
-        mine[D] = m;
-        mine[D + 1] = l;
-    }
-    __syncthreads();
-    for (int d = tid; d < D; d += 256) {
-        float mx = -INFINITY, sum = 0.0f, acc = 0.0f;
-        for (int k = 0; k < W * PW; ++k) mx = fmaxf(mx, part[k][D]);
-        for (int k = 0; k < W * PW; ++k) {
-            const float lk = part[k][D + 1];
-            if (lk == 0.0f) continue;            // nothing seen there
-            const float f = part[k][D] == mx ? 1.0f : expf(part[k][D] - mx);
-            sum += lk * f;
-            acc += part[k][d] * f;
+}
+
+// ---- joining the parts --------------------------------------------------------------------
+
+// 16 rows of a tile of several parts a workgroup.
+template <int D, int ROWS, int KEYS>
+__global__ __launch_bounds__(256) void rf_paged_attn_join_kernel(const rf_paged_attention a, const rf_paged_cache c,
+                                                                 const Plan plan) {
+    constexpr int SUB = ROWS / kMergeRows;
+    const int nkv = c.num_kv_heads;
+    const int item = blockIdx.x / SUB, first = kMergeRows * (blockIdx.x % SUB), kvh = item % nkv;
+    Share s;
+    if (!find_share<ROWS, KEYS>(a, c, plan, item / nkv, true, s)) return;
+    const int rows = s.n * plan.group, r0 = ROWS * s.tile;
+    const int live = min(rows - r0, first + kMergeRows) - first;
+    const int64_t next = (int64_t)s.tiles * nkv * (ROWS * (D + 2));
+    const float* part0 = slot_of<ROWS, D>(static_cast<float*>(a.workspace), s, 0, kvh, nkv);
+    for (int i = threadIdx.x; i < live * (D / 4); i += 256) {
+        const int row = first + i / (D / 4), d = 4 * (i % (D / 4));
+        float mx = kNone, sum = 0.0f;
+        for (int k = 0; k < s.parts; ++k) mx = fmaxf(mx, part0[k * next + ROWS * D + row]);
+        f4 acc = {0, 0, 0, 0};
+        for (int k = 0; k < s.parts; ++k) {
+            const float* p = part0 + k * next;
+            const float f = __builtin_amdgcn_exp2f(p[ROWS * D + row] - mx);
+            sum += p[ROWS * (D + 1) + row] * f;
+            acc += *reinterpret_cast<const f4*>(p + row * D + d) * f;
         }
-        const float res = sum == 0.0f ? 0.0f : acc / sum;
-        if (a.out_f32)
-            static_cast<float*>(a.out)[r * a.ld_out + (int64_t)h * D + d] = res;
-        else
-            static_cast<uint16_t*>(a.out)[r * a.ld_out + (int64_t)h * D + d] = f16_bits_rn(res);
+        const int tk = (r0 + row) / plan.group, hd = r0 + row - tk * plan.group;
+        store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d,
+               sum == 0.0f ? f4{0, 0, 0, 0} : acc * (1.0f / sum));
     }
 }
 
@@ -100,11 +712,46 @@ __global__ __launch_bounds__(256) void rf_paged_attn_rows_kernel(const rf_paged_
 
 // ---- launchers -----------------------------------------------------------------------------
 
+// Bytes of the narrow and the wide parts of a launch.
+static size_t narrow_bytes(int d) { return (size_t)2 * rf::kNarrowParts * rf::kNarrowRows * (d + 2) * sizeof(float); }
+static size_t wide_bytes(int d) { return (size_t)2 * rf::kWideParts * (d == 256 ? 128 : 256) * (d + 2) * sizeof(float); }
+
 extern "C" size_t rf_paged_attention_workspace_bytes(int num_heads, int num_kv_heads, int head_dim) {
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
         (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return 0;
-    return 16;
+    return narrow_bytes(head_dim) + wide_bytes(head_dim);
+}
+
+template <int D, int ROWS, int KEYS, class Kernel>
+static void attn_go(Kernel kernel, int threads, rf_paged_attention a, const rf_paged_cache& c, rf::Plan p,
+                    float* workspace, hipStream_t stream) {
+    a.workspace = workspace;
+    // Items: every tile has a part, and at most p.parts more (each of them is p.parts' share long);
+    // no more either than the table's width gives room for.
+    const int64_t tiles = ((int64_t)a.rows * p.group / ROWS + a.num_seqs) * c.num_kv_heads;
+    const int64_t most = ((int64_t)a.max_blocks * c.page_size + KEYS * p.least - 1) / (KEYS * p.least);
+    p.items = std::min(tiles + p.parts, tiles * std::max<int64_t>(most, 1));
+    const unsigned grid = (unsigned)std::min<int64_t>(p.items, 1 << 20);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, stream, a, c, p);
+    if (most > 1)
+        hipLaunchKernelGGL((rf::rf_paged_attn_join_kernel<D, ROWS, KEYS>),
+                           dim3((unsigned)std::min<int64_t>(tiles, p.parts) * (ROWS / rf::kMergeRows)), dim3(256), 0,
+                           stream, a, c, p);
+}
+
+template <int D, int W, int S, int NW>
+static void attn_dim(const rf_paged_attention& a, const rf_paged_cache& c, hipStream_t stream) {
+    const int group = a.num_heads / c.num_kv_heads;
+    const bool both = (int64_t)a.max_new * group > rf::kNarrowRows;
+    float* ws = static_cast<float*>(a.workspace);
+    rf::Plan p = {group, 0, both ? rf::kNarrowRows : INT_MAX, rf::kNarrowParts, rf::kNarrowLeast, 0};
+    attn_go<D, rf::kNarrowRows, rf::kNarrowKeys>(rf::rf_paged_attn_narrow_kernel<D, W, S>, 64 * W, a, c, p, ws, stream);
+    if (both) {
+        p = {group, rf::kNarrowRows, INT_MAX, rf::kWideParts, rf::kWideLeast, 0};
+        attn_go<D, 32 * NW, rf::kWideKeys>(rf::rf_paged_attn_wide_kernel<D, NW>, 64 * NW, a, c, p,
+                                           ws + narrow_bytes(D) / sizeof(float), stream);
+    }
 }
 
 extern "C" hipError_t rf_paged_attention_launch(const rf_paged_attention* step, const rf_paged_cache* cache,
@@ -114,7 +761,8 @@ extern "C" hipError_t rf_paged_attention_launch(const rf_paged_attention* step, 
     const rf_paged_cache& c = *cache;
     if (!rf::cache_ok(c) || a.num_seqs < 0 || a.rows < 0 || a.rows > (1 << 23) || a.max_blocks < 0 ||
         a.num_heads <= 0 || a.num_heads > 65535 || a.num_heads % c.num_kv_heads != 0 ||
-        a.num_heads / c.num_kv_heads > 64 || a.window < 0 || !std::isfinite(a.scale))
+        a.num_heads / c.num_kv_heads > 64 || a.window < 0 || !std::isfinite(a.scale) ||
+        (int64_t)a.max_blocks * c.page_size > INT_MAX)
         return hipErrorInvalidValue;
     if (a.rows == 0 || a.num_seqs == 0) return hipSuccess;
     const int64_t width = (int64_t)a.num_heads * c.head_dim;
@@ -124,11 +772,10 @@ extern "C" hipError_t rf_paged_attention_launch(const rf_paged_attention* step, 
           reinterpret_cast<uintptr_t>(a.workspace)) & 15u) != 0 ||
         a.workspace_bytes < rf_paged_attention_workspace_bytes(a.num_heads, c.num_kv_heads, c.head_dim))
         return hipErrorInvalidValue;
-    const dim3 grid(a.rows, a.num_heads), blk(256);
     switch (c.head_dim) {
-    case 64: hipLaunchKernelGGL(rf::rf_paged_attn_rows_kernel<64>, grid, blk, 0, stream, a, c); break;
-    case 128: hipLaunchKernelGGL(rf::rf_paged_attn_rows_kernel<128>, grid, blk, 0, stream, a, c); break;
-    default: hipLaunchKernelGGL(rf::rf_paged_attn_rows_kernel<256>, grid, blk, 0, stream, a, c); break;
+    case 64: attn_dim<64, 4, 4, 8>(a, c, stream); break;
+    case 128: attn_dim<128, 4, 2, 8>(a, c, stream); break;
+    default: attn_dim<256, 2, 2, 4>(a, c, stream); break;
     }
     return hipGetLastError();
 }

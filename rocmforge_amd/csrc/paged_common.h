@@ -14,7 +14,7 @@ inline bool cache_ok(const rf_paged_cache& c) {
         return false;
     if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return false;
     if (((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15u) != 0) return false;
-    return c.page_stride > 0 && c.row_stride > 0 && c.head_stride > 0 &&
+    return c.page_stride > 0 && c.row_stride > 0 && c.head_stride > 0 && c.row_stride <= (1 << 26) &&
            ((c.page_stride | c.row_stride | c.head_stride) & 7) == 0;
 }
 

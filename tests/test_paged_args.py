@@ -48,7 +48,7 @@ def refused(fn, *args):
     assert e.value.code == 1
 
 
-BAD_CACHE = [dict(k=None), dict(v=None), dict(k=ODD), dict(v=ODD), dict(page_stride=4100), dict(row_stride=0),
+BAD_CACHE = [dict(k=None), dict(v=None), dict(k=ODD), dict(v=ODD), dict(page_stride=4100), dict(row_stride=0), dict(row_stride=(1 << 26) + 8),
              dict(head_stride=-128), dict(num_pages=0), dict(num_pages=1 << 28), dict(page_size=24), dict(page_size=4),
              dict(page_size=2048), dict(num_kv_heads=0), dict(head_dim=96)]
 
@@ -76,7 +76,7 @@ def test_rotary_steps(rf, bad):
 
 @pytest.mark.parametrize("bad", [{n: None} for n in ("q", "out", "block_tables", "q_start", "kv_lens", "workspace")] + [
     dict(q=ODD), dict(out=ODD), dict(workspace=ODD), dict(ld_q=516), dict(ld_q=504), dict(ld_out=504), dict(rows=-1),
-    dict(rows=(1 << 23) + 1), dict(num_seqs=-1), dict(max_blocks=-1), dict(num_heads=0), dict(num_heads=3),
+    dict(rows=(1 << 23) + 1), dict(num_seqs=-1), dict(max_blocks=-1), dict(max_blocks=1 << 27), dict(num_heads=0), dict(num_heads=3),
     dict(num_heads=256, ld_q=256 * 128, ld_out=256 * 128), dict(window=-1), dict(scale=float("nan")),
     dict(scale=float("inf")), dict(workspace_bytes=0)])
 def test_attentions(rf, bad):
