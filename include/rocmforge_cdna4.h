@@ -774,7 +774,7 @@ hipError_t rf_paged_rope_write_launch(const rf_paged_rope* step, const rf_paged_
  * (rounded once from fp32) or fp32 (out_f32 != 0) [row][ld_out].  The weights are
  * rounded to fp16 before they meet V; scores, maxima, sums and outputs are held
  * in fp32.  max_new is a hint, the largest n of the step, that picks the
- * kernels; results hold for any.  kv_lens beyond max_blocks * page_size (< 2^31) are
+ * kernels; results hold for any.  kv_lens beyond max_blocks * page_size (<= 2^30) are
  * clipped, q_start beyond rows too; rows of a request whose table names a page
  * outside [0, num_pages) in the positions that it sees may get NaN, and nothing
  * outside the cache is read.  workspace: rf_paged_attention_workspace_bytes

@@ -1897,15 +1897,6 @@ constexpr uint32_t kAttRow = 2 * kAttD;          // bytes of a K / V row in LDS
 constexpr uint32_t kAttTile = 64 * kAttRow;      // one 64-key tile of K or of V
 constexpr float kAttFar = 128.0f;                // |m| from which scores are rounded before the exp
 
-// fmaxf of values that are no signalling NaNs, as one instruction: where the compiler
-// cannot know that, it quiets both operands first, a serial chain between the scores
-// and their exps (32 / 8 heads, 4096 positions 150.3 / 149.6 us, 8192 563 / 558).
-__device__ __forceinline__ float max_raw(float a, float b) {
-    float r;
-    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-
 // NW waves as NW / KS units times KS key groups: group g takes the tiles
 // t % KS == g and the groups' partial (m, l, O) are merged through LDS (more
 // waves and a shorter walk per unit when the units are few).  VE: the V

@@ -209,11 +209,10 @@ struct Finite {
         return __ballot(!ok) == 0;
     }
 };
-__device__ __forceinline__ h8 finite_or_zero(h8 v) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (!(v[i] - v[i] == (_Float16)0)) v[i] = 0;
-    return v;
+// The value, or a finite one in the place of an infinity or NaN.
+__device__ __forceinline__ h8 finite_of(h8 v) {
+    const h8 most = (h8)(_Float16)65504.0f;
+    return __builtin_elementwise_min(__builtin_elementwise_max(v, -most), most);
 }
 
 // ---- few rows -------------------------------------------------------------------------
@@ -239,204 +238,201 @@ __global__ __launch_bounds__(64 * W) void rf_paged_attn_narrow_kernel(const rf_p
     const uint32_t ring = lds0 + (uint32_t)wave * (S * STAGE);
     const int dr = lane / LPR, ds = lane % LPR;
 
-    for (int64_t item = blockIdx.x; item < plan.items; item += gridDim.x) {
-        Share s;
-        const int kvh = (int)(item % nkv);
-        if (!find_share<kNarrowRows, kNarrowKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
-        const int rows = s.n * plan.group, r0 = kNarrowRows * s.tile;
-        const Span t = span_of(s, r0, min(r0 + kNarrowRows, rows) - 1, plan.group, a.window);
-        // the part's pieces
-        const int p0 = t.lo / kNarrowKeys, p1 = (t.hi + kNarrowKeys - 1) / kNarrowKeys;
-        const int each = (max(p1 - p0, 0) + s.parts - 1) / s.parts;
-        const int begin = p0 + s.part * each, end = min(begin + each, p1);
-        const int steps = max((end - begin - wave + W - 1) / W, 0);
-        // this lane's packed row
-        const int r = r0 + col, token = min(r, rows - 1) / plan.group, head = min(r, rows - 1) - token * plan.group;
-        const int pos = s.kv - s.n + token;
-        const int* table = a.block_tables + (int64_t)s.b * a.max_blocks;
-        const uint16_t* kc = c.k + kvh * c.head_stride;
-        const uint16_t* vc = c.v + kvh * c.head_stride;
+    const int64_t item = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+    Share s;
+    const int kvh = (int)(item % nkv);
+    if (!find_share<kNarrowRows, kNarrowKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
+    const int rows = s.n * plan.group, r0 = kNarrowRows * s.tile;
+    const Span t = span_of(s, r0, min(r0 + kNarrowRows, rows) - 1, plan.group, a.window);
+    // the part's pieces
+    const int p0 = t.lo / kNarrowKeys, p1 = (t.hi + kNarrowKeys - 1) / kNarrowKeys;
+    const int each = (max(p1 - p0, 0) + s.parts - 1) / s.parts;
+    const int begin = p0 + s.part * each, end = min(begin + each, p1);
+    const int steps = max((end - begin - wave + W - 1) / W, 0);
+    // this lane's packed row
+    const int r = r0 + col, token = min(r, rows - 1) / plan.group, head = min(r, rows - 1) - token * plan.group;
+    const int pos = s.kv - s.n + token;
+    const int* table = a.block_tables + (int64_t)s.b * a.max_blocks;
+    const uint16_t* kc = c.k + kvh * c.head_stride;
+    const uint16_t* vc = c.v + kvh * c.head_stride;
 
-        // page ids of 64 / ppp pieces to come, lane (step, page of the piece)
-        const int ppp = c.page_size >= kNarrowKeys ? 1 : kNarrowKeys >> psh, window = 64 / ppp;
-        int ids = 0, ids_step = 0;
-        bool bad = false;
-        auto load_ids = [&](int step) {
-            const int piece = begin + wave + W * (step + lane / ppp);
-            const int page = min(max((piece * kNarrowKeys >> psh) + lane % ppp, t.lo >> psh), (t.hi - 1) >> psh);
-            ids = table[page];
-            const bool out = (unsigned)ids >= (unsigned)c.num_pages;
-            bad = bad || __ballot(out) != 0;
-            ids = out ? 0 : ids;
-            ids_step = step;
-        };
-        auto stage = [&](int step) {
-            if (step >= steps) return;
-            if (step - ids_step >= window) load_ids(step);
-            const int k0 = kNarrowKeys * (begin + wave + W * step);
-            const uint32_t dst = ring + (uint32_t)(step % S) * STAGE;
-            const bool whole = k0 >= t.lo && k0 + kNarrowKeys <= t.hi;
-            // the ring's last readers are done
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // page ids of 64 / ppp pieces to come, lane (step, page of the piece)
+    const int ppp = c.page_size >= kNarrowKeys ? 1 : kNarrowKeys >> psh, window = 64 / ppp;
+    int ids = 0, ids_step = 0;
+    bool bad = false;
+    auto load_ids = [&](int step) {
+        const int piece = begin + wave + W * (step + lane / ppp);
+        const int page = min(max((piece * kNarrowKeys >> psh) + lane % ppp, t.lo >> psh), (t.hi - 1) >> psh);
+        ids = table[page];
+        const bool out = (unsigned)ids >= (unsigned)c.num_pages;
+        bad = bad || __ballot(out) != 0;
+        ids = out ? 0 : ids;
+        ids_step = step;
+    };
+    auto stage = [&](int step) {
+        if (step >= steps) return;
+        if (step - ids_step >= window) load_ids(step);
+        const int k0 = kNarrowKeys * (begin + wave + W * step);
+        const uint32_t dst = ring + (uint32_t)(step % S) * STAGE;
+        const bool whole = k0 >= t.lo && k0 + kNarrowKeys <= t.hi;
+        // the ring's last readers are done
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                // positions that no row sees are taken from the nearest one that some row sees
-                const int at = whole ? k0 + RPI * i
-                                     : max(min(k0 + RPI * i, (t.hi - 1) & ~(RPI - 1)), t.lo & ~(RPI - 1));
-                const int back = whole ? dr : min(max(at + dr, t.lo), t.hi - 1) - at;
-                const int page = __builtin_amdgcn_readlane(ids, (step - ids_step) * ppp + ((at >> psh) - (k0 >> psh)));
-                const int64_t off = (int64_t)page * c.page_stride + (int64_t)(at & pmask) * c.row_stride;
-                const uint32_t row = (uint32_t)back * (uint32_t)(2 * c.row_stride);
-                const int lr = RPI * i + dr;
-                lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * i), row + 16u * (uint32_t)(ds ^ k_swizzle<D>(lr)),
-                          reinterpret_cast<const uint8_t*>(kc + off));
-                lds_dma16(__builtin_amdgcn_readfirstlane(dst + MAT + 1024u * i),
-                          row + 16u * (uint32_t)(ds ^ v_swizzle<D>(lr)), reinterpret_cast<const uint8_t*>(vc + off));
-            }
-        };
-        h8 q[KS];
-        const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * quad;
+        for (int i = 0; i < NI; ++i) {
+            // positions that no row sees are taken from the nearest one that some row sees
+            const int at = whole ? k0 + RPI * i
+                                 : max(min(k0 + RPI * i, (t.hi - 1) & ~(RPI - 1)), t.lo & ~(RPI - 1));
+            const int back = whole ? dr : min(max(at + dr, t.lo), t.hi - 1) - at;
+            const int page = __builtin_amdgcn_readlane(ids, (step - ids_step) * ppp + ((at >> psh) - (k0 >> psh)));
+            const int64_t off = (int64_t)page * c.page_stride + (int64_t)(at & pmask) * c.row_stride;
+            const uint32_t row = (uint32_t)back * (uint32_t)(2 * c.row_stride);
+            const int lr = RPI * i + dr;
+            lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * i), row + 16u * (uint32_t)(ds ^ k_swizzle<D>(lr)),
+                      reinterpret_cast<const uint8_t*>(kc + off));
+            lds_dma16(__builtin_amdgcn_readfirstlane(dst + MAT + 1024u * i),
+                      row + 16u * (uint32_t)(ds ^ v_swizzle<D>(lr)), reinterpret_cast<const uint8_t*>(vc + off));
+        }
+    };
+    h8 q[KS];
+    const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * quad;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const h8*>(qrow + 32 * k);
-        if (steps > 0) load_ids(0);
-        // (q has arrived before the DMAs start, so that none but theirs are counted below)
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const h8*>(qrow + 32 * k);
+    if (steps > 0) load_ids(0);
+    // (q has arrived before the DMAs start, so that none but theirs are counted below)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < S - 1; ++i) stage(i);
+    for (int i = 0; i < S - 1; ++i) stage(i);
 
-        // operand addresses: 4 k + quad = 4 k ^ quad and so on, so one base and an xor each
-        const uint32_t ka = ring + (uint32_t)col * ROWB + 16u * (uint32_t)(quad ^ k_swizzle<D>(col));
-        const int vr = 4 * quad + (col >> 2);
-        const uint32_t va = ring + MAT + (uint32_t)vr * ROWB + 16u * (uint32_t)(((col >> 1) & 1) ^ v_swizzle<D>(vr)) +
-                            8u * (uint32_t)(col & 1);
+    // operand addresses: 4 k + quad = 4 k ^ quad and so on, so one base and an xor each
+    const uint32_t ka = ring + (uint32_t)col * ROWB + 16u * (uint32_t)(quad ^ k_swizzle<D>(col));
+    const int vr = 4 * quad + (col >> 2);
+    const uint32_t va = ring + MAT + (uint32_t)vr * ROWB + 16u * (uint32_t)(((col >> 1) & 1) ^ v_swizzle<D>(vr)) +
+                        8u * (uint32_t)(col & 1);
 
-        const float scale = a.scale * kLog2e;
-        f4 o[NB];
+    const float scale = a.scale * kLog2e;
+    f4 o[NB];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) o[i] = f4{0, 0, 0, 0};
-        float m = kNone, l = 0.0f;
-        for (int step = 0; step < steps; ++step) {
-            stage(step + S - 1);
-            if (step + S <= steps)
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * 2 * NI) : "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            const int k0 = kNarrowKeys * (begin + wave + W * step);
-            const uint32_t at = (uint32_t)(step % S) * STAGE;
-            f4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    for (int i = 0; i < NB; ++i) o[i] = f4{0, 0, 0, 0};
+    float m = kNone, l = 0.0f;
+    for (int step = 0; step < steps; ++step) {
+        stage(step + S - 1);
+        if (step + S <= steps)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * 2 * NI) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const int k0 = kNarrowKeys * (begin + wave + W * step);
+        const uint32_t at = (uint32_t)(step % S) * STAGE;
+        // (opaque, so that a piece's addresses are not kept in registers over the loop)
+        uint32_t kt = ka + at, vt = va + at;
+        asm("" : "+v"(kt), "+v"(vt));
+        f4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-                    x[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(lds_h8)((ka ^ (64u * k)) + at + 16u * b * ROWB), q[k],
-                                                                  x[b], 0, 0, 0);
-            const bool masked = k0 + kNarrowKeys - 1 > t.first || (a.window > 0 && k0 <= t.last - a.window);
-            float top = -INFINITY;
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int b = 0; b < 2; ++b)
+                x[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(lds_h8)((kt ^ (64u * k)) + 16u * b * ROWB), q[k],
+                                                              x[b], 0, 0, 0);
+        const bool masked = k0 + kNarrowKeys - 1 > t.first || (a.window > 0 && k0 <= t.last - a.window);
+        const int ahead = pos - k0 - 4 * quad, behind = a.window > 0 ? ahead - a.window : INT_MIN;
+        float top = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[b][e] *= scale;
-                    if (masked) {
-                        const int key = k0 + 16 * b + 4 * quad + e;
-                        if (key > pos || (a.window > 0 && key <= pos - a.window)) x[b][e] = -INFINITY;
-                    }
-                    top = fmaxf(top, x[b][e]);
-                }
-            top = xor_max<32, 16>(top);
-            if (__ballot(top > m)) {
-                const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= f;
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < NB; ++i) o[i] *= f;
+            for (int e = 0; e < 4; ++e) {
+                x[b][e] *= scale;
+                if (masked && (16 * b + e > ahead || 16 * b + e <= behind)) x[b][e] = -INFINITY;
+                top = fmaxf(top, x[b][e]);
             }
-            h8 p;
+        top = xor_butterfly<32, 16>(top, max_raw);
+        if (__ballot(top > m)) {
+            const float mn = max_raw(m, top), f = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int i = 0; i < NB; ++i) o[i] *= f;
+        }
+        h8 p;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float w = __builtin_amdgcn_exp2f(x[b][e] - m);
-                    l += w;
-                    p[4 * b + e] = (_Float16)w;
-                }
-            // V^T: lane (dim 16 i + col) takes keys 4 quad + {0 .. 3, 16 .. 19}, as p holds them
-            auto v_frag = [&](int i) {
-                const uint32_t v = (va ^ (32u * i)) + at;
-                return join(read_tr(v), read_tr(v + 16u * ROWB));
-            };
-            bool clean = true;
-            if (masked) {
-                Finite fin;
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < NB; ++i) fin.take(v_frag(i));
-                clean = fin.all();
-                asm volatile("" ::: "memory");   // (read again: kept, they would crowd the registers)
+            for (int e = 0; e < 4; ++e) {
+                const float w = __builtin_amdgcn_exp2f(x[b][e] - m);
+                l += w;
+                p[4 * b + e] = (_Float16)w;
             }
-            if (clean) {
+        // V^T: lane (dim 16 i + col) takes keys 4 quad + {0 .. 3, 16 .. 19}, as p holds them
+        auto v_frag = [&](int i) {
+            const uint32_t v = vt ^ (32u * i);
+            return join(read_tr(v), read_tr(v + 16u * ROWB));
+        };
+        if (!masked) {
 #pragma unroll
-                for (int i = 0; i < NB; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_frag(i), p, o[i], 0, 0, 0);
-            } else {
-                // infinities or NaN among values that some rows do not see: they reach the
-                // others by an addition
+            for (int i = 0; i < NB; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_frag(i), p, o[i], 0, 0, 0);
+            continue;
+        }
+        // infinities and NaN among values that some rows do not see must not meet their zero
+        // weights: finite ones take their place, and the rows that see them get them by an addition
+        Finite fin;
 #pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(finite_or_zero(v_frag(i)), p, o[i], 0, 0, 0);
-                    for (int j = 0; j < kNarrowKeys; ++j) {
-                        const int key = k0 + j;
-                        if (key > pos || (a.window > 0 && key <= pos - a.window)) continue;
-                        const int piece = 2 * i + (quad >> 1);
-                        const h4 v = *(lds_h4)(ring + at + MAT + (uint32_t)j * ROWB +
-                                               16u * (uint32_t)(piece ^ v_swizzle<D>(j)) + 8u * (uint32_t)(quad & 1));
+        for (int i = 0; i < NB; ++i) {
+            const h8 v = v_frag(i);
+            fin.take(v);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(finite_of(v), p, o[i], 0, 0, 0);
+        }
+        if (fin.all()) continue;
+#pragma unroll 1
+        for (int j = 0; j < kNarrowKeys; ++j) {
+            if (k0 + j > pos || (a.window > 0 && k0 + j <= pos - a.window)) continue;
+            const uint32_t row = ring + at + MAT + (uint32_t)j * ROWB + 8u * (uint32_t)(quad & 1);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!(v[e] - v[e] == (_Float16)0)) o[i][e] += (float)v[e];
-                    }
-                }
+            for (int i = 0; i < NB; ++i) {
+                const h4 v = *(lds_h4)(row + 16u * (uint32_t)((2 * i + (quad >> 1)) ^ v_swizzle<D>(j)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!(v[e] - v[e] == (_Float16)0)) o[i][e] += (float)v[e];
             }
         }
-        l = xor_sum<32, 16>(l);
-        if (bad) l = NAN;
-        // the waves' states
-        float* join_o = reinterpret_cast<float*>(lds);
-        float* join_m = join_o + W * kNarrowRows * PADD;
-        float* join_l = join_m + W * kNarrowRows;
-        __syncthreads();
+    }
+    l = xor_sum<32, 16>(l);
+    if (bad) l = NAN;
+    // the waves' states
+    float* join_o = reinterpret_cast<float*>(lds);
+    float* join_m = join_o + W * kNarrowRows * PADD;
+    float* join_l = join_m + W * kNarrowRows;
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
-            *reinterpret_cast<f4*>(join_o + (wave * kNarrowRows + col) * PADD + 16 * i + 4 * quad) = o[i];
-        if (quad == 0) {
-            join_m[wave * kNarrowRows + col] = m;
-            join_l[wave * kNarrowRows + col] = l;
+    for (int i = 0; i < NB; ++i)
+        *reinterpret_cast<f4*>(join_o + (wave * kNarrowRows + col) * PADD + 16 * i + 4 * quad) = o[i];
+    if (quad == 0) {
+        join_m[wave * kNarrowRows + col] = m;
+        join_l[wave * kNarrowRows + col] = l;
+    }
+    __syncthreads();
+    const int live = min(rows - r0, kNarrowRows);
+    float* part = slot_of<kNarrowRows, D>(static_cast<float*>(a.workspace), s, s.part, kvh, nkv);
+    for (int i = threadIdx.x; i < live * (D / 4); i += 64 * W) {
+        const int row = i / (D / 4), d = 4 * (i % (D / 4));
+        float mx = kNone, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) mx = fmaxf(mx, join_m[w * kNarrowRows + row]);
+        f4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = __builtin_amdgcn_exp2f(join_m[w * kNarrowRows + row] - mx);
+            sum += join_l[w * kNarrowRows + row] * f;
+            acc += *reinterpret_cast<f4*>(join_o + (w * kNarrowRows + row) * PADD + d) * f;
         }
-        __syncthreads();
-        const int live = min(rows - r0, kNarrowRows);
-        float* part = slot_of<kNarrowRows, D>(static_cast<float*>(a.workspace), s, s.part, kvh, nkv);
-        for (int i = threadIdx.x; i < live * (D / 4); i += 64 * W) {
-            const int row = i / (D / 4), d = 4 * (i % (D / 4));
-            float mx = kNone, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) mx = fmaxf(mx, join_m[w * kNarrowRows + row]);
-            f4 acc = {0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float f = __builtin_amdgcn_exp2f(join_m[w * kNarrowRows + row] - mx);
-                sum += join_l[w * kNarrowRows + row] * f;
-                acc += *reinterpret_cast<f4*>(join_o + (w * kNarrowRows + row) * PADD + d) * f;
+        if (s.parts > 1) {
+            *reinterpret_cast<f4*>(part + row * D + d) = acc;
+            if (d == 0) {
+                part[kNarrowRows * D + row] = mx;
+                part[kNarrowRows * (D + 1) + row] = sum;
             }
-            if (s.parts > 1) {
-                *reinterpret_cast<f4*>(part + row * D + d) = acc;
-                if (d == 0) {
-                    part[kNarrowRows * D + row] = mx;
-                    part[kNarrowRows * (D + 1) + row] = sum;
-                }
-            } else {
-                const int tk = (r0 + row) / plan.group, hd = r0 + row - tk * plan.group;
-                store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d,
-                       sum == 0.0f ? f4{0, 0, 0, 0} : acc * (1.0f / sum));
-            }
+        } else {
+            const int tk = (r0 + row) / plan.group, hd = r0 + row - tk * plan.group;
+            store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d,
+                   sum == 0.0f ? f4{0, 0, 0, 0} : acc * (1.0f / sum));
         }
-        __syncthreads();
     }
 }
 
@@ -459,219 +455,217 @@ void rf_paged_attn_wide_kernel(const rf_paged_attention a, const rf_paged_cache 
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     const int dr = lane / LPR, ds = lane % LPR;
 
-    for (int64_t item = blockIdx.x; item < plan.items; item += gridDim.x) {
-        Share s;
-        const int kvh = (int)(item % nkv);
-        if (!find_share<ROWS, kWideKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
-        const int rows = s.n * plan.group, r0 = ROWS * s.tile;
-        const Span t = span_of(s, r0, min(r0 + ROWS, rows) - 1, plan.group, a.window);
-        const int w0 = r0 + 32 * wave;
-        const bool active = w0 < rows;
-        const Span u = span_of(s, min(w0, rows - 1), min(w0 + 32, rows) - 1, plan.group, a.window);
-        const int p0 = t.lo / kWideKeys, p1 = (t.hi + kWideKeys - 1) / kWideKeys;
-        const int each = (max(p1 - p0, 0) + s.parts - 1) / s.parts;
-        const int begin = p0 + s.part * each, end = min(begin + each, p1);
-        const int r = min(w0 + col, rows - 1), token = r / plan.group, head = r - token * plan.group;
-        const int pos = s.kv - s.n + token;
-        const int* table = a.block_tables + (int64_t)s.b * a.max_blocks;
-        const uint16_t* kc = c.k + kvh * c.head_stride;
-        const uint16_t* vc = c.v + kvh * c.head_stride;
+    const int64_t item = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+    Share s;
+    const int kvh = (int)(item % nkv);
+    if (!find_share<ROWS, kWideKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
+    const int rows = s.n * plan.group, r0 = ROWS * s.tile;
+    const Span t = span_of(s, r0, min(r0 + ROWS, rows) - 1, plan.group, a.window);
+    const int w0 = r0 + 32 * wave;
+    const bool active = w0 < rows;
+    const Span u = span_of(s, min(w0, rows - 1), min(w0 + 32, rows) - 1, plan.group, a.window);
+    const int p0 = t.lo / kWideKeys, p1 = (t.hi + kWideKeys - 1) / kWideKeys;
+    const int each = (max(p1 - p0, 0) + s.parts - 1) / s.parts;
+    const int begin = p0 + s.part * each, end = min(begin + each, p1);
+    const int r = min(w0 + col, rows - 1), token = r / plan.group, head = r - token * plan.group;
+    const int pos = s.kv - s.n + token;
+    const int* table = a.block_tables + (int64_t)s.b * a.max_blocks;
+    const uint16_t* kc = c.k + kvh * c.head_stride;
+    const uint16_t* vc = c.v + kvh * c.head_stride;
 
-        // page ids, 64 at a time (a tile's pages never straddle), the next ones ahead
-        bool bad = false;
-        int ids = 0, next = 0, ids_at = -1;
-        auto load_ids = [&](int at) { return table[min(max(at + lane, t.lo >> psh), (t.hi - 1) >> psh)]; };
-        auto stage = [&](int tile) {
-            const int k0 = kWideKeys * tile, at64 = (k0 >> psh) & ~63;
-            if (at64 != ids_at) {
-                ids = next;
-                const bool out = (unsigned)ids >= (unsigned)c.num_pages;
-                bad = bad || __ballot(out) != 0;
-                ids = out ? 0 : ids;
-                ids_at = at64;
-                next = load_ids(at64 + 64);
-            }
-            const uint32_t dst = lds0 + (uint32_t)(tile & 1) * STAGE;
-            const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int g = NW * i + wave, lr = RPI * g + dr;
-                // positions that no row sees are taken from the nearest one that some row sees
-                const int at = whole ? k0 + RPI * g
-                                     : max(min(k0 + RPI * g, (t.hi - 1) & ~(RPI - 1)), t.lo & ~(RPI - 1));
-                const int back = whole ? dr : min(max(at + dr, t.lo), t.hi - 1) - at;
-                const int page = __builtin_amdgcn_readlane(ids, (at >> psh) - ids_at);
-                const int64_t off = (int64_t)page * c.page_stride + (int64_t)(at & pmask) * c.row_stride;
-                const uint32_t row = (uint32_t)back * (uint32_t)(2 * c.row_stride);
-                lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * g), row + 16u * (uint32_t)(ds ^ k_swizzle<D>(lr)),
-                          reinterpret_cast<const uint8_t*>(kc + off));
-                lds_dma16(__builtin_amdgcn_readfirstlane(dst + MAT + 1024u * g),
-                          row + 16u * (uint32_t)(ds ^ v_swizzle<D>(lr)), reinterpret_cast<const uint8_t*>(vc + off));
-            }
-        };
-        if (begin < end) {
-            next = load_ids((kWideKeys * begin >> psh) & ~63);
-            stage(begin);
+    // page ids, 64 at a time (a tile's pages never straddle), the next ones ahead
+    bool bad = false;
+    int ids = 0, next = 0, ids_at = -1;
+    auto load_ids = [&](int at) { return table[min(max(at + lane, t.lo >> psh), (t.hi - 1) >> psh)]; };
+    auto stage = [&](int tile) {
+        const int k0 = kWideKeys * tile, at64 = (k0 >> psh) & ~63;
+        if (at64 != ids_at) {
+            ids = next;
+            const bool out = (unsigned)ids >= (unsigned)c.num_pages;
+            bad = bad || __ballot(out) != 0;
+            ids = out ? 0 : ids;
+            ids_at = at64;
+            next = load_ids(at64 + 64);
         }
-        // a negative scale moves its sign to Q (exact), so that the largest S has the largest weight
-        const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
-        const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
-        h8 q[KS];
-        const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * hi;
+        const uint32_t dst = lds0 + (uint32_t)(tile & 1) * STAGE;
+        const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) q[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qrow + 16 * k) ^ sign);
-        // operand addresses: 2 k + hi = 2 k ^ hi and so on, so one base and an xor each
-        const int i16 = lane & 15, vr = 4 * hi + (i16 >> 2);
-        const uint32_t ka = lds0 + (uint32_t)col * ROWB + 16u * (uint32_t)(hi ^ k_swizzle<D>(col));
-        const uint32_t va = lds0 + MAT + (uint32_t)vr * ROWB +
-                            16u * (uint32_t)((2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ v_swizzle<D>(vr)) +
-                            8u * (uint32_t)(i16 & 1);
-        f16v o[NB];
+        for (int i = 0; i < NI; ++i) {
+            const int g = NW * i + wave, lr = RPI * g + dr;
+            // positions that no row sees are taken from the nearest one that some row sees
+            const int at = whole ? k0 + RPI * g
+                                 : max(min(k0 + RPI * g, (t.hi - 1) & ~(RPI - 1)), t.lo & ~(RPI - 1));
+            const int back = whole ? dr : min(max(at + dr, t.lo), t.hi - 1) - at;
+            const int page = __builtin_amdgcn_readlane(ids, (at >> psh) - ids_at);
+            const int64_t off = (int64_t)page * c.page_stride + (int64_t)(at & pmask) * c.row_stride;
+            const uint32_t row = (uint32_t)back * (uint32_t)(2 * c.row_stride);
+            lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * g), row + 16u * (uint32_t)(ds ^ k_swizzle<D>(lr)),
+                      reinterpret_cast<const uint8_t*>(kc + off));
+            lds_dma16(__builtin_amdgcn_readfirstlane(dst + MAT + 1024u * g),
+                      row + 16u * (uint32_t)(ds ^ v_swizzle<D>(lr)), reinterpret_cast<const uint8_t*>(vc + off));
+        }
+    };
+    if (begin < end) {
+        next = load_ids((kWideKeys * begin >> psh) & ~63);
+        stage(begin);
+    }
+    // a negative scale moves its sign to Q (exact), so that the largest S has the largest weight
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+    h8 q[KS];
+    const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * hi;
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+    for (int k = 0; k < KS; ++k) q[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qrow + 16 * k) ^ sign);
+    // operand addresses: 2 k + hi = 2 k ^ hi and so on, so one base and an xor each
+    const int i16 = lane & 15, vr = 4 * hi + (i16 >> 2);
+    const uint32_t ka = lds0 + (uint32_t)col * ROWB + 16u * (uint32_t)(hi ^ k_swizzle<D>(col));
+    const uint32_t va = lds0 + MAT + (uint32_t)vr * ROWB +
+                        16u * (uint32_t)((2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ v_swizzle<D>(vr)) +
+                        8u * (uint32_t)(i16 & 1);
+    f16v o[NB];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
-        float m = kNone, l = 0.0f;
-        bool far = false;
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+    float m = kNone, l = 0.0f;
+    bool far = false;
 
-        for (int tile = begin; tile < end; ++tile) {
-            // this wave's share of the tile has landed; past the barrier everyone's has, and
-            // the other buffer's reads are done
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            lds_barrier();
-            if (tile + 1 < end) stage(tile + 1);
-            const int k0 = kWideKeys * tile;
-            if (!active || k0 > u.last || (a.window > 0 && k0 + kWideKeys - 1 <= u.first - a.window)) continue;
-            const uint32_t at = (uint32_t)(tile & 1) * STAGE;
-            f16v x[2];
+    for (int tile = begin; tile < end; ++tile) {
+        // this wave's share of the tile has landed; past the barrier everyone's has, and
+        // the other buffer's reads are done
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();
+        if (tile + 1 < end) stage(tile + 1);
+        const int k0 = kWideKeys * tile;
+        if (!active || k0 > u.last || (a.window > 0 && k0 + kWideKeys - 1 <= u.first - a.window)) continue;
+        const uint32_t at = (uint32_t)(tile & 1) * STAGE;
+        // (opaque, so that a tile's addresses are not kept in registers over the loop)
+        uint32_t kt = ka + at, vt = va + at;
+        asm("" : "+v"(kt), "+v"(vt));
+        f16v x[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[b][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[b][e] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-                    x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(lds_h8)((ka ^ (32u * k)) + at + 32u * b * ROWB), q[k],
-                                                                  x[b], 0, 0, 0);
-            // V^T (k-step j, dims 32 i ..): lane (dim 32 i + col) takes keys 16 j + 4 hi + {0 .. 3, 8 .. 11}, as
-            // the weights' registers hold them
-            auto v_frag = [&](int j, int i) {
-                const uint32_t v = (va ^ (64u * i)) + at + 16u * j * ROWB;
-                return join(read_tr(v), read_tr(v + 8u * ROWB));
-            };
-            const bool masked = k0 + kWideKeys - 1 > u.first || (a.window > 0 && k0 <= u.last - a.window);
-            if (masked) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = k0 + 32 * b + 8 * (e >> 2) + 4 * hi + (e & 3);
-                        if (key > pos || (a.window > 0 && key <= pos - a.window)) x[b][e] = -INFINITY;
-                    }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[b][e]);
-            top = xor_max<32, 32>(top) * scale;
-            // exp(x - m) as 2^(x scale - m), one fma: m is a rounded product and the fma's is not, so
-            // a row's weights are off by one common factor of 2^(half a step of m).  Far from zero
-            // (2^7) scores are rounded as m is, lest the factor leave fp16's range.
-            float mul = scale;
-            if (__ballot(top > m) || far) {
-                const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= f;
-#pragma unroll
-                for (int i = 0; i < NB; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[i][e] *= f;
-                far = __ballot(fabsf(m) >= 128.0f && m != kNone) != 0;
-                if (far) {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) x[b][e] = __fmul_rn(x[b][e], scale);
-                    mul = 1.0f;
-                }
-            }
-            h8 p[4];
+                x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(lds_h8)((kt ^ (32u * k)) + 32u * b * ROWB), q[k],
+                                                              x[b], 0, 0, 0);
+        // V^T (k-step j, dims 32 i ..): lane (dim 32 i + col) takes keys 16 j + 4 hi + {0 .. 3, 8 .. 11}, as
+        // the weights' registers hold them
+        auto v_frag = [&](int j, int i) {
+            const uint32_t v = (vt ^ (64u * i)) + 16u * j * ROWB;
+            return join(read_tr(v), read_tr(v + 8u * ROWB));
+        };
+        const bool masked = k0 + kWideKeys - 1 > u.first || (a.window > 0 && k0 <= u.last - a.window);
+        if (masked) {
+            const int ahead = pos - k0 - 4 * hi, behind = a.window > 0 ? ahead - a.window : INT_MIN;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], mul, -m));
-                    l += w;
-                    p[2 * b + (e >> 3)][e & 7] = (_Float16)w;
+                    const int key = 32 * b + 8 * (e >> 2) + (e & 3);     // less k0 + 4 hi
+                    if (key > ahead || key <= behind) x[b][e] = -INFINITY;
                 }
-            bool clean = true;
-            if (masked) {
-                Finite fin;
+        }
+        float top = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int i = 0; i < NB; ++i) fin.take(v_frag(j, i));
-                clean = fin.all();
-                asm volatile("" ::: "memory");   // (read again: kept, they would crowd the registers)
-            }
-            if (clean) {
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, x[b][e]);
+        top = xor_butterfly<32, 32>(top, max_raw) * scale;
+        // exp(x - m) as 2^(x scale - m), one fma: m is a rounded product and the fma's is not, so
+        // a row's weights are off by one common factor of 2^(half a step of m).  Far from zero
+        // (2^7) scores are rounded as m is, lest the factor leave fp16's range.
+        float mul = scale;
+        if (__ballot(top > m) || far) {
+            const float mn = max_raw(m, top), f = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+            for (int i = 0; i < NB; ++i)
 #pragma unroll
-                    for (int i = 0; i < NB; ++i)
-                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(j, i), p[j], o[i], 0, 0, 0);
-            } else {
-                // infinities or NaN among values that some rows do not see: they reach the
-                // others by an addition
+                for (int e = 0; e < 16; ++e) o[i][e] *= f;
+            far = __ballot(fabsf(m) >= 128.0f && m != kNone) != 0;
+            if (far) {
 #pragma unroll
-                for (int i = 0; i < NB; ++i) {
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_or_zero(v_frag(j, i)), p[j], o[i], 0, 0, 0);
-                    for (int j = 0; j < kWideKeys; ++j) {
-                        const int key = k0 + j;
-                        if (key > pos || (a.window > 0 && key <= pos - a.window)) continue;
-#pragma unroll
-                        for (int e4 = 0; e4 < 4; ++e4) {
-                            const h4 v = *(lds_h4)(lds0 + at + MAT + (uint32_t)j * ROWB +
-                                                   16u * (uint32_t)((4 * i + e4) ^ v_swizzle<D>(j)) + 8u * (uint32_t)hi);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (!(v[e] - v[e] == (_Float16)0)) o[i][4 * e4 + e] += (float)v[e];
-                        }
-                    }
-                }
+                    for (int e = 0; e < 16; ++e) x[b][e] = __fmul_rn(x[b][e], scale);
+                mul = 1.0f;
             }
         }
-        lds_barrier();                           // the last tile's reads are done before another item's DMAs
-        if (active && w0 + col < rows) {
-            l += lane_xor<32>(l);
-            if (bad) l = NAN;
-            if (s.parts > 1) {
-                float* part = slot_of<ROWS, D>(static_cast<float*>(a.workspace), s, s.part, kvh, nkv);
-                const int row = 32 * wave + col;
+        h8 p[4];
 #pragma unroll
-                for (int i = 0; i < NB; ++i)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int e4 = 0; e4 < 4; ++e4)
-                        *reinterpret_cast<f4*>(part + row * D + 32 * i + 8 * e4 + 4 * hi) =
-                            f4{o[i][4 * e4], o[i][4 * e4 + 1], o[i][4 * e4 + 2], o[i][4 * e4 + 3]};
-                if (hi == 0) {
-                    part[ROWS * D + row] = m;
-                    part[ROWS * (D + 1) + row] = l;
-                }
-            } else {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int64_t at = (int64_t)(s.q0 + token) * a.ld_out + (int64_t)(kvh * plan.group + head) * D + 4 * hi;
-#pragma unroll
-                for (int i = 0; i < NB; ++i)
-#pragma unroll
-                    for (int e4 = 0; e4 < 4; ++e4)
-                        store4(a, at + 32 * i + 8 * e4,
-                               f4{o[i][4 * e4], o[i][4 * e4 + 1], o[i][4 * e4 + 2], o[i][4 * e4 + 3]} * inv);
+            for (int e = 0; e < 16; ++e) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], mul, -m));
+                l += w;
+                p[2 * b + (e >> 3)][e & 7] = (_Float16)w;
             }
+        if (!masked) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(j, i), p[j], o[i], 0, 0, 0);
+            continue;
+        }
+        // infinities and NaN among values that some rows do not see must not meet their zero
+        // weights: finite ones take their place, and the rows that see them get them by an addition
+        Finite fin;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const h8 v = v_frag(j, i);
+                fin.take(v);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_of(v), p[j], o[i], 0, 0, 0);
+            }
+        if (fin.all()) continue;
+#pragma unroll 1
+        for (int j = 0; j < kWideKeys; ++j) {
+            if (k0 + j > pos || (a.window > 0 && k0 + j <= pos - a.window)) continue;
+            const uint32_t row = lds0 + at + MAT + (uint32_t)j * ROWB + 8u * (uint32_t)hi;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4) {
+                    const h4 v = *(lds_h4)(row + 16u * (uint32_t)((4 * i + e4) ^ v_swizzle<D>(j)));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(v[e] - v[e] == (_Float16)0)) o[i][4 * e4 + e] += (float)v[e];
+                }
+        }
+    }
+    if (active && w0 + col < rows) {
+        l += lane_xor<32>(l);
+        if (bad) l = NAN;
+        if (s.parts > 1) {
+            float* part = slot_of<ROWS, D>(static_cast<float*>(a.workspace), s, s.part, kvh, nkv);
+            const int row = 32 * wave + col;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4)
+                    *reinterpret_cast<f4*>(part + row * D + 32 * i + 8 * e4 + 4 * hi) =
+                        f4{o[i][4 * e4], o[i][4 * e4 + 1], o[i][4 * e4 + 2], o[i][4 * e4 + 3]};
+            if (hi == 0) {
+                part[ROWS * D + row] = m;
+                part[ROWS * (D + 1) + row] = l;
+            }
+        } else {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t at = (int64_t)(s.q0 + token) * a.ld_out + (int64_t)(kvh * plan.group + head) * D + 4 * hi;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4)
+                    store4(a, at + 32 * i + 8 * e4,
+                           f4{o[i][4 * e4], o[i][4 * e4 + 1], o[i][4 * e4 + 2], o[i][4 * e4 + 3]} * inv);
         }
     }
 }
@@ -732,8 +726,8 @@ static void attn_go(Kernel kernel, int threads, rf_paged_attention a, const rf_p
     const int64_t tiles = ((int64_t)a.rows * p.group / ROWS + a.num_seqs) * c.num_kv_heads;
     const int64_t most = ((int64_t)a.max_blocks * c.page_size + KEYS * p.least - 1) / (KEYS * p.least);
     p.items = std::min(tiles + p.parts, tiles * std::max<int64_t>(most, 1));
-    const unsigned grid = (unsigned)std::min<int64_t>(p.items, 1 << 20);
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, stream, a, c, p);
+    const unsigned gx = (unsigned)std::min<int64_t>(p.items, 1 << 20), gy = (unsigned)((p.items + gx - 1) / gx);
+    hipLaunchKernelGGL(kernel, dim3(gx, gy), dim3(threads), 0, stream, a, c, p);
     if (most > 1)
         hipLaunchKernelGGL((rf::rf_paged_attn_join_kernel<D, ROWS, KEYS>),
                            dim3((unsigned)std::min<int64_t>(tiles, p.parts) * (ROWS / rf::kMergeRows)), dim3(256), 0,
@@ -757,12 +751,12 @@ static void attn_dim(const rf_paged_attention& a, const rf_paged_cache& c, hipSt
 extern "C" hipError_t rf_paged_attention_launch(const rf_paged_attention* step, const rf_paged_cache* cache,
                                                 hipStream_t stream) {
     if (step == nullptr || cache == nullptr) return hipErrorInvalidValue;
-    const rf_paged_attention& a = *step;
+    rf_paged_attention a = *step;
     const rf_paged_cache& c = *cache;
     if (!rf::cache_ok(c) || a.num_seqs < 0 || a.rows < 0 || a.rows > (1 << 23) || a.max_blocks < 0 ||
         a.num_heads <= 0 || a.num_heads > 65535 || a.num_heads % c.num_kv_heads != 0 ||
         a.num_heads / c.num_kv_heads > 64 || a.window < 0 || !std::isfinite(a.scale) ||
-        (int64_t)a.max_blocks * c.page_size > INT_MAX)
+        (int64_t)a.max_blocks * c.page_size > (1 << 30))
         return hipErrorInvalidValue;
     if (a.rows == 0 || a.num_seqs == 0) return hipSuccess;
     const int64_t width = (int64_t)a.num_heads * c.head_dim;
@@ -772,6 +766,7 @@ extern "C" hipError_t rf_paged_attention_launch(const rf_paged_attention* step, 
           reinterpret_cast<uintptr_t>(a.workspace)) & 15u) != 0 ||
         a.workspace_bytes < rf_paged_attention_workspace_bytes(a.num_heads, c.num_kv_heads, c.head_dim))
         return hipErrorInvalidValue;
+    if (a.window >= (int64_t)a.max_blocks * c.page_size) a.window = 0;     // reaches past every position
     switch (c.head_dim) {
     case 64: attn_dim<64, 4, 4, 8>(a, c, stream); break;
     case 128: attn_dim<128, 4, 2, 8>(a, c, stream); break;

@@ -507,6 +507,16 @@ __device__ __forceinline__ uint16_t f16_bits_rn(float v) {
     return (uint16_t)r;
 }
 
+// fmaxf of values that are no signalling NaNs, as one instruction: where the compiler
+// cannot know that, it quiets both operands first, a serial chain between the scores
+// and their exps (prefill attention, 32 / 8 heads, 4096 positions 150.3 / 149.6 us,
+// 8192 563 / 558).
+__device__ __forceinline__ float max_raw(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
 // Workgroup barrier that does not wait for outstanding global loads
 // (__syncthreads() implies a fence, i.e. vmcnt(0), which would drain the
 // loads a pipeline keeps in flight across the barrier).  LDS writes of this
