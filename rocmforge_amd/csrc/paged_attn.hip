@@ -49,7 +49,6 @@ constexpr int kWideKeys = 64;
 // most twice as many parts are written to the workspace.
 constexpr int kNarrowParts = 512, kNarrowLeast = 4;
 constexpr int kWideParts = 256, kWideLeast = 8;
-constexpr int kMergeRows = 16;
 
 // ---- which part of which request a workgroup does ---------------------------------------
 
@@ -66,6 +65,7 @@ struct Plan {
     int from_rows, to_rows;      // requests of from_rows < packed rows <= to_rows are this kernel's
     int parts, least;
     int64_t items;               // at least as many as there are
+    float* slots;                // the parts' states
 };
 
 struct Request {
@@ -223,14 +223,13 @@ __device__ __forceinline__ h8 finite_of(h8 v) {
 // The waves' (m, l, O) are joined through LDS at the end.  16 KB of K and V a
 // piece (head_dim 128), 64 KB and more in flight a CU.
 template <int D, int W, int S>
-__global__ __launch_bounds__(64 * W) void rf_paged_attn_narrow_kernel(const rf_paged_attention a, const rf_paged_cache c,
-                                                                      const Plan plan) {
+__device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan,
+                                            int64_t item, uint8_t* lds) {
     constexpr int ROWB = 2 * D, MAT = kNarrowKeys * ROWB, STAGE = 2 * MAT;
     constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = kNarrowKeys / RPI;   // instructions a matrix
     constexpr int KS = D / 32, NB = D / 16;
     constexpr int PADD = D + 4;                          // floats a row of the join
-    static_assert(W * kNarrowRows * (PADD + 2) * 4 <= W * S * STAGE, "the join fits the ring");
-    __shared__ __align__(1024) uint8_t lds[W * S * STAGE];
+    static_assert(kNarrowRows * (PADD + 2) * 4 <= S * STAGE, "the join fits the ring");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
     const int nkv = c.num_kv_heads, psh = __ffs(c.page_size) - 1, pmask = c.page_size - 1;
@@ -238,7 +237,6 @@ __global__ __launch_bounds__(64 * W) void rf_paged_attn_narrow_kernel(const rf_p
     const uint32_t ring = lds0 + (uint32_t)wave * (S * STAGE);
     const int dr = lane / LPR, ds = lane % LPR;
 
-    const int64_t item = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
     Share s;
     const int kvh = (int)(item % nkv);
     if (!find_share<kNarrowRows, kNarrowKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
@@ -409,7 +407,7 @@ __global__ __launch_bounds__(64 * W) void rf_paged_attn_narrow_kernel(const rf_p
     }
     __syncthreads();
     const int live = min(rows - r0, kNarrowRows);
-    float* part = slot_of<kNarrowRows, D>(static_cast<float*>(a.workspace), s, s.part, kvh, nkv);
+    float* part = slot_of<kNarrowRows, D>(plan.slots, s, s.part, kvh, nkv);
     for (int i = threadIdx.x; i < live * (D / 4); i += 64 * W) {
         const int row = i / (D / 4), d = 4 * (i % (D / 4));
         float mx = kNone, sum = 0.0f;
@@ -442,20 +440,18 @@ __global__ __launch_bounds__(64 * W) void rf_paged_attn_narrow_kernel(const rf_p
 // DMA, double buffered, one barrier a tile: S^T by 32x32x16 MFMAs (two blocks of
 // 32 keys), lane (row lane % 32, keys 8 (e / 4) + 4 (lane / 32) + e % 4).
 template <int D, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4)))
-void rf_paged_attn_wide_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan plan) {
+__device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan,
+                                          int64_t item, uint8_t* lds) {
     constexpr int ROWB = 2 * D, MAT = kWideKeys * ROWB, STAGE = 2 * MAT, ROWS = 32 * NW;
     constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = kWideKeys / (RPI * NW);   // a wave's instructions a matrix
     constexpr int KS = D / 16, NB = D / 32;
     static_assert(NI >= 1, "every wave has rows to fetch");
-    __shared__ __align__(1024) uint8_t lds[2 * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, hi = lane >> 5;
     const int nkv = c.num_kv_heads, psh = __ffs(c.page_size) - 1, pmask = c.page_size - 1;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     const int dr = lane / LPR, ds = lane % LPR;
 
-    const int64_t item = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
     Share s;
     const int kvh = (int)(item % nkv);
     if (!find_share<ROWS, kWideKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
@@ -645,7 +641,7 @@ void rf_paged_attn_wide_kernel(const rf_paged_attention a, const rf_paged_cache 
         l += lane_xor<32>(l);
         if (bad) l = NAN;
         if (s.parts > 1) {
-            float* part = slot_of<ROWS, D>(static_cast<float*>(a.workspace), s, s.part, kvh, nkv);
+            float* part = slot_of<ROWS, D>(plan.slots, s, s.part, kvh, nkv);
             const int row = 32 * wave + col;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
@@ -670,82 +666,171 @@ void rf_paged_attn_wide_kernel(const rf_paged_attention a, const rf_paged_cache 
     }
 }
 
-// ---- joining the parts --------------------------------------------------------------------
+// ---- the launches -------------------------------------------------------------------------
 
-// 16 rows of a tile of several parts a workgroup.
-template <int D, int ROWS, int KEYS>
-__global__ __launch_bounds__(256) void rf_paged_attn_join_kernel(const rf_paged_attention a, const rf_paged_cache c,
-                                                                 const Plan plan) {
-    constexpr int SUB = ROWS / kMergeRows;
-    const int nkv = c.num_kv_heads;
-    const int item = blockIdx.x / SUB, first = kMergeRows * (blockIdx.x % SUB), kvh = item % nkv;
-    Share s;
-    if (!find_share<ROWS, KEYS>(a, c, plan, item / nkv, true, s)) return;
-    const int rows = s.n * plan.group, r0 = ROWS * s.tile;
-    const int live = min(rows - r0, first + kMergeRows) - first;
-    const int64_t next = (int64_t)s.tiles * nkv * (ROWS * (D + 2));
-    const float* part0 = slot_of<ROWS, D>(static_cast<float*>(a.workspace), s, 0, kvh, nkv);
-    for (int i = threadIdx.x; i < live * (D / 4); i += 256) {
-        const int row = first + i / (D / 4), d = 4 * (i % (D / 4));
-        float mx = kNone, sum = 0.0f;
-        for (int k = 0; k < s.parts; ++k) mx = fmaxf(mx, part0[k * next + ROWS * D + row]);
-        f4 acc = {0, 0, 0, 0};
-        for (int k = 0; k < s.parts; ++k) {
-            const float* p = part0 + k * next;
-            const float f = __builtin_amdgcn_exp2f(p[ROWS * D + row] - mx);
-            sum += p[ROWS * (D + 1) + row] * f;
-            acc += *reinterpret_cast<const f4*>(p + row * D + d) * f;
-        }
-        const int tk = (r0 + row) / plan.group, hd = r0 + row - tk * plan.group;
-        store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d,
-               sum == 0.0f ? f4{0, 0, 0, 0} : acc * (1.0f / sum));
+constexpr int kJoinRows = 16;
+constexpr int kJoinParts = kNarrowParts + 1;     // of a tile, at most
+
+// Head dims, waves and stages of the narrow part, waves of the wide one.
+template <int D> struct Shape;
+template <> struct Shape<64> { static constexpr int W = 4, S = 4, NW = 8; };
+template <> struct Shape<128> { static constexpr int W = 4, S = 2, NW = 8; };
+template <> struct Shape<256> { static constexpr int W = 2, S = 2, NW = 4; };
+template <int D>
+constexpr int narrow_lds() { return Shape<D>::W * Shape<D>::S * 2 * kNarrowKeys * 2 * D; }
+template <int D>
+constexpr int wide_lds() { return 2 * 2 * kWideKeys * 2 * D; }
+template <int D>
+constexpr int wide_rows() { return 32 * Shape<D>::NW; }
+
+template <int D>
+__global__ __launch_bounds__(64 * Shape<D>::W)
+void rf_paged_attn_narrow_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan plan) {
+    __shared__ __align__(1024) uint8_t lds[narrow_lds<D>()];
+    narrow_part<D, Shape<D>::W, Shape<D>::S>(a, c, plan, blockIdx.x + (int64_t)blockIdx.y * gridDim.x, lds);
+}
+
+// Both kinds in one launch, the wide items first: their workgroups are the
+// longer ones, and the narrow ones fill the CUs that they leave.
+template <int D>
+__global__ __launch_bounds__(64 * Shape<D>::NW) __attribute__((amdgpu_waves_per_eu(Shape<D>::NW / 4)))
+void rf_paged_attn_mixed_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan wide, const Plan narrow) {
+    __shared__ __align__(1024) uint8_t lds[narrow_lds<D>() > wide_lds<D>() ? narrow_lds<D>() : wide_lds<D>()];
+    const int64_t item = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+    if (item < wide.items) {
+        wide_part<D, Shape<D>::NW>(a, c, wide, item, lds);
+    } else {
+        if (threadIdx.x >= 64 * Shape<D>::W) return;     // whole waves, before any barrier
+        narrow_part<D, Shape<D>::W, Shape<D>::S>(a, c, narrow, item - wide.items, lds);
     }
+}
+
+// Joins 16 rows of a tile of several parts: the parts' weights 2^(m - max m)
+// through LDS, then each output over the parts, by as many threads as there are
+// for it.
+template <int D, int ROWS, int KEYS>
+__device__ __forceinline__ void join_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan, int item,
+                                          float (*weight)[kJoinRows], f4* sums) {
+    constexpr int SUB = ROWS / kJoinRows;
+    const int nkv = c.num_kv_heads, tid = threadIdx.x;
+    const int first = kJoinRows * (item % SUB), kvh = item / SUB % nkv;
+    Share s;
+    if (!find_share<ROWS, KEYS>(a, c, plan, item / SUB / nkv, true, s)) return;
+    const int rows = s.n * plan.group, r0 = ROWS * s.tile;
+    const int live = min(rows - r0 - first, kJoinRows);
+    if (live <= 0) return;
+    const int64_t next = (int64_t)s.tiles * nkv * (ROWS * (D + 2));
+    const float* part0 = slot_of<ROWS, D>(plan.slots, s, 0, kvh, nkv) + first * D;
+    const float* m0 = part0 + (ROWS - first) * D + first;
+    {
+        const int row = tid / 16;                // 16 lanes a row
+        float mx = kNone, sum = 0.0f;
+        if (row < live) {
+            for (int k = tid % 16; k < s.parts; k += 16) mx = fmaxf(mx, m0[k * next + row]);
+            mx = xor_max<8, 1>(mx);
+            for (int k = tid % 16; k < s.parts; k += 16) {
+                const float f = __builtin_amdgcn_exp2f(m0[k * next + row] - mx);
+                weight[k][row] = f;
+                sum += m0[k * next + ROWS + row] * f;
+            }
+            sum = xor_sum<8, 1>(sum);
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            for (int k = tid % 16; k < s.parts; k += 16) weight[k][row] *= inv;
+        }
+    }
+    __syncthreads();
+    const int outs = live * (D / 4), groups = max(256 / outs, 1);
+    for (int o0 = 0; o0 < outs; o0 += 256) {
+        const int g = groups == 1 ? 0 : tid / outs, i = groups == 1 ? o0 + tid : tid - g * outs;
+        f4 acc = {0, 0, 0, 0};
+        if (g < groups && i < outs) {
+            const int row = i / (D / 4);
+#pragma unroll 4
+            for (int k = g; k < s.parts; k += groups) {
+                const float f = weight[k][row];
+                const f4 v = *reinterpret_cast<const f4*>(part0 + k * next + 4 * i);
+                acc += v * f;
+            }
+        }
+        if (groups > 1) {
+            sums[tid] = acc;
+            __syncthreads();
+            if (tid < outs)
+                for (int k = 1; k < groups; ++k) acc += sums[tid + k * outs];
+        }
+        if (i < outs && g == 0) {
+            const int row = r0 + first + i / (D / 4), d = 4 * (i % (D / 4));
+            const int tk = row / plan.group, hd = row - tk * plan.group;
+            store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d, acc);
+        }
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void rf_paged_attn_join_kernel(const rf_paged_attention a, const rf_paged_cache c,
+                                                                 const Plan wide, const Plan narrow, int wide_items) {
+    __shared__ float weight[kJoinParts][kJoinRows];
+    __shared__ f4 sums[256];
+    const int item = blockIdx.x;
+    if (item < wide_items)
+        join_part<D, wide_rows<D>(), kWideKeys>(a, c, wide, item, weight, sums);
+    else
+        join_part<D, kNarrowRows, kNarrowKeys>(a, c, narrow, item - wide_items, weight, sums);
 }
 
 }  // namespace rf
 
-// ---- launchers -----------------------------------------------------------------------------
-
 // Bytes of the narrow and the wide parts of a launch.
-static size_t narrow_bytes(int d) { return (size_t)2 * rf::kNarrowParts * rf::kNarrowRows * (d + 2) * sizeof(float); }
-static size_t wide_bytes(int d) { return (size_t)2 * rf::kWideParts * (d == 256 ? 128 : 256) * (d + 2) * sizeof(float); }
+template <int D>
+static constexpr size_t narrow_bytes() { return (size_t)2 * rf::kNarrowParts * rf::kNarrowRows * (D + 2) * sizeof(float); }
+template <int D>
+static constexpr size_t wide_bytes() { return (size_t)2 * rf::kWideParts * rf::wide_rows<D>() * (D + 2) * sizeof(float); }
 
 extern "C" size_t rf_paged_attention_workspace_bytes(int num_heads, int num_kv_heads, int head_dim) {
-    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
-        (head_dim != 64 && head_dim != 128 && head_dim != 256))
-        return 0;
-    return narrow_bytes(head_dim) + wide_bytes(head_dim);
-}
-
-template <int D, int ROWS, int KEYS, class Kernel>
-static void attn_go(Kernel kernel, int threads, rf_paged_attention a, const rf_paged_cache& c, rf::Plan p,
-                    float* workspace, hipStream_t stream) {
-    a.workspace = workspace;
-    // Items: every tile has a part, and at most p.parts more (each of them is p.parts' share long);
-    // no more either than the table's width gives room for.
-    const int64_t tiles = ((int64_t)a.rows * p.group / ROWS + a.num_seqs) * c.num_kv_heads;
-    const int64_t most = ((int64_t)a.max_blocks * c.page_size + KEYS * p.least - 1) / (KEYS * p.least);
-    p.items = std::min(tiles + p.parts, tiles * std::max<int64_t>(most, 1));
-    const unsigned gx = (unsigned)std::min<int64_t>(p.items, 1 << 20), gy = (unsigned)((p.items + gx - 1) / gx);
-    hipLaunchKernelGGL(kernel, dim3(gx, gy), dim3(threads), 0, stream, a, c, p);
-    if (most > 1)
-        hipLaunchKernelGGL((rf::rf_paged_attn_join_kernel<D, ROWS, KEYS>),
-                           dim3((unsigned)std::min<int64_t>(tiles, p.parts) * (ROWS / rf::kMergeRows)), dim3(256), 0,
-                           stream, a, c, p);
-}
-
-template <int D, int W, int S, int NW>
-static void attn_dim(const rf_paged_attention& a, const rf_paged_cache& c, hipStream_t stream) {
-    const int group = a.num_heads / c.num_kv_heads;
-    const bool both = (int64_t)a.max_new * group > rf::kNarrowRows;
-    float* ws = static_cast<float*>(a.workspace);
-    rf::Plan p = {group, 0, both ? rf::kNarrowRows : INT_MAX, rf::kNarrowParts, rf::kNarrowLeast, 0};
-    attn_go<D, rf::kNarrowRows, rf::kNarrowKeys>(rf::rf_paged_attn_narrow_kernel<D, W, S>, 64 * W, a, c, p, ws, stream);
-    if (both) {
-        p = {group, rf::kNarrowRows, INT_MAX, rf::kWideParts, rf::kWideLeast, 0};
-        attn_go<D, 32 * NW, rf::kWideKeys>(rf::rf_paged_attn_wide_kernel<D, NW>, 64 * NW, a, c, p,
-                                           ws + narrow_bytes(D) / sizeof(float), stream);
+    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0) return 0;
+    switch (head_dim) {
+    case 64: return narrow_bytes<64>() + wide_bytes<64>();
+    case 128: return narrow_bytes<128>() + wide_bytes<128>();
+    case 256: return narrow_bytes<256>() + wide_bytes<256>();
+    default: return 0;
     }
+}
+
+template <int D>
+static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStream_t stream) {
+    using namespace rf;
+    constexpr int ROWS = wide_rows<D>();
+    const int nkv = c.num_kv_heads, group = a.num_heads / nkv;
+    const int64_t packed = (int64_t)a.rows * group, positions = (int64_t)a.max_blocks * c.page_size;
+    const bool both = (int64_t)a.max_new * group > kNarrowRows;
+    float* ws = static_cast<float*>(a.workspace);
+    Plan narrow = {group, 0, both ? kNarrowRows : INT_MAX, kNarrowParts, kNarrowLeast, 0, ws};
+    Plan wide = {group, kNarrowRows, INT_MAX, kWideParts, kWideLeast, 0, ws + narrow_bytes<D>() / sizeof(float)};
+    // Items: every tile has a part, and there are at most `parts` parts more (each of them a share
+    // long); no more either than the table's width gives room for.
+    const auto items = [&](int64_t tiles, const Plan& p, int keys, int64_t* joins) {
+        const int64_t most = std::max<int64_t>((positions + keys * p.least - 1) / (keys * p.least), 1);
+        *joins = most > 1 ? std::min<int64_t>(tiles, p.parts) : 0;
+        return std::min(tiles + p.parts, tiles * most);
+    };
+    const int64_t some = std::min<int64_t>(a.num_seqs, a.rows);        // requests with rows
+    int64_t narrow_joins, wide_joins = 0;
+    narrow.items = items((both ? some : packed / kNarrowRows + some) * nkv, narrow, kNarrowKeys, &narrow_joins);
+    if (both) {
+        wide.items = items((packed / ROWS + std::min(some, packed / kNarrowRows)) * nkv, wide, kWideKeys, &wide_joins);
+        // (workgroups i and i + 8 share an XCD's L2, and items i and i + num_kv_heads their K and V)
+        wide.items = (wide.items + 8 * nkv - 1) / (8 * nkv) * (8 * nkv);
+    }
+    const int64_t total = wide.items + narrow.items;
+    const dim3 grid((unsigned)std::min<int64_t>(total, 1 << 20), (unsigned)((total + (1 << 20) - 1) >> 20));
+    if (both)
+        hipLaunchKernelGGL(rf_paged_attn_mixed_kernel<D>, grid, dim3(64 * Shape<D>::NW), 0, stream, a, c, wide, narrow);
+    else
+        hipLaunchKernelGGL(rf_paged_attn_narrow_kernel<D>, grid, dim3(64 * Shape<D>::W), 0, stream, a, c, narrow);
+    const int wide_blocks = (int)wide_joins * (ROWS / kJoinRows);
+    if (wide_joins + narrow_joins > 0)
+        hipLaunchKernelGGL(rf_paged_attn_join_kernel<D>, dim3((unsigned)(wide_blocks + narrow_joins)), dim3(256), 0,
+                           stream, a, c, wide, narrow, wide_blocks);
 }
 
 extern "C" hipError_t rf_paged_attention_launch(const rf_paged_attention* step, const rf_paged_cache* cache,
@@ -768,9 +853,9 @@ extern "C" hipError_t rf_paged_attention_launch(const rf_paged_attention* step, 
         return hipErrorInvalidValue;
     if (a.window >= (int64_t)a.max_blocks * c.page_size) a.window = 0;     // reaches past every position
     switch (c.head_dim) {
-    case 64: attn_dim<64, 4, 4, 8>(a, c, stream); break;
-    case 128: attn_dim<128, 4, 2, 8>(a, c, stream); break;
-    default: attn_dim<256, 2, 2, 4>(a, c, stream); break;
+    case 64: attn_go<64>(a, c, stream); break;
+    case 128: attn_go<128>(a, c, stream); break;
+    default: attn_go<256>(a, c, stream); break;
     }
     return hipGetLastError();
 }
