@@ -41,6 +41,10 @@ typedef __attribute__((address_space(3))) const h4* lds_h4;
 
 constexpr float kNone = -3.0e+38f;               // the maximum of no scores
 constexpr float kLog2e = 1.4426950408889634f;
+// A row's maximum is left behind until a score passes it by more than 2^8: most
+// tiles then rescale nothing.  Weights reach 256 (fp16 ends at 65504), and since
+// the sum is of the rounded weights, a row of one key still has it exactly.
+constexpr float kLag = 8.0f;
 
 constexpr int kNarrowRows = 16, kNarrowKeys = 32;
 constexpr int kWideKeys = 64;
@@ -48,7 +52,7 @@ constexpr int kWideKeys = 64;
 // keys.  A tile is cut only where its share is longer than total / parts, so at
 // most twice as many parts are written to the workspace.
 constexpr int kNarrowParts = 512, kNarrowLeast = 4;
-constexpr int kWideParts = 256, kWideLeast = 8;
+constexpr int kWideParts = 512, kWideLeast = 8;
 
 // ---- which part of which request a workgroup does ---------------------------------------
 
@@ -198,6 +202,15 @@ __device__ __forceinline__ h4 read_tr(uint32_t at) {
 
 __device__ __forceinline__ h8 join(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+// l + the eight weights, products with one in fp32.
+__device__ __forceinline__ float sum8(h8 p, float l) {
+    const h2 one = {1, 1};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l = __builtin_amdgcn_fdot2(h2{p[2 * i], p[2 * i + 1]}, one, l, false);
+    return l;
+}
+
 // Whether any of the values is an infinity or NaN: 0 * x is then not 0.
 struct Finite {
     h8 acc = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -342,7 +355,7 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
                 top = fmaxf(top, x[b][e]);
             }
         top = xor_butterfly<32, 16>(top, max_raw);
-        if (__ballot(top > m)) {
+        if (__ballot(top > m + kLag)) {
             const float mn = max_raw(m, top), f = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= f;
@@ -353,41 +366,38 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float w = __builtin_amdgcn_exp2f(x[b][e] - m);
-                l += w;
-                p[4 * b + e] = (_Float16)w;
-            }
+            for (int e = 0; e < 4; ++e) p[4 * b + e] = (_Float16)__builtin_amdgcn_exp2f(x[b][e] - m);
+        l = sum8(p, l);
         // V^T: lane (dim 16 i + col) takes keys 4 quad + {0 .. 3, 16 .. 19}, as p holds them
-        auto v_frag = [&](int i) {
-            const uint32_t v = vt ^ (32u * i);
-            return join(read_tr(v), read_tr(v + 16u * ROWB));
-        };
-        if (!masked) {
+        h8 v[NB];
 #pragma unroll
-            for (int i = 0; i < NB; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_frag(i), p, o[i], 0, 0, 0);
-            continue;
+        for (int i = 0; i < NB; ++i) {
+            const uint32_t row = vt ^ (32u * i);
+            v[i] = join(read_tr(row), read_tr(row + 16u * ROWB));
         }
         // infinities and NaN among values that some rows do not see must not meet their zero
         // weights: finite ones take their place, and the rows that see them get them by an addition
         Finite fin;
+        if (masked) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const h8 v = v_frag(i);
-            fin.take(v);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(finite_of(v), p, o[i], 0, 0, 0);
+            for (int i = 0; i < NB; ++i) {
+                fin.take(v[i]);
+                v[i] = finite_of(v[i]);
+            }
         }
-        if (fin.all()) continue;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i], p, o[i], 0, 0, 0);
+        if (!masked || fin.all()) continue;
 #pragma unroll 1
         for (int j = 0; j < kNarrowKeys; ++j) {
             if (k0 + j > pos || (a.window > 0 && k0 + j <= pos - a.window)) continue;
             const uint32_t row = ring + at + MAT + (uint32_t)j * ROWB + 8u * (uint32_t)(quad & 1);
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                const h4 v = *(lds_h4)(row + 16u * (uint32_t)((2 * i + (quad >> 1)) ^ v_swizzle<D>(j)));
+                const h4 w = *(lds_h4)(row + 16u * (uint32_t)((2 * i + (quad >> 1)) ^ v_swizzle<D>(j)));
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (!(v[e] - v[e] == (_Float16)0)) o[i][e] += (float)v[e];
+                    if (!(w[e] - w[e] == (_Float16)0)) o[i][e] += (float)w[e];
             }
         }
     }
@@ -556,6 +566,16 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
             return join(read_tr(v), read_tr(v + 8u * ROWB));
         };
         const bool masked = k0 + kWideKeys - 1 > u.first || (a.window > 0 && k0 <= u.last - a.window);
+        // (all of V's operands before the softmax where the registers allow it: in flight meanwhile)
+        constexpr int JG = D <= 128 ? 4 : 1;
+        h8 v[JG][NB];
+        if constexpr (JG == 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < NB; ++i) v[j][i] = v_frag(j, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (masked) {
             const int ahead = pos - k0 - 4 * hi, behind = a.window > 0 ? ahead - a.window : INT_MIN;
 #pragma unroll
@@ -576,7 +596,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         // a row's weights are off by one common factor of 2^(half a step of m).  Far from zero
         // (2^7) scores are rounded as m is, lest the factor leave fp16's range.
         float mul = scale;
-        if (__ballot(top > m) || far) {
+        if (__ballot(top > m + kLag) || far) {
             const float mn = max_raw(m, top), f = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= f;
@@ -597,31 +617,34 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], mul, -m));
-                l += w;
-                p[2 * b + (e >> 3)][e & 7] = (_Float16)w;
-            }
-        if (!masked) {
+            for (int e = 0; e < 16; ++e)
+                p[2 * b + (e >> 3)][e & 7] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], mul, -m));
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < NB; ++i)
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(j, i), p[j], o[i], 0, 0, 0);
-            continue;
-        }
+        for (int j = 0; j < 4; ++j) l = sum8(p[j], l);
         // infinities and NaN among values that some rows do not see must not meet their zero
         // weights: finite ones take their place, and the rows that see them get them by an addition
         Finite fin;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j0 = 0; j0 < 4; j0 += JG) {
+            if constexpr (JG < 4)
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                const h8 v = v_frag(j, i);
-                fin.take(v);
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_of(v), p[j], o[i], 0, 0, 0);
+                for (int i = 0; i < NB; ++i) v[0][i] = v_frag(j0, i);
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < JG; ++j)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) {
+                        fin.take(v[j][i]);
+                        v[j][i] = finite_of(v[j][i]);
+                    }
             }
-        if (fin.all()) continue;
+#pragma unroll
+            for (int j = 0; j < JG; ++j)
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[j][i], p[j0 + j], o[i], 0, 0, 0);
+        }
+        if (!masked || fin.all()) continue;
 #pragma unroll 1
         for (int j = 0; j < kWideKeys; ++j) {
             if (k0 + j > pos || (a.window > 0 && k0 + j <= pos - a.window)) continue;
@@ -630,10 +653,10 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
             for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int e4 = 0; e4 < 4; ++e4) {
-                    const h4 v = *(lds_h4)(row + 16u * (uint32_t)((4 * i + e4) ^ v_swizzle<D>(j)));
+                    const h4 w = *(lds_h4)(row + 16u * (uint32_t)((4 * i + e4) ^ v_swizzle<D>(j)));
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!(v[e] - v[e] == (_Float16)0)) o[i][4 * e4 + e] += (float)v[e];
+                        if (!(w[e] - w[e] == (_Float16)0)) o[i][4 * e4 + e] += (float)w[e];
                 }
         }
     }
@@ -672,12 +695,13 @@ constexpr int kJoinRows = 16;
 constexpr int kJoinParts = kNarrowParts + 1;     // of a tile, at most
 
 // Head dims, waves and stages of the narrow part, waves of the wide one.
+// (MW, MS: of the narrow part beside wide ones)
 template <int D> struct Shape;
-template <> struct Shape<64> { static constexpr int W = 4, S = 4, NW = 8; };
-template <> struct Shape<128> { static constexpr int W = 4, S = 2, NW = 8; };
-template <> struct Shape<256> { static constexpr int W = 2, S = 2, NW = 4; };
+template <> struct Shape<64> { static constexpr int W = 4, S = 4, NW = 4, MW = 4, MS = 2, EU = 2; };
+template <> struct Shape<128> { static constexpr int W = 4, S = 2, NW = 4, MW = 2, MS = 2, EU = 2; };
+template <> struct Shape<256> { static constexpr int W = 2, S = 2, NW = 4, MW = 2, MS = 2, EU = 1; };
 template <int D>
-constexpr int narrow_lds() { return Shape<D>::W * Shape<D>::S * 2 * kNarrowKeys * 2 * D; }
+constexpr int narrow_lds(int w, int s) { return w * s * 2 * kNarrowKeys * 2 * D; }
 template <int D>
 constexpr int wide_lds() { return 2 * 2 * kWideKeys * 2 * D; }
 template <int D>
@@ -686,22 +710,23 @@ constexpr int wide_rows() { return 32 * Shape<D>::NW; }
 template <int D>
 __global__ __launch_bounds__(64 * Shape<D>::W)
 void rf_paged_attn_narrow_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan plan) {
-    __shared__ __align__(1024) uint8_t lds[narrow_lds<D>()];
+    __shared__ __align__(1024) uint8_t lds[narrow_lds<D>(Shape<D>::W, Shape<D>::S)];
     narrow_part<D, Shape<D>::W, Shape<D>::S>(a, c, plan, blockIdx.x + (int64_t)blockIdx.y * gridDim.x, lds);
 }
 
 // Both kinds in one launch, the wide items first: their workgroups are the
 // longer ones, and the narrow ones fill the CUs that they leave.
 template <int D>
-__global__ __launch_bounds__(64 * Shape<D>::NW) __attribute__((amdgpu_waves_per_eu(Shape<D>::NW / 4)))
+__global__ __launch_bounds__(64 * Shape<D>::NW) __attribute__((amdgpu_waves_per_eu(Shape<D>::EU)))
 void rf_paged_attn_mixed_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan wide, const Plan narrow) {
-    __shared__ __align__(1024) uint8_t lds[narrow_lds<D>() > wide_lds<D>() ? narrow_lds<D>() : wide_lds<D>()];
+    constexpr int MW = Shape<D>::MW, MS = Shape<D>::MS, NEED = narrow_lds<D>(MW, MS);
+    __shared__ __align__(1024) uint8_t lds[NEED > wide_lds<D>() ? NEED : wide_lds<D>()];
     const int64_t item = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
     if (item < wide.items) {
         wide_part<D, Shape<D>::NW>(a, c, wide, item, lds);
     } else {
-        if (threadIdx.x >= 64 * Shape<D>::W) return;     // whole waves, before any barrier
-        narrow_part<D, Shape<D>::W, Shape<D>::S>(a, c, narrow, item - wide.items, lds);
+        if (threadIdx.x >= 64 * MW) return;      // whole waves, before any barrier
+        narrow_part<D, MW, MS>(a, c, narrow, item - wide.items, lds);
     }
 }
 

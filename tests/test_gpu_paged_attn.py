@@ -295,3 +295,18 @@ def test_two_streams_with_workspaces_of_their_own(rf, dev):
     torch.cuda.synchronize()
     for c, w in zip(cases, want):
         assert torch.equal(c.live(), w)
+
+
+@pytest.mark.parametrize("lead", [8.0, 10.0, 10.5, 11.0, 12.0])
+@pytest.mark.parametrize("new,kv", [([1], [16000]), ([40], [16000]), ([2], [3000])])
+def test_many_small_weights_beside_a_large_one(rf, dev, lead, new, kv):
+    # weights around and below fp16's smallest normal one, thousands of them: they count
+    c = Case(new, kv, nh=2, nkv=1)
+    for j in range(-(-kv[0] // 16)):
+        c.k[c.tab[0, j].long()] = 0.0
+    t = kv[0] // 3
+    c.k[c.tab[0, t // 16].long(), t % 16, 0, 0] = 1.0
+    c.q.zero_()
+    c.q.view(-1, 2, 128)[:, :, 0] = lead / c.scale
+    c.v.copy_((c.v.float().abs() + 1).half())
+    c.check()
