@@ -24,6 +24,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "paged_common.h"
 #include "qk_common.h"
@@ -188,11 +189,39 @@ __device__ __forceinline__ int v_swizzle(int row) {
     return (D == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3)) ^ (2 * ((row >> 2) & 1));
 }
 
-// LDS DMA of a group of rows of one page: its lanes' row and piece.
+// LDS DMA of a group of rows: lanes a row, rows an instruction.
 template <int D>
 struct Dma {
-    static constexpr int LPR = D / 8, RPI = 64 / LPR;     // lanes a row, rows an instruction
+    static constexpr int LPR = D / 8, RPI = 64 / LPR;
 };
+
+// Where K's rows of a request lie, by units of 8 positions (no page is smaller):
+// a lane holds the address of one unit, so that a group of rows costs two lane
+// reads and no table lookup or product.  lo, hi: the positions that are seen; units
+// outside are taken from the nearest one inside.
+struct Units {
+    const int* table;
+    const uint16_t* k;
+    int psh, pmask, unit_lo, unit_hi, num_pages;
+    int64_t page_stride, row_stride;
+    __device__ __forceinline__ Units(const rf_paged_attention& a, const rf_paged_cache& c, int b, int kvh, int lo, int hi)
+        : table(a.block_tables + (int64_t)b * a.max_blocks), k(c.k + kvh * c.head_stride), psh(__ffs(c.page_size) - 1),
+          pmask(c.page_size - 1), unit_lo(lo >> 3), unit_hi((hi - 1) >> 3), num_pages(c.num_pages),
+          page_stride(c.page_stride), row_stride(c.row_stride) {}
+    __device__ __forceinline__ int seen(int unit) const { return min(max(unit, unit_lo), unit_hi); }
+    __device__ __forceinline__ int page_of(int unit) const { return table[(8 * seen(unit)) >> psh]; }
+    // page: page_of(unit); one outside the cache is read as page 0, and reported
+    __device__ __forceinline__ uint64_t address(int unit, int page, bool& bad) const {
+        const bool out = (unsigned)page >= (unsigned)num_pages;
+        bad = bad || __ballot(out) != 0;
+        return reinterpret_cast<uint64_t>(k + (int64_t)(out ? 0 : page) * page_stride +
+                                          (int64_t)((8 * seen(unit)) & pmask) * row_stride);
+    }
+};
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) |
+           ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32);
+}
 
 // One LDS read of four keys of one dim: 16 lanes read 4 rows of 32 bytes (lane i
 // row i / 4, 8-byte piece i % 4) and receive dim i's four keys.
@@ -223,8 +252,9 @@ struct Finite {
     }
 };
 // The value, or a finite one in the place of an infinity or NaN.
-__device__ __forceinline__ h8 finite_of(h8 v) {
-    const h8 most = (h8)(_Float16)65504.0f;
+template <class V>
+__device__ __forceinline__ V finite_of(V v) {
+    const V most = (V)(_Float16)65504.0f;
     return __builtin_elementwise_min(__builtin_elementwise_max(v, -most), most);
 }
 
@@ -245,7 +275,7 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
     static_assert(kNarrowRows * (PADD + 2) * 4 <= S * STAGE, "the join fits the ring");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
-    const int nkv = c.num_kv_heads, psh = __ffs(c.page_size) - 1, pmask = c.page_size - 1;
+    const int nkv = c.num_kv_heads;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     const uint32_t ring = lds0 + (uint32_t)wave * (S * STAGE);
     const int dr = lane / LPR, ds = lane % LPR;
@@ -263,52 +293,48 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
     // this lane's packed row
     const int r = r0 + col, token = min(r, rows - 1) / plan.group, head = min(r, rows - 1) - token * plan.group;
     const int pos = s.kv - s.n + token;
-    const int* table = a.block_tables + (int64_t)s.b * a.max_blocks;
-    const uint16_t* kc = c.k + kvh * c.head_stride;
-    const uint16_t* vc = c.v + kvh * c.head_stride;
-
-    // page ids of 64 / ppp pieces to come, lane (step, page of the piece)
-    const int ppp = c.page_size >= kNarrowKeys ? 1 : kNarrowKeys >> psh, window = 64 / ppp;
-    int ids = 0, ids_step = 0;
+    // the addresses of the units of 16 pieces to come, lane (step, unit of the piece)
+    const Units units(a, c, s.b, kvh, t.lo, t.hi);
     bool bad = false;
-    auto load_ids = [&](int step) {
-        const int piece = begin + wave + W * (step + lane / ppp);
-        const int page = min(max((piece * kNarrowKeys >> psh) + lane % ppp, t.lo >> psh), (t.hi - 1) >> psh);
-        ids = table[page];
-        const bool out = (unsigned)ids >= (unsigned)c.num_pages;
-        bad = bad || __ballot(out) != 0;
-        ids = out ? 0 : ids;
-        ids_step = step;
+    int window = 0;
+    uint64_t address = 0;
+    const uint64_t v_from_k = (uint64_t)c.v - (uint64_t)c.k;
+    const uint32_t stride = (uint32_t)(2 * c.row_stride);
+    auto load_units = [&](int step) {
+        const int unit = 4 * (begin + wave + W * (step + (lane >> 2))) + (lane & 3);
+        address = units.address(unit, units.page_of(unit), bad);
+        window = step;
     };
     auto stage = [&](int step) {
         if (step >= steps) return;
-        if (step - ids_step >= window) load_ids(step);
-        const int k0 = kNarrowKeys * (begin + wave + W * step);
+        if (step - window >= 16) load_units(step);
+        const int piece = begin + wave + W * step, k0 = kNarrowKeys * piece;
         const uint32_t dst = ring + (uint32_t)(step % S) * STAGE;
         const bool whole = k0 >= t.lo && k0 + kNarrowKeys <= t.hi;
         // the ring's last readers are done
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            // positions that no row sees are taken from the nearest one that some row sees
-            const int at = whole ? k0 + RPI * i
-                                 : max(min(k0 + RPI * i, (t.hi - 1) & ~(RPI - 1)), t.lo & ~(RPI - 1));
-            const int back = whole ? dr : min(max(at + dr, t.lo), t.hi - 1) - at;
-            const int page = __builtin_amdgcn_readlane(ids, (step - ids_step) * ppp + ((at >> psh) - (k0 >> psh)));
-            const int64_t off = (int64_t)page * c.page_stride + (int64_t)(at & pmask) * c.row_stride;
-            const uint32_t row = (uint32_t)back * (uint32_t)(2 * c.row_stride);
             const int lr = RPI * i + dr;
+            int unit = 4 * piece + (RPI * i >> 3);
+            uint32_t row = (uint32_t)((RPI * i & 7) + dr) * stride;
+            if (!whole) {
+                // positions that no row sees are taken from the nearest one that some row sees
+                unit = units.seen(unit);
+                row = (uint32_t)(min(max(k0 + lr, t.lo), t.hi - 1) - 8 * unit) * stride;
+            }
+            const uint64_t at = read_lane(address, 4 * (step - window) + unit - 4 * piece);
             lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * i), row + 16u * (uint32_t)(ds ^ k_swizzle<D>(lr)),
-                      reinterpret_cast<const uint8_t*>(kc + off));
+                      reinterpret_cast<const uint8_t*>(at));
             lds_dma16(__builtin_amdgcn_readfirstlane(dst + MAT + 1024u * i),
-                      row + 16u * (uint32_t)(ds ^ v_swizzle<D>(lr)), reinterpret_cast<const uint8_t*>(vc + off));
+                      row + 16u * (uint32_t)(ds ^ v_swizzle<D>(lr)), reinterpret_cast<const uint8_t*>(at + v_from_k));
         }
     };
     h8 q[KS];
     const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * quad;
 #pragma unroll
     for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const h8*>(qrow + 32 * k);
-    if (steps > 0) load_ids(0);
+    if (steps > 0) load_units(0);
     // (q has arrived before the DMAs start, so that none but theirs are counted below)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
@@ -325,6 +351,7 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
 #pragma unroll
     for (int i = 0; i < NB; ++i) o[i] = f4{0, 0, 0, 0};
     float m = kNone, l = 0.0f;
+    bool dirty = false;
     for (int step = 0; step < steps; ++step) {
         stage(step + S - 1);
         if (step + S <= steps)
@@ -376,7 +403,7 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
             v[i] = join(read_tr(row), read_tr(row + 16u * ROWB));
         }
         // infinities and NaN among values that some rows do not see must not meet their zero
-        // weights: finite ones take their place, and the rows that see them get them by an addition
+        // weights: finite ones take their place, and the rows that see them get them at the end
         Finite fin;
         if (masked) {
 #pragma unroll
@@ -387,17 +414,27 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i], p, o[i], 0, 0, 0);
-        if (!masked || fin.all()) continue;
+        if (masked) dirty = dirty || !fin.all();
+    }
+    if (dirty) {
+        // the values that were replaced, to the rows that see them
+        const int psh = units.psh, pmask = units.pmask;
+        const int* table = units.table;
+        const uint16_t* vc = c.v + kvh * c.head_stride;
 #pragma unroll 1
-        for (int j = 0; j < kNarrowKeys; ++j) {
-            if (k0 + j > pos || (a.window > 0 && k0 + j <= pos - a.window)) continue;
-            const uint32_t row = ring + at + MAT + (uint32_t)j * ROWB + 8u * (uint32_t)(quad & 1);
+        for (int k0 = kNarrowKeys * begin; k0 < kNarrowKeys * end; ++k0) {
+            const int k32 = k0 & ~31;
+            if (k32 / kNarrowKeys % W != (begin + wave) % W || k0 < t.lo || k0 >= t.hi) continue;
+            if (!(k32 + 31 > t.first || (a.window > 0 && k32 <= t.last - a.window))) continue;
+            const int page = table[k0 >> psh];
+            if ((unsigned)page >= (unsigned)c.num_pages) continue;
+            const uint16_t* row = vc + (int64_t)page * c.page_stride + (int64_t)(k0 & pmask) * c.row_stride + 4 * quad;
+            const bool seen = k0 <= pos && (a.window == 0 || k0 > pos - a.window);
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                const h4 w = *(lds_h4)(row + 16u * (uint32_t)((2 * i + (quad >> 1)) ^ v_swizzle<D>(j)));
+                const h4 w = *reinterpret_cast<const h4*>(row + 16 * i), f = finite_of(w);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (!(w[e] - w[e] == (_Float16)0)) o[i][e] += (float)w[e];
+                for (int e = 0; e < 4; ++e) o[i][e] += seen ? (float)w[e] - (float)f[e] : 0.0f;
             }
         }
     }
@@ -452,13 +489,13 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
 template <int D, int NW>
 __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan,
                                           int64_t item, uint8_t* lds) {
-    constexpr int ROWB = 2 * D, MAT = kWideKeys * ROWB, STAGE = 2 * MAT, ROWS = 32 * NW;
-    constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = kWideKeys / (RPI * NW);   // a wave's instructions a matrix
+    constexpr int ROWB = 2 * D, SLOT = 32 * ROWB, VALUES = 4 * SLOT, ROWS = 32 * NW;
+    constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = 32 / (RPI * NW);    // a wave's instructions a slot
     constexpr int KS = D / 16, NB = D / 32;
     static_assert(NI >= 1, "every wave has rows to fetch");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, hi = lane >> 5;
-    const int nkv = c.num_kv_heads, psh = __ffs(c.page_size) - 1, pmask = c.page_size - 1;
+    const int nkv = c.num_kv_heads;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     const int dr = lane / LPR, ds = lane % LPR;
 
@@ -475,46 +512,42 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     const int begin = p0 + s.part * each, end = min(begin + each, p1);
     const int r = min(w0 + col, rows - 1), token = r / plan.group, head = r - token * plan.group;
     const int pos = s.kv - s.n + token;
-    const int* table = a.block_tables + (int64_t)s.b * a.max_blocks;
-    const uint16_t* kc = c.k + kvh * c.head_stride;
-    const uint16_t* vc = c.v + kvh * c.head_stride;
-
-    // page ids, 64 at a time (a tile's pages never straddle), the next ones ahead
+    // the addresses of 64 units, and the pages of the next 64
+    const Units units(a, c, s.b, kvh, t.lo, t.hi);
     bool bad = false;
-    int ids = 0, next = 0, ids_at = -1;
-    auto load_ids = [&](int at) { return table[min(max(at + lane, t.lo >> psh), (t.hi - 1) >> psh)]; };
-    auto stage = [&](int tile) {
-        const int k0 = kWideKeys * tile, at64 = (k0 >> psh) & ~63;
-        if (at64 != ids_at) {
-            ids = next;
-            const bool out = (unsigned)ids >= (unsigned)c.num_pages;
-            bad = bad || __ballot(out) != 0;
-            ids = out ? 0 : ids;
-            ids_at = at64;
-            next = load_ids(at64 + 64);
+    int next = 0, window = -1;
+    uint64_t address = 0;
+    const uint64_t v_from_k = (uint64_t)c.v - (uint64_t)c.k;
+    const uint32_t stride = (uint32_t)(2 * c.row_stride);
+    const int wave_row = RPI * wave;
+    // this wave's rows of positions 32 h .. + 31 of K or V, into slot h % 4
+    auto stage = [&](int h, bool values) {
+        if (h < 2 * begin || h >= 2 * end) return;
+        const int u0 = 4 * h;
+        if ((u0 & ~63) != window) {
+            window = u0 & ~63;
+            address = units.address(window + lane, next, bad);
+            next = units.page_of(window + 64 + lane);
         }
-        const uint32_t dst = lds0 + (uint32_t)(tile & 1) * STAGE;
-        const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
+        const uint32_t dst = lds0 + (values ? VALUES : 0) + (uint32_t)(h & 3) * SLOT + 1024u * wave;
+        const bool whole = 32 * h >= t.lo && 32 * h + 32 <= t.hi;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int g = NW * i + wave, lr = RPI * g + dr;
-            // positions that no row sees are taken from the nearest one that some row sees
-            const int at = whole ? k0 + RPI * g
-                                 : max(min(k0 + RPI * g, (t.hi - 1) & ~(RPI - 1)), t.lo & ~(RPI - 1));
-            const int back = whole ? dr : min(max(at + dr, t.lo), t.hi - 1) - at;
-            const int page = __builtin_amdgcn_readlane(ids, (at >> psh) - ids_at);
-            const int64_t off = (int64_t)page * c.page_stride + (int64_t)(at & pmask) * c.row_stride;
-            const uint32_t row = (uint32_t)back * (uint32_t)(2 * c.row_stride);
-            lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * g), row + 16u * (uint32_t)(ds ^ k_swizzle<D>(lr)),
-                      reinterpret_cast<const uint8_t*>(kc + off));
-            lds_dma16(__builtin_amdgcn_readfirstlane(dst + MAT + 1024u * g),
-                      row + 16u * (uint32_t)(ds ^ v_swizzle<D>(lr)), reinterpret_cast<const uint8_t*>(vc + off));
+            // (unit and row in it: RPI NW i is a multiple of 8)
+            const int row = wave_row + RPI * NW * i, lr = row + dr;
+            const uint32_t piece = 16u * (uint32_t)(ds ^ (values ? v_swizzle<D>(lr) : k_swizzle<D>(lr)));
+            int unit = u0 + (row >> 3);
+            uint32_t off = (uint32_t)((wave_row & 7) + dr) * stride + piece;
+            if (!whole) {
+                // positions that no row sees are taken from the nearest one that some row sees
+                unit = units.seen(unit);
+                off = (uint32_t)(min(max(32 * h + lr, t.lo), t.hi - 1) - max(8 * unit, 0)) * stride + piece;
+            }
+            const uint64_t at = read_lane(address, unit - window) + (values ? v_from_k : 0);
+            lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * NW * i), off, reinterpret_cast<const uint8_t*>(at));
         }
     };
-    if (begin < end) {
-        next = load_ids((kWideKeys * begin >> psh) & ~63);
-        stage(begin);
-    }
+    if (begin < end) next = units.page_of((8 * begin & ~63) + lane);
     // a negative scale moves its sign to Q (exact), so that the largest S has the largest weight
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
     const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
@@ -525,7 +558,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     // operand addresses: 2 k + hi = 2 k ^ hi and so on, so one base and an xor each
     const int i16 = lane & 15, vr = 4 * hi + (i16 >> 2);
     const uint32_t ka = lds0 + (uint32_t)col * ROWB + 16u * (uint32_t)(hi ^ k_swizzle<D>(col));
-    const uint32_t va = lds0 + MAT + (uint32_t)vr * ROWB +
+    const uint32_t va = lds0 + VALUES + (uint32_t)vr * ROWB +
                         16u * (uint32_t)((2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ v_swizzle<D>(vr)) +
                         8u * (uint32_t)(i16 & 1);
     f16v o[NB];
@@ -534,49 +567,49 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
     float m = kNone, l = 0.0f;
-    bool far = false;
+    bool far = false, dirty = false;
 
-    for (int tile = begin; tile < end; ++tile) {
-        // this wave's share of the tile has landed; past the barrier everyone's has, and
-        // the other buffer's reads are done
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        lds_barrier();
-        if (tile + 1 < end) stage(tile + 1);
-        const int k0 = kWideKeys * tile;
-        if (!active || k0 > u.last || (a.window > 0 && k0 + kWideKeys - 1 <= u.first - a.window)) continue;
-        const uint32_t at = (uint32_t)(tile & 1) * STAGE;
+    // S^T of a tile; beside(k): what is done beside k-step k's two products
+    auto scores = [&](int tile, f16v (&y)[2], auto beside) {
         // (opaque, so that a tile's addresses are not kept in registers over the loop)
-        uint32_t kt = ka + at, vt = va + at;
-        asm("" : "+v"(kt), "+v"(vt));
-        f16v x[2];
+        uint32_t kt = ka + (uint32_t)(tile & 1) * (2 * SLOT);
+        asm("" : "+v"(kt));
+        auto k_frag = [&](int k, int b) { return *(lds_h8)((kt ^ (32u * k)) + SLOT * b); };
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[b][e] = 0.0f;
+            for (int e = 0; e < 16; ++e) y[b][e] = 0.0f;
+        constexpr int AHEAD = 2;
+        h8 kf[AHEAD + 1][2];
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) kf[k][b] = k_frag(k, b);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            if (k + AHEAD < KS)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) kf[(k + AHEAD) % (AHEAD + 1)][b] = k_frag(k + AHEAD, b);
 #pragma unroll
             for (int b = 0; b < 2; ++b)
-                x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(lds_h8)((kt ^ (32u * k)) + 32u * b * ROWB), q[k],
-                                                              x[b], 0, 0, 0);
+                y[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k % (AHEAD + 1)][b], q[k], y[b], 0, 0, 0);
+            beside(k);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // The softmax of x, a tile's scores, beside the next tile's, and its product with V
+    auto step = [&](auto mask, int tile, f16v (&x)[2], f16v (&y)[2]) {
+        constexpr bool masked = decltype(mask)::value;
+        const int k0 = kWideKeys * tile;
+        uint32_t vt = va + (uint32_t)(tile & 1) * (2 * SLOT);
+        asm("" : "+v"(vt));
         // V^T (k-step j, dims 32 i ..): lane (dim 32 i + col) takes keys 16 j + 4 hi + {0 .. 3, 8 .. 11}, as
         // the weights' registers hold them
         auto v_frag = [&](int j, int i) {
             const uint32_t v = (vt ^ (64u * i)) + 16u * j * ROWB;
             return join(read_tr(v), read_tr(v + 8u * ROWB));
         };
-        const bool masked = k0 + kWideKeys - 1 > u.first || (a.window > 0 && k0 <= u.last - a.window);
-        // (all of V's operands before the softmax where the registers allow it: in flight meanwhile)
-        constexpr int JG = D <= 128 ? 4 : 1;
-        h8 v[JG][NB];
-        if constexpr (JG == 4) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < NB; ++i) v[j][i] = v_frag(j, i);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if (masked) {
+        if constexpr (masked) {
             const int ahead = pos - k0 - 4 * hi, behind = a.window > 0 ? ahead - a.window : INT_MIN;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -613,50 +646,100 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
                 mul = 1.0f;
             }
         }
+        // (past the last tile of K the scores are of what the ring holds, and are not used)
+        scores(tile + 1, y, [&](int k) {
+            constexpr int N = 32 / KS;
+#pragma unroll
+            for (int e = N * k; e < N * (k + 1); ++e) {
+                float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 4][e & 15], mul, -m));
+                asm volatile("" : "+v"(w));      // here, not where it is used
+                x[e >> 4][e & 15] = w;
+            }
+        });
         h8 p[4];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                p[2 * b + (e >> 3)][e & 7] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[b][e], mul, -m));
+        for (int e = 0; e < 32; ++e) p[e >> 3][e & 7] = (_Float16)x[e >> 4][e & 15];
 #pragma unroll
         for (int j = 0; j < 4; ++j) l = sum8(p[j], l);
         // infinities and NaN among values that some rows do not see must not meet their zero
-        // weights: finite ones take their place, and the rows that see them get them by an addition
-        Finite fin;
+        // weights: finite ones take their place, and the rows that see them get them at the end
+        if constexpr (!masked) {
 #pragma unroll
-        for (int j0 = 0; j0 < 4; j0 += JG) {
-            if constexpr (JG < 4)
-#pragma unroll
-                for (int i = 0; i < NB; ++i) v[0][i] = v_frag(j0, i);
-            if (masked) {
-#pragma unroll
-                for (int j = 0; j < JG; ++j)
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) {
-                        fin.take(v[j][i]);
-                        v[j][i] = finite_of(v[j][i]);
-                    }
-            }
-#pragma unroll
-            for (int j = 0; j < JG; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int i = 0; i < NB; ++i)
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[j][i], p[j0 + j], o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(j, i), p[j], o[i], 0, 0, 0);
+        } else {
+            Finite fin;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    const h8 v = v_frag(j, i);
+                    fin.take(v);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_of(v), p[j], o[i], 0, 0, 0);
+                }
+            dirty = dirty || !fin.all();
         }
-        if (!masked || fin.all()) continue;
+    };
+
+    // K runs a tile ahead of V.  At a tile's start this wave's share
+    // of what its step reads has landed; past the barrier everyone's has, and the slots that
+    // are filled next have been read.
+    auto advance = [&](int tile) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();
 #pragma unroll 1
-        for (int j = 0; j < kWideKeys; ++j) {
-            if (k0 + j > pos || (a.window > 0 && k0 + j <= pos - a.window)) continue;
-            const uint32_t row = lds0 + at + MAT + (uint32_t)j * ROWB + 8u * (uint32_t)hi;
+        for (int w = 0; w < 4; ++w) stage(2 * tile + 2 + w, w < 2);
+    };
+    // the tiles that this wave's rows see, and among them those that all its rows see whole
+    const int mine = active ? min(max(u.lo / kWideKeys, begin), end) : end;
+    const int mine_end = active ? max(min((u.hi + kWideKeys - 1) / kWideKeys, end), mine) : end;
+    const int behind = a.window > 0 ? max(u.last - a.window + kWideKeys, 0) / kWideKeys : 0;
+    const int full = min(max(behind, mine), mine_end);
+    const int full_end = min(max((u.first + 1) >> 6, full), mine_end);
+    int tile = begin - 2;
+#pragma unroll 1
+    for (; tile < mine - 1; ++tile) advance(tile);
+    if (mine < mine_end) {
+        f16v x[2], y[2];
+        advance(tile++);
+        scores(mine, x, [](int) {});
+        auto run = [&](auto mask, int to) {
+#pragma unroll 1
+            for (; tile < to; ++tile) {
+                advance(tile);
+                step(mask, tile, x, y);
+                x[0] = y[0];
+                x[1] = y[1];
+            }
+        };
+        run(std::true_type(), full);
+        run(std::false_type(), full_end);
+        run(std::true_type(), mine_end);
+    }
+#pragma unroll 1
+    for (; tile < end; ++tile) advance(tile);
+    if (dirty) {
+        // the values that were replaced, to the rows that see them
+        const int psh = units.psh, pmask = units.pmask;
+        const int* table = units.table;
+        const uint16_t* vc = c.v + kvh * c.head_stride;
+#pragma unroll 1
+        for (int k0 = kWideKeys * begin; k0 < kWideKeys * end; ++k0) {
+            const int k32 = k0 & ~31;
+            if (!(k32 + 31 > u.first || (a.window > 0 && k32 <= u.last - a.window)) || k0 < t.lo || k0 >= t.hi) continue;
+            const int page = table[k0 >> psh];
+            if ((unsigned)page >= (unsigned)c.num_pages) continue;
+            const uint16_t* row = vc + (int64_t)page * c.page_stride + (int64_t)(k0 & pmask) * c.row_stride + 4 * hi;
+            const bool seen = k0 <= pos && (a.window == 0 || k0 > pos - a.window);
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int e4 = 0; e4 < 4; ++e4) {
-                    const h4 w = *(lds_h4)(row + 16u * (uint32_t)((4 * i + e4) ^ v_swizzle<D>(j)));
+                    const h4 w = *reinterpret_cast<const h4*>(row + 32 * i + 8 * e4), f = finite_of(w);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!(w[e] - w[e] == (_Float16)0)) o[i][4 * e4 + e] += (float)w[e];
+                    for (int e = 0; e < 4; ++e) o[i][4 * e4 + e] += seen ? (float)w[e] - (float)f[e] : 0.0f;
                 }
         }
     }
@@ -703,7 +786,7 @@ template <> struct Shape<256> { static constexpr int W = 2, S = 2, NW = 4, MW = 
 template <int D>
 constexpr int narrow_lds(int w, int s) { return w * s * 2 * kNarrowKeys * 2 * D; }
 template <int D>
-constexpr int wide_lds() { return 2 * 2 * kWideKeys * 2 * D; }
+constexpr int wide_lds() { return 2 * 4 * 32 * 2 * D; }
 template <int D>
 constexpr int wide_rows() { return 32 * Shape<D>::NW; }
 
