@@ -489,8 +489,8 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
 template <int D, int NW>
 __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan,
                                           int64_t item, uint8_t* lds) {
-    constexpr int ROWB = 2 * D, SLOT = 32 * ROWB, VALUES = 4 * SLOT, ROWS = 32 * NW;
-    constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = 32 / (RPI * NW);    // a wave's instructions a slot
+    constexpr int ROWB = 2 * D, MAT = kWideKeys * ROWB, ROWS = 32 * NW;
+    constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = kWideKeys / (RPI * NW);   // a wave's instructions a tile
     constexpr int KS = D / 16, NB = D / 32;
     static_assert(NI >= 1, "every wave has rows to fetch");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -520,30 +520,34 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     const uint64_t v_from_k = (uint64_t)c.v - (uint64_t)c.k;
     const uint32_t stride = (uint32_t)(2 * c.row_stride);
     const int wave_row = RPI * wave;
-    // this wave's rows of positions 32 h .. + 31 of K or V, into slot h % 4
-    auto stage = [&](int h, bool values) {
-        if (h < 2 * begin || h >= 2 * end) return;
-        const int u0 = 4 * h;
-        if ((u0 & ~63) != window) {
-            window = u0 & ~63;
+    const uint32_t lane_row = (uint32_t)((wave_row & 7) + dr) * stride;
+    // this wave's rows of a tile of K or V into its buffer; K goes first and moves the window
+    auto stage = [&](auto which, int tile) {
+        constexpr bool values = decltype(which)::value;
+        if (tile < begin || tile >= end) return;
+        const int k0 = kWideKeys * tile;
+        if (!values && (8 * tile & ~63) != window) {
+            window = 8 * tile & ~63;
             address = units.address(window + lane, next, bad);
             next = units.page_of(window + 64 + lane);
         }
-        const uint32_t dst = lds0 + (values ? VALUES : 0) + (uint32_t)(h & 3) * SLOT + 1024u * wave;
-        const bool whole = 32 * h >= t.lo && 32 * h + 32 <= t.hi;
+        const uint32_t dst = lds0 + (values ? 2 * MAT : 0) + (uint32_t)(tile & 1) * MAT + 1024u * wave;
+        const int u0 = 8 * tile - window;
+        const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            // (unit and row in it: RPI NW i is a multiple of 8)
+            // (RPI NW i is a multiple of 8: a lane's row in its unit is the same in each)
             const int row = wave_row + RPI * NW * i, lr = row + dr;
             const uint32_t piece = 16u * (uint32_t)(ds ^ (values ? v_swizzle<D>(lr) : k_swizzle<D>(lr)));
             int unit = u0 + (row >> 3);
-            uint32_t off = (uint32_t)((wave_row & 7) + dr) * stride + piece;
+            uint32_t off = lane_row + piece;
             if (!whole) {
                 // positions that no row sees are taken from the nearest one that some row sees
-                unit = units.seen(unit);
-                off = (uint32_t)(min(max(32 * h + lr, t.lo), t.hi - 1) - max(8 * unit, 0)) * stride + piece;
+                unit = units.seen(unit + window);
+                off = (uint32_t)(min(max(k0 + lr, t.lo), t.hi - 1) - 8 * unit) * stride + piece;
+                unit -= window;
             }
-            const uint64_t at = read_lane(address, unit - window) + (values ? v_from_k : 0);
+            const uint64_t at = read_lane(address, unit) + (values ? v_from_k : 0);
             lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * NW * i), off, reinterpret_cast<const uint8_t*>(at));
         }
     };
@@ -558,7 +562,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     // operand addresses: 2 k + hi = 2 k ^ hi and so on, so one base and an xor each
     const int i16 = lane & 15, vr = 4 * hi + (i16 >> 2);
     const uint32_t ka = lds0 + (uint32_t)col * ROWB + 16u * (uint32_t)(hi ^ k_swizzle<D>(col));
-    const uint32_t va = lds0 + VALUES + (uint32_t)vr * ROWB +
+    const uint32_t va = lds0 + 2 * MAT + (uint32_t)vr * ROWB +
                         16u * (uint32_t)((2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ v_swizzle<D>(vr)) +
                         8u * (uint32_t)(i16 & 1);
     f16v o[NB];
@@ -572,9 +576,9 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     // S^T of a tile; beside(k): what is done beside k-step k's two products
     auto scores = [&](int tile, f16v (&y)[2], auto beside) {
         // (opaque, so that a tile's addresses are not kept in registers over the loop)
-        uint32_t kt = ka + (uint32_t)(tile & 1) * (2 * SLOT);
+        uint32_t kt = ka + (uint32_t)(tile & 1) * MAT;
         asm("" : "+v"(kt));
-        auto k_frag = [&](int k, int b) { return *(lds_h8)((kt ^ (32u * k)) + SLOT * b); };
+        auto k_frag = [&](int k, int b) { return *(lds_h8)((kt ^ (32u * k)) + 32u * b * ROWB); };
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -601,7 +605,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     auto step = [&](auto mask, int tile, f16v (&x)[2], f16v (&y)[2]) {
         constexpr bool masked = decltype(mask)::value;
         const int k0 = kWideKeys * tile;
-        uint32_t vt = va + (uint32_t)(tile & 1) * (2 * SLOT);
+        uint32_t vt = va + (uint32_t)(tile & 1) * MAT;
         asm("" : "+v"(vt));
         // V^T (k-step j, dims 32 i ..): lane (dim 32 i + col) takes keys 16 j + 4 hi + {0 .. 3, 8 .. 11}, as
         // the weights' registers hold them
@@ -646,7 +650,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
                 mul = 1.0f;
             }
         }
-        // (past the last tile of K the scores are of what the ring holds, and are not used)
+        // (past the last tile of K the scores are of what its buffer holds, and are not used)
         scores(tile + 1, y, [&](int k) {
             constexpr int N = 32 / KS;
 #pragma unroll
@@ -684,13 +688,13 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     };
 
     // K runs a tile ahead of V.  At a tile's start this wave's share
-    // of what its step reads has landed; past the barrier everyone's has, and the slots that
-    // are filled next have been read.
+    // of what its step reads has landed; past the barrier everyone's has, and the buffers
+    // that are filled next have been read.
     auto advance = [&](int tile) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();
-#pragma unroll 1
-        for (int w = 0; w < 4; ++w) stage(2 * tile + 2 + w, w < 2);
+        stage(std::true_type(), tile + 1);
+        stage(std::false_type(), tile + 2);
     };
     // the tiles that this wave's rows see, and among them those that all its rows see whole
     const int mine = active ? min(max(u.lo / kWideKeys, begin), end) : end;
@@ -786,7 +790,7 @@ template <> struct Shape<256> { static constexpr int W = 2, S = 2, NW = 4, MW = 
 template <int D>
 constexpr int narrow_lds(int w, int s) { return w * s * 2 * kNarrowKeys * 2 * D; }
 template <int D>
-constexpr int wide_lds() { return 2 * 4 * 32 * 2 * D; }
+constexpr int wide_lds() { return 4 * kWideKeys * 2 * D; }
 template <int D>
 constexpr int wide_rows() { return 32 * Shape<D>::NW; }
 
