@@ -651,20 +651,34 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
             }
         }
         // (past the last tile of K the scores are of what its buffer holds, and are not used)
+        u32x4 w[4];                              // the weights, two in a register
+        h8 v[2][NB];                             // V's operands of k-steps 0 and 1: in flight meanwhile
         scores(tile + 1, y, [&](int k) {
             constexpr int N = 32 / KS;
 #pragma unroll
-            for (int e = N * k; e < N * (k + 1); ++e) {
-                float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 4][e & 15], mul, -m));
-                asm volatile("" : "+v"(w));      // here, not where it is used
-                x[e >> 4][e & 15] = w;
+            for (int e = N * k; e < N * (k + 1); e += 2) {
+                float f[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    f[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 4][(e & 15) + i], mul, -m));
+                w[e >> 3][(e >> 1) & 3] = __builtin_bit_cast(uint32_t, h2{(_Float16)f[0], (_Float16)f[1]});
+                asm volatile("" : "+v"(w[e >> 3][(e >> 1) & 3]));        // here, not where it is used
+            }
+            if constexpr (D <= 128) {
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    if (k == KS - 3) v[0][i] = v_frag(0, i);
+                    if (k == KS - 2) v[1][i] = v_frag(1, i);
+                }
             }
         });
         h8 p[4];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) p[e >> 3][e & 7] = (_Float16)x[e >> 4][e & 15];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) l = sum8(p[j], l);
+        for (int j = 0; j < 4; ++j) {
+            p[j] = __builtin_bit_cast(h8, w[j]);
+            l = sum8(p[j], l);
+        }
+        auto operand = [&](int j, int i) { return D <= 128 && j < 2 ? v[j][i] : v_frag(j, i); };
         // infinities and NaN among values that some rows do not see must not meet their zero
         // weights: finite ones take their place, and the rows that see them get them at the end
         if constexpr (!masked) {
@@ -672,16 +686,16 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int i = 0; i < NB; ++i)
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(j, i), p[j], o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand(j, i), p[j], o[i], 0, 0, 0);
         } else {
             Finite fin;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
-                    const h8 v = v_frag(j, i);
-                    fin.take(v);
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_of(v), p[j], o[i], 0, 0, 0);
+                    const h8 f = operand(j, i);
+                    fin.take(f);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_of(f), p[j], o[i], 0, 0, 0);
                 }
             dirty = dirty || !fin.all();
         }
@@ -709,13 +723,20 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         f16v x[2], y[2];
         advance(tile++);
         scores(mine, x, [](int) {});
+        // (whole tiles in pairs, so that x and y change places without copies)
         auto run = [&](auto mask, int to) {
+            constexpr bool pairs = !decltype(mask)::value;
 #pragma unroll 1
             for (; tile < to; ++tile) {
                 advance(tile);
                 step(mask, tile, x, y);
-                x[0] = y[0];
-                x[1] = y[1];
+                if (pairs && tile + 1 < to) {
+                    advance(++tile);
+                    step(mask, tile, y, x);
+                } else {
+                    x[0] = y[0];
+                    x[1] = y[1];
+                }
             }
         };
         run(std::true_type(), full);
