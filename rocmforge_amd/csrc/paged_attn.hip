@@ -53,7 +53,7 @@ constexpr int kWideKeys = 64;
 // keys.  A tile is cut only where its share is longer than total / parts, so at
 // most twice as many parts are written to the workspace.
 constexpr int kNarrowParts = 512, kNarrowLeast = 4;
-constexpr int kWideParts = 512, kWideLeast = 8;
+constexpr int kWideLeast = 8;                    // (as many parts as workgroups fit the chip)
 
 // ---- which part of which request a workgroup does ---------------------------------------
 
@@ -652,7 +652,14 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         }
         // (past the last tile of K the scores are of what its buffer holds, and are not used)
         u32x4 w[4];                              // the weights, two in a register
-        h8 v[2][NB];                             // V's operands of k-steps 0 and 1: in flight meanwhile
+        // V's operands, in fours: those of the first products are read beside the scores, the others
+        // two fours ahead
+        constexpr int FOURS = NB, AHEAD = FOURS < 2 ? FOURS : 2;
+        h8 v[AHEAD + 1][4];
+        auto read_four = [&](int f) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[f % (AHEAD + 1)][i] = v_frag((4 * f + i) / NB, (4 * f + i) % NB);
+        };
         scores(tile + 1, y, [&](int k) {
             constexpr int N = 32 / KS;
 #pragma unroll
@@ -664,13 +671,9 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
                 w[e >> 3][(e >> 1) & 3] = __builtin_bit_cast(uint32_t, h2{(_Float16)f[0], (_Float16)f[1]});
                 asm volatile("" : "+v"(w[e >> 3][(e >> 1) & 3]));        // here, not where it is used
             }
-            if constexpr (D <= 128) {
 #pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    if (k == KS - 3) v[0][i] = v_frag(0, i);
-                    if (k == KS - 2) v[1][i] = v_frag(1, i);
-                }
-            }
+            for (int f = 0; f < AHEAD; ++f)
+                if (k == KS - 1 - AHEAD + f) read_four(f);
         });
         h8 p[4];
 #pragma unroll
@@ -678,27 +681,25 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
             p[j] = __builtin_bit_cast(h8, w[j]);
             l = sum8(p[j], l);
         }
-        auto operand = [&](int j, int i) { return D <= 128 && j < 2 ? v[j][i] : v_frag(j, i); };
         // infinities and NaN among values that some rows do not see must not meet their zero
         // weights: finite ones take their place, and the rows that see them get them at the end
-        if constexpr (!masked) {
+        Finite fin;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int f = 0; f < FOURS; ++f) {
+            if (f + AHEAD < FOURS) read_four(f + AHEAD);
 #pragma unroll
-                for (int i = 0; i < NB; ++i)
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand(j, i), p[j], o[i], 0, 0, 0);
-        } else {
-            Finite fin;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    const h8 f = operand(j, i);
-                    fin.take(f);
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(finite_of(f), p[j], o[i], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+                const int j = (4 * f + i) / NB, d = (4 * f + i) % NB;
+                h8 b = v[f % (AHEAD + 1)][i];
+                if constexpr (masked) {
+                    fin.take(b);
+                    b = finite_of(b);
                 }
-            dirty = dirty || !fin.all();
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, p[j], o[d], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (masked) dirty = dirty || !fin.all();
     };
 
     // K runs a tile ahead of V.  At a tile's start this wave's share
@@ -814,6 +815,8 @@ template <int D>
 constexpr int wide_lds() { return 4 * kWideKeys * 2 * D; }
 template <int D>
 constexpr int wide_rows() { return 32 * Shape<D>::NW; }
+template <int D>
+constexpr int wide_parts() { return 256 * Shape<D>::EU; }
 
 template <int D>
 __global__ __launch_bounds__(64 * Shape<D>::W)
@@ -917,7 +920,7 @@ __global__ __launch_bounds__(256) void rf_paged_attn_join_kernel(const rf_paged_
 template <int D>
 static constexpr size_t narrow_bytes() { return (size_t)2 * rf::kNarrowParts * rf::kNarrowRows * (D + 2) * sizeof(float); }
 template <int D>
-static constexpr size_t wide_bytes() { return (size_t)2 * rf::kWideParts * rf::wide_rows<D>() * (D + 2) * sizeof(float); }
+static constexpr size_t wide_bytes() { return (size_t)2 * rf::wide_parts<D>() * rf::wide_rows<D>() * (D + 2) * sizeof(float); }
 
 extern "C" size_t rf_paged_attention_workspace_bytes(int num_heads, int num_kv_heads, int head_dim) {
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0) return 0;
@@ -938,7 +941,7 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
     const bool both = (int64_t)a.max_new * group > kNarrowRows;
     float* ws = static_cast<float*>(a.workspace);
     Plan narrow = {group, 0, both ? kNarrowRows : INT_MAX, kNarrowParts, kNarrowLeast, 0, ws};
-    Plan wide = {group, kNarrowRows, INT_MAX, kWideParts, kWideLeast, 0, ws + narrow_bytes<D>() / sizeof(float)};
+    Plan wide = {group, kNarrowRows, INT_MAX, wide_parts<D>(), kWideLeast, 0, ws + narrow_bytes<D>() / sizeof(float)};
     // Items: every tile has a part, and there are at most `parts` parts more (each of them a share
     // long); no more either than the table's width gives room for.
     const auto items = [&](int64_t tiles, const Plan& p, int keys, int64_t* joins) {
