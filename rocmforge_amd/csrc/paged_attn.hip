@@ -800,8 +800,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
 
 // ---- the launches -------------------------------------------------------------------------
 
-constexpr int kJoinRows = 16;
-constexpr int kJoinParts = kNarrowParts + 1;     // of a tile, at most
+constexpr int kJoinRows = 32, kJoinParts = 64;
 
 // Head dims, waves and stages of the narrow part, waves of the wide one.
 // (MW, MS: of the narrow part beside wide ones)
@@ -841,64 +840,68 @@ void rf_paged_attn_mixed_kernel(const rf_paged_attention a, const rf_paged_cache
     }
 }
 
-// Joins 16 rows of a tile of several parts: the parts' weights 2^(m - max m)
-// through LDS, then each output over the parts, by as many threads as there are
-// for it.
+// Joins kJoinRows rows of a tile of several parts: the parts' weights 2^(m - max m)
+// through LDS, 64 parts at a time, and each output over the parts, by as many
+// threads as there are for it.
 template <int D, int ROWS, int KEYS>
 __device__ __forceinline__ void join_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan, int item,
                                           float (*weight)[kJoinRows], f4* sums) {
-    constexpr int SUB = ROWS / kJoinRows;
+    constexpr int JR = ROWS < kJoinRows ? ROWS : kJoinRows, SUB = ROWS / JR, LANES = 256 / JR;
+    constexpr int PER = JR * (D / 4) / 256 > 1 ? JR * (D / 4) / 256 : 1;       // outputs a thread, of four
     const int nkv = c.num_kv_heads, tid = threadIdx.x;
-    const int first = kJoinRows * (item % SUB), kvh = item / SUB % nkv;
+    const int first = JR * (item % SUB), kvh = item / SUB % nkv;
     Share s;
     if (!find_share<ROWS, KEYS>(a, c, plan, item / SUB / nkv, true, s)) return;
     const int rows = s.n * plan.group, r0 = ROWS * s.tile;
-    const int live = min(rows - r0 - first, kJoinRows);
+    const int live = min(rows - r0 - first, JR);
     if (live <= 0) return;
     const int64_t next = (int64_t)s.tiles * nkv * (ROWS * (D + 2));
     const float* part0 = slot_of<ROWS, D>(plan.slots, s, 0, kvh, nkv) + first * D;
     const float* m0 = part0 + (ROWS - first) * D + first;
-    {
-        const int row = tid / 16;                // 16 lanes a row
-        float mx = kNone, sum = 0.0f;
-        if (row < live) {
-            for (int k = tid % 16; k < s.parts; k += 16) mx = fmaxf(mx, m0[k * next + row]);
-            mx = xor_max<8, 1>(mx);
-            for (int k = tid % 16; k < s.parts; k += 16) {
-                const float f = __builtin_amdgcn_exp2f(m0[k * next + row] - mx);
-                weight[k][row] = f;
-                sum += m0[k * next + ROWS + row] * f;
-            }
-            sum = xor_sum<8, 1>(sum);
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            for (int k = tid % 16; k < s.parts; k += 16) weight[k][row] *= inv;
-        }
-    }
-    __syncthreads();
+    const int row = tid / LANES;                 // LANES lanes a row
+    float mx = kNone, sum = 0.0f;
+    if (row < live)
+        for (int k = tid % LANES; k < s.parts; k += LANES) mx = fmaxf(mx, m0[k * next + row]);
+    mx = xor_max<LANES / 2, 1>(mx);
     const int outs = live * (D / 4), groups = max(256 / outs, 1);
-    for (int o0 = 0; o0 < outs; o0 += 256) {
-        const int g = groups == 1 ? 0 : tid / outs, i = groups == 1 ? o0 + tid : tid - g * outs;
-        f4 acc = {0, 0, 0, 0};
-        if (g < groups && i < outs) {
-            const int row = i / (D / 4);
-#pragma unroll 4
-            for (int k = g; k < s.parts; k += groups) {
-                const float f = weight[k][row];
-                const f4 v = *reinterpret_cast<const f4*>(part0 + k * next + 4 * i);
-                acc += v * f;
+    const int g = groups == 1 ? 0 : tid / outs, i0 = groups == 1 ? tid : tid - g * outs;
+    f4 acc[PER];
+#pragma unroll
+    for (int o = 0; o < PER; ++o) acc[o] = f4{0, 0, 0, 0};
+    for (int k0 = 0; k0 < s.parts; k0 += kJoinParts) {
+        const int n = min(s.parts - k0, kJoinParts);
+        if (k0 > 0) __syncthreads();             // the last weights are read
+        if (row < live)
+            for (int k = tid % LANES; k < n; k += LANES) {
+                const float f = __builtin_amdgcn_exp2f(m0[(k0 + k) * next + row] - mx);
+                weight[k][row] = f;
+                sum += m0[(k0 + k) * next + ROWS + row] * f;
             }
-        }
-        if (groups > 1) {
-            sums[tid] = acc;
-            __syncthreads();
-            if (tid < outs)
-                for (int k = 1; k < groups; ++k) acc += sums[tid + k * outs];
-        }
-        if (i < outs && g == 0) {
-            const int row = r0 + first + i / (D / 4), d = 4 * (i % (D / 4));
-            const int tk = row / plan.group, hd = row - tk * plan.group;
-            store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d, acc);
-        }
+        __syncthreads();
+        if (g < groups)
+#pragma unroll
+            for (int o = 0; o < PER; ++o) {
+                const int i = i0 + 256 * o;
+                if (i >= outs) continue;
+#pragma unroll 4
+                for (int k = g; k < n; k += groups)
+                    acc[o] += *reinterpret_cast<const f4*>(part0 + (k0 + k) * next + 4 * i) * weight[k][i / (D / 4)];
+            }
+    }
+    sum = xor_sum<LANES / 2, 1>(sum);
+    __syncthreads();
+    if (row < live && tid % LANES == 0) weight[0][row] = sum == 0.0f ? 0.0f : 1.0f / sum;
+    sums[tid] = acc[0];
+    __syncthreads();
+    if (g > 0) return;
+#pragma unroll
+    for (int o = 0; o < PER; ++o) {
+        const int i = i0 + 256 * o;
+        if (i >= outs) continue;
+        for (int k = 1; k < groups; ++k) acc[o] += sums[tid + k * outs];
+        const int at = r0 + first + i / (D / 4), d = 4 * (i % (D / 4));
+        const int tk = at / plan.group, hd = at - tk * plan.group;
+        store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d, acc[o] * weight[0][i / (D / 4)]);
     }
 }
 
