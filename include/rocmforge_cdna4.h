@@ -780,7 +780,8 @@ hipError_t rf_paged_rope_write_launch(const rf_paged_rope* step, const rf_paged_
  * outside the cache is read.  workspace: rf_paged_attention_workspace_bytes
  * bytes, 16-byte aligned (launches that share one must be stream-ordered).
  * q, out 16-byte aligned, ld_q, ld_out multiples of 8; scale finite; window >= 0;
- * num_heads a multiple of num_kv_heads, at most 64 of them a KV head. */
+ * num_heads a multiple of num_kv_heads, at most 64 of them a KV head; rows *
+ * num_heads <= 2^27. */
 typedef struct rf_paged_attention {
     const uint16_t* q;
     void* out;

@@ -53,7 +53,7 @@ constexpr int kWideKeys = 64;
 // keys.  A tile is cut only where its share is longer than total / parts, so at
 // most twice as many parts are written to the workspace.
 constexpr int kNarrowParts = 512, kNarrowLeast = 4;
-constexpr int kWideLeast = 8;                    // (as many parts as workgroups fit the chip)
+constexpr int kWideLeast = 16;                   // (as many parts as workgroups fit the chip)
 
 // ---- which part of which request a workgroup does ---------------------------------------
 
@@ -67,11 +67,16 @@ struct Share {
 // What the host knows of a launch.
 struct Plan {
     int group;
+    uint32_t group_inv;          // 2^32 / group rounded up where r / group is the high word of r group_inv, else 0
     int from_rows, to_rows;      // requests of from_rows < packed rows <= to_rows are this kernel's
     int parts, least;
-    int64_t items;               // at least as many as there are
+    int items;                   // at least as many as there are
     float* slots;                // the parts' states
 };
+
+__device__ __forceinline__ int token_of(const Plan& p, int r) {
+    return p.group == 1 ? r : p.group_inv ? (int)__umulhi((uint32_t)r, p.group_inv) : r / p.group;
+}
 
 struct Request {
     int q0, n, kv, tiles, units;
@@ -93,13 +98,15 @@ __device__ __forceinline__ Request request_of(const rf_paged_attention& a, const
     return r;
 }
 
-__device__ __forceinline__ int wave_scan(int v) {        // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o);
-        if (lane >= o) v += u;
-    }
+// Inclusive prefix sum over the wave: within rows of 16 lanes, then the rows' last lanes
+// into the rows behind them.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);      // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);      // row_bcast 15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);      // row_bcast 31 into rows 2 and 3
     return v;
 }
 
@@ -153,10 +160,10 @@ struct Span {
     int first, last;             // positions of the first and the last row
     int lo, hi;
 };
-__device__ __forceinline__ Span span_of(const Share& s, int r0, int r1, int group, int window) {
+__device__ __forceinline__ Span span_of(const Plan& p, const Share& s, int r0, int r1, int window) {
     Span t;
-    t.first = s.kv - s.n + r0 / group;
-    t.last = s.kv - s.n + r1 / group;
+    t.first = s.kv - s.n + token_of(p, r0);
+    t.last = s.kv - s.n + token_of(p, r1);
     t.hi = max(t.last + 1, 0);
     t.lo = window > 0 ? (int)max((int64_t)t.first - window + 1, (int64_t)0) : 0;
     return t;
@@ -267,7 +274,7 @@ __device__ __forceinline__ V finite_of(V v) {
 // piece (head_dim 128), 64 KB and more in flight a CU.
 template <int D, int W, int S>
 __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan,
-                                            int64_t item, uint8_t* lds) {
+                                            int item, uint8_t* lds) {
     constexpr int ROWB = 2 * D, MAT = kNarrowKeys * ROWB, STAGE = 2 * MAT;
     constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = kNarrowKeys / RPI;   // instructions a matrix
     constexpr int KS = D / 32, NB = D / 16;
@@ -281,17 +288,17 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
     const int dr = lane / LPR, ds = lane % LPR;
 
     Share s;
-    const int kvh = (int)(item % nkv);
-    if (!find_share<kNarrowRows, kNarrowKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
+    const int kvh = item % nkv;
+    if (!find_share<kNarrowRows, kNarrowKeys>(a, c, plan, item / nkv, false, s)) return;
     const int rows = s.n * plan.group, r0 = kNarrowRows * s.tile;
-    const Span t = span_of(s, r0, min(r0 + kNarrowRows, rows) - 1, plan.group, a.window);
+    const Span t = span_of(plan, s, r0, min(r0 + kNarrowRows, rows) - 1, a.window);
     // the part's pieces
     const int p0 = t.lo / kNarrowKeys, p1 = (t.hi + kNarrowKeys - 1) / kNarrowKeys;
     const int each = (max(p1 - p0, 0) + s.parts - 1) / s.parts;
     const int begin = p0 + s.part * each, end = min(begin + each, p1);
     const int steps = max((end - begin - wave + W - 1) / W, 0);
     // this lane's packed row
-    const int r = r0 + col, token = min(r, rows - 1) / plan.group, head = min(r, rows - 1) - token * plan.group;
+    const int r = r0 + col, token = token_of(plan, min(r, rows - 1)), head = min(r, rows - 1) - token * plan.group;
     const int pos = s.kv - s.n + token;
     // the addresses of the units of 16 pieces to come, lane (step, unit of the piece)
     const Units units(a, c, s.b, kvh, t.lo, t.hi);
@@ -395,25 +402,29 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
 #pragma unroll
             for (int e = 0; e < 4; ++e) p[4 * b + e] = (_Float16)__builtin_amdgcn_exp2f(x[b][e] - m);
         l = sum8(p, l);
-        // V^T: lane (dim 16 i + col) takes keys 4 quad + {0 .. 3, 16 .. 19}, as p holds them
-        h8 v[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const uint32_t row = vt ^ (32u * i);
-            v[i] = join(read_tr(row), read_tr(row + 16u * ROWB));
-        }
-        // infinities and NaN among values that some rows do not see must not meet their zero
-        // weights: finite ones take their place, and the rows that see them get them at the end
+        // V^T: lane (dim 16 i + col) takes keys 4 quad + {0 .. 3, 16 .. 19}, as p holds them.
+        // Infinities and NaN among values that some rows do not see must not meet their zero
+        // weights: finite ones take their place, and the rows that see them get them at the end.
         Finite fin;
-        if (masked) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                fin.take(v[i]);
-                v[i] = finite_of(v[i]);
+        for (int i0 = 0; i0 < NB; i0 += 4) {
+            h8 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t row = vt ^ (32u * (i0 + i));
+                v[i] = join(read_tr(row), read_tr(row + 16u * ROWB));
             }
-        }
+            if (masked) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i], p, o[i], 0, 0, 0);
+                for (int i = 0; i < 4; ++i) {
+                    fin.take(v[i]);
+                    v[i] = finite_of(v[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                o[i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i], p, o[i0 + i], 0, 0, 0);
+        }
         if (masked) dirty = dirty || !fin.all();
     }
     if (dirty) {
@@ -474,7 +485,7 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
                 part[kNarrowRows * (D + 1) + row] = sum;
             }
         } else {
-            const int tk = (r0 + row) / plan.group, hd = r0 + row - tk * plan.group;
+            const int tk = token_of(plan, r0 + row), hd = r0 + row - tk * plan.group;
             store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d,
                    sum == 0.0f ? f4{0, 0, 0, 0} : acc * (1.0f / sum));
         }
@@ -483,34 +494,63 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
 
 // ---- pieces of prompt -------------------------------------------------------------------
 //
-// NW waves of 32 packed rows each over tiles of 64 positions, K and V by LDS
-// DMA, double buffered, one barrier a tile: S^T by 32x32x16 MFMAs (two blocks of
-// 32 keys), lane (row lane % 32, keys 8 (e / 4) + 4 (lane / 32) + e % 4).
-template <int D, int NW>
+// NW waves of M packed rows each over tiles of 64 positions, K and V by LDS
+// DMA, double buffered, one barrier a tile.  The scores of a tile are computed
+// beside the weights of the one before (MFMA beside exp), so K runs a tile ahead.
+// M = 32 where a wave's queries and outputs fit its registers (head_dim 64 and
+// 128); at 256 they would take 192 of them, and M = 16 has two waves a SIMD.
+
+// The two MFMA shapes.  M packed rows a wave; acc: a block of scores or outputs, whose
+// element e belongs to key (or dim) key(e) + 4 (lane / M) of it; DK dims a step of the scores,
+// PK keys a step of the product.
+template <int M>
+struct Geo;
+template <>
+struct Geo<32> {
+    typedef f16v acc;
+    static constexpr int E = 16, DK = 16, PK = 16;
+    static __device__ __forceinline__ constexpr int key(int e) { return 8 * (e >> 2) + (e & 3); }
+    static __device__ __forceinline__ acc mfma(h8 a, h8 b, acc c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Geo<16> {
+    typedef f4 acc;
+    static constexpr int E = 4, DK = 32, PK = 32;
+    static __device__ __forceinline__ constexpr int key(int e) { return e; }
+    static __device__ __forceinline__ acc mfma(h8 a, h8 b, acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+template <int D, int NW, int M>
 __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan,
-                                          int64_t item, uint8_t* lds) {
-    constexpr int ROWB = 2 * D, MAT = kWideKeys * ROWB, ROWS = 32 * NW;
+                                          int item, uint8_t* lds) {
+    constexpr int ROWB = 2 * D, MAT = kWideKeys * ROWB, ROWS = M * NW;
     constexpr int LPR = Dma<D>::LPR, RPI = Dma<D>::RPI, NI = kWideKeys / (RPI * NW);   // a wave's instructions a tile
-    constexpr int KS = D / 16, NB = D / 32;
+    typedef Geo<M> G;
+    typedef typename G::acc Acc;
+    constexpr int KS = D / G::DK, NB = D / M, XB = kWideKeys / M, E = G::E, XE = XB * E;
     static_assert(NI >= 1, "every wave has rows to fetch");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 31, hi = lane >> 5;
+    const int col = lane % M, part = lane / M;   // a lane's packed row, and which keys or dims of it it has
     const int nkv = c.num_kv_heads;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     const int dr = lane / LPR, ds = lane % LPR;
 
     Share s;
-    const int kvh = (int)(item % nkv);
-    if (!find_share<ROWS, kWideKeys>(a, c, plan, (int)(item / nkv), false, s)) return;
+    const int kvh = item % nkv;
+    if (!find_share<ROWS, kWideKeys>(a, c, plan, item / nkv, false, s)) return;
     const int rows = s.n * plan.group, r0 = ROWS * s.tile;
-    const Span t = span_of(s, r0, min(r0 + ROWS, rows) - 1, plan.group, a.window);
-    const int w0 = r0 + 32 * wave;
+    const Span t = span_of(plan, s, r0, min(r0 + ROWS, rows) - 1, a.window);
+    const int w0 = r0 + M * wave;
     const bool active = w0 < rows;
-    const Span u = span_of(s, min(w0, rows - 1), min(w0 + 32, rows) - 1, plan.group, a.window);
+    const Span u = span_of(plan, s, min(w0, rows - 1), min(w0 + M, rows) - 1, a.window);
     const int p0 = t.lo / kWideKeys, p1 = (t.hi + kWideKeys - 1) / kWideKeys;
     const int each = (max(p1 - p0, 0) + s.parts - 1) / s.parts;
     const int begin = p0 + s.part * each, end = min(begin + each, p1);
-    const int r = min(w0 + col, rows - 1), token = r / plan.group, head = r - token * plan.group;
+    const int r = min(w0 + col, rows - 1), token = token_of(plan, r), head = r - token * plan.group;
     const int pos = s.kv - s.n + token;
     // the addresses of 64 units, and the pages of the next 64
     const Units units(a, c, s.b, kvh, t.lo, t.hi);
@@ -520,7 +560,11 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     const uint64_t v_from_k = (uint64_t)c.v - (uint64_t)c.k;
     const uint32_t stride = (uint32_t)(2 * c.row_stride);
     const int wave_row = RPI * wave;
+    // (a wave's groups of rows are a multiple of 16 apart: the same row of a unit, the same swizzle)
+    static_assert(RPI * NW % 16 == 0, "one piece a lane for all of them");
     const uint32_t lane_row = (uint32_t)((wave_row & 7) + dr) * stride;
+    const uint32_t k_piece = 16u * (uint32_t)(ds ^ k_swizzle<D>(wave_row + dr));
+    const uint32_t v_piece = 16u * (uint32_t)(ds ^ v_swizzle<D>(wave_row + dr));
     // this wave's rows of a tile of K or V into its buffer; K goes first and moves the window
     auto stage = [&](auto which, int tile) {
         constexpr bool values = decltype(which)::value;
@@ -536,99 +580,105 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            // (RPI NW i is a multiple of 8: a lane's row in its unit is the same in each)
-            const int row = wave_row + RPI * NW * i, lr = row + dr;
-            const uint32_t piece = 16u * (uint32_t)(ds ^ (values ? v_swizzle<D>(lr) : k_swizzle<D>(lr)));
+            const int row = wave_row + RPI * NW * i;
             int unit = u0 + (row >> 3);
-            uint32_t off = lane_row + piece;
+            uint32_t off = lane_row + (values ? v_piece : k_piece);
             if (!whole) {
                 // positions that no row sees are taken from the nearest one that some row sees
                 unit = units.seen(unit + window);
-                off = (uint32_t)(min(max(k0 + lr, t.lo), t.hi - 1) - 8 * unit) * stride + piece;
+                off = (uint32_t)(min(max(k0 + row + dr, t.lo), t.hi - 1) - 8 * unit) * stride + (values ? v_piece : k_piece);
                 unit -= window;
             }
             const uint64_t at = read_lane(address, unit) + (values ? v_from_k : 0);
             lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * NW * i), off, reinterpret_cast<const uint8_t*>(at));
         }
     };
-    if (begin < end) next = units.page_of((8 * begin & ~63) + lane);
+    if (begin < end) {
+        next = units.page_of((8 * begin & ~63) + lane);
+        stage(std::false_type(), begin);
+        stage(std::true_type(), begin);
+        stage(std::false_type(), begin + 1);
+    }
     // a negative scale moves its sign to Q (exact), so that the largest S has the largest weight
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
     const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
     h8 q[KS];
-    const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * hi;
+    const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * part;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) q[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qrow + 16 * k) ^ sign);
-    // operand addresses: 2 k + hi = 2 k ^ hi and so on, so one base and an xor each
-    const int i16 = lane & 15, vr = 4 * hi + (i16 >> 2);
-    const uint32_t ka = lds0 + (uint32_t)col * ROWB + 16u * (uint32_t)(hi ^ k_swizzle<D>(col));
+    for (int k = 0; k < KS; ++k) q[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qrow + G::DK * k) ^ sign);
+    // operand addresses: one base, and an xor for each k-step or block of dims
+    const int i16 = lane & 15, vr = 4 * part + (i16 >> 2);
+    const uint32_t ka = lds0 + (uint32_t)col * ROWB + 16u * (uint32_t)(part ^ k_swizzle<D>(col));
     const uint32_t va = lds0 + 2 * MAT + (uint32_t)vr * ROWB +
-                        16u * (uint32_t)((2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1)) ^ v_swizzle<D>(vr)) +
+                        16u * (uint32_t)(((M == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((i16 >> 1) & 1)) ^ v_swizzle<D>(vr)) +
                         8u * (uint32_t)(i16 & 1);
-    f16v o[NB];
+    Acc o[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+        for (int e = 0; e < E; ++e) o[i][e] = 0.0f;
     float m = kNone, l = 0.0f;
     bool far = false, dirty = false;
 
-    // S^T of a tile; beside(k): what is done beside k-step k's two products
-    auto scores = [&](int tile, f16v (&y)[2], auto beside) {
+    // S^T of a tile; beside(n): what is done beside the n-th two of its products
+    auto scores = [&](int tile, Acc (&y)[XB], auto beside) {
         // (opaque, so that a tile's addresses are not kept in registers over the loop)
         uint32_t kt = ka + (uint32_t)(tile & 1) * MAT;
         asm("" : "+v"(kt));
-        auto k_frag = [&](int k, int b) { return *(lds_h8)((kt ^ (32u * k)) + 32u * b * ROWB); };
+        auto k_frag = [&](int k, int b) { return *(lds_h8)((kt ^ (2u * G::DK * k)) + (uint32_t)(M * b) * ROWB); };
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < XB; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[b][e] = 0.0f;
+            for (int e = 0; e < E; ++e) y[b][e] = 0.0f;
+        // two blocks at a time, their operands two k-steps ahead
         constexpr int AHEAD = 2;
-        h8 kf[AHEAD + 1][2];
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
+        for (int b0 = 0; b0 < XB; b0 += 2) {
+            h8 kf[AHEAD + 1][2];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) kf[k][b] = k_frag(k, b);
+            for (int k = 0; k < AHEAD; ++k)
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            if (k + AHEAD < KS)
+                for (int b = 0; b < 2; ++b) kf[k][b] = k_frag(k, b0 + b);
 #pragma unroll
-                for (int b = 0; b < 2; ++b) kf[(k + AHEAD) % (AHEAD + 1)][b] = k_frag(k + AHEAD, b);
+            for (int k = 0; k < KS; ++k) {
+                if (k + AHEAD < KS)
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-                y[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k % (AHEAD + 1)][b], q[k], y[b], 0, 0, 0);
-            beside(k);
-            __builtin_amdgcn_sched_barrier(0);
+                    for (int b = 0; b < 2; ++b) kf[(k + AHEAD) % (AHEAD + 1)][b] = k_frag(k + AHEAD, b0 + b);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) y[b0 + b] = G::mfma(kf[k % (AHEAD + 1)][b], q[k], y[b0 + b]);
+                beside(b0 / 2 * KS + k);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
     // The softmax of x, a tile's scores, beside the next tile's, and its product with V
-    auto step = [&](auto mask, int tile, f16v (&x)[2], f16v (&y)[2]) {
+    auto step = [&](auto mask, int tile, Acc (&x)[XB], Acc (&y)[XB]) {
         constexpr bool masked = decltype(mask)::value;
         const int k0 = kWideKeys * tile;
         uint32_t vt = va + (uint32_t)(tile & 1) * MAT;
         asm("" : "+v"(vt));
-        // V^T (k-step j, dims 32 i ..): lane (dim 32 i + col) takes keys 16 j + 4 hi + {0 .. 3, 8 .. 11}, as
-        // the weights' registers hold them
+        // V^T (k-step j, block of dims i): the lane takes its dim's keys in the order in which the
+        // weights' registers hold them, PK j + 4 part + {0 .. 3, PK / 2 ..}
         auto v_frag = [&](int j, int i) {
-            const uint32_t v = (vt ^ (64u * i)) + 16u * j * ROWB;
-            return join(read_tr(v), read_tr(v + 8u * ROWB));
+            const uint32_t v = (vt ^ (2u * M * i)) + (uint32_t)(G::PK * j) * ROWB;
+            return join(read_tr(v), read_tr(v + (uint32_t)(G::PK / 2) * ROWB));
         };
         if constexpr (masked) {
-            const int ahead = pos - k0 - 4 * hi, behind = a.window > 0 ? ahead - a.window : INT_MIN;
+            const int ahead = pos - k0 - 4 * part, behind = a.window > 0 ? ahead - a.window : INT_MIN;
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < XB; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = 32 * b + 8 * (e >> 2) + (e & 3);     // less k0 + 4 hi
+                for (int e = 0; e < E; ++e) {
+                    const int key = M * b + G::key(e);       // less k0 + 4 part
                     if (key > ahead || key <= behind) x[b][e] = -INFINITY;
                 }
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < XB; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, x[b][e]);
-        top = xor_butterfly<32, 32>(top, max_raw) * scale;
+            for (int e = 0; e < E; ++e) top = fmaxf(top, x[b][e]);
+        top = xor_butterfly<32, M>(top, max_raw) * scale;
         // exp(x - m) as 2^(x scale - m), one fma: m is a rounded product and the fma's is not, so
         // a row's weights are off by one common factor of 2^(half a step of m).  Far from zero
         // (2^7) scores are rounded as m is, lest the factor leave fp16's range.
@@ -640,44 +690,46 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[i][e] *= f;
+                for (int e = 0; e < E; ++e) o[i][e] *= f;
             far = __ballot(fabsf(m) >= 128.0f && m != kNone) != 0;
             if (far) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < XB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[b][e] = __fmul_rn(x[b][e], scale);
+                    for (int e = 0; e < E; ++e) x[b][e] = __fmul_rn(x[b][e], scale);
                 mul = 1.0f;
             }
         }
         // (past the last tile of K the scores are of what its buffer holds, and are not used)
-        u32x4 w[4];                              // the weights, two in a register
+        constexpr int STEPS = XE / 8;            // of the product
+        u32x4 w[STEPS];                          // the weights, two in a register
         // V's operands, in fours: those of the first products are read beside the scores, the others
-        // two fours ahead
-        constexpr int FOURS = NB, AHEAD = FOURS < 2 ? FOURS : 2;
+        // one or two fours ahead
+        constexpr int FOURS = STEPS * NB / 4, AHEAD = FOURS < 2 ? FOURS : M == 32 ? 2 : 1;
         h8 v[AHEAD + 1][4];
         auto read_four = [&](int f) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[f % (AHEAD + 1)][i] = v_frag((4 * f + i) / NB, (4 * f + i) % NB);
         };
-        scores(tile + 1, y, [&](int k) {
-            constexpr int N = 32 / KS;
+        constexpr int TWOS = KS * XB / 2;
+        scores(tile + 1, y, [&](int two) {
 #pragma unroll
-            for (int e = N * k; e < N * (k + 1); e += 2) {
+            for (int n = 0; n < XE; n += 2) {
+                if (n / 2 * TWOS / (XE / 2) != two) continue;
                 float f[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    f[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 4][(e & 15) + i], mul, -m));
-                w[e >> 3][(e >> 1) & 3] = __builtin_bit_cast(uint32_t, h2{(_Float16)f[0], (_Float16)f[1]});
-                asm volatile("" : "+v"(w[e >> 3][(e >> 1) & 3]));        // here, not where it is used
+                    f[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n / E][n % E + i], mul, -m));
+                w[n >> 3][(n >> 1) & 3] = __builtin_bit_cast(uint32_t, h2{(_Float16)f[0], (_Float16)f[1]});
+                asm volatile("" : "+v"(w[n >> 3][(n >> 1) & 3]));        // here, not where it is used
             }
 #pragma unroll
             for (int f = 0; f < AHEAD; ++f)
-                if (k == KS - 1 - AHEAD + f) read_four(f);
+                if (two == TWOS - 1 - AHEAD + f) read_four(f);
         });
-        h8 p[4];
+        h8 p[STEPS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < STEPS; ++j) {
             p[j] = __builtin_bit_cast(h8, w[j]);
             l = sum8(p[j], l);
         }
@@ -695,7 +747,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
                     fin.take(b);
                     b = finite_of(b);
                 }
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, p[j], o[d], 0, 0, 0);
+                o[d] = G::mfma(b, p[j], o[d]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -708,6 +760,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     auto advance = [&](int tile) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();
+        if (tile < begin) return;
         stage(std::true_type(), tile + 1);
         stage(std::false_type(), tile + 2);
     };
@@ -717,11 +770,11 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     const int behind = a.window > 0 ? max(u.last - a.window + kWideKeys, 0) / kWideKeys : 0;
     const int full = min(max(behind, mine), mine_end);
     const int full_end = min(max((u.first + 1) >> 6, full), mine_end);
-    int tile = begin - 2;
+    int tile = begin - 1;
 #pragma unroll 1
     for (; tile < mine - 1; ++tile) advance(tile);
     if (mine < mine_end) {
-        f16v x[2], y[2];
+        Acc x[XB], y[XB];
         advance(tile++);
         scores(mine, x, [](int) {});
         // (whole tiles in pairs, so that x and y change places without copies)
@@ -735,8 +788,8 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
                     advance(++tile);
                     step(mask, tile, y, x);
                 } else {
-                    x[0] = y[0];
-                    x[1] = y[1];
+#pragma unroll
+                    for (int b = 0; b < XB; ++b) x[b] = y[b];
                 }
             }
         };
@@ -757,43 +810,46 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
             if (!(k32 + 31 > u.first || (a.window > 0 && k32 <= u.last - a.window)) || k0 < t.lo || k0 >= t.hi) continue;
             const int page = table[k0 >> psh];
             if ((unsigned)page >= (unsigned)c.num_pages) continue;
-            const uint16_t* row = vc + (int64_t)page * c.page_stride + (int64_t)(k0 & pmask) * c.row_stride + 4 * hi;
+            const uint16_t* row = vc + (int64_t)page * c.page_stride + (int64_t)(k0 & pmask) * c.row_stride + 4 * part;
             const bool seen = k0 <= pos && (a.window == 0 || k0 > pos - a.window);
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int e4 = 0; e4 < 4; ++e4) {
-                    const h4 w = *reinterpret_cast<const h4*>(row + 32 * i + 8 * e4), f = finite_of(w);
+                for (int e = 0; e < E; e += 4) {
+                    const h4 w = *reinterpret_cast<const h4*>(row + M * i + G::key(e)), f = finite_of(w);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][4 * e4 + e] += seen ? (float)w[e] - (float)f[e] : 0.0f;
+                    for (int n = 0; n < 4; ++n) o[i][e + n] += seen ? (float)w[n] - (float)f[n] : 0.0f;
                 }
         }
     }
     if (active && w0 + col < rows) {
-        l += lane_xor<32>(l);
+        l = xor_sum<32, M>(l);
         if (bad) l = NAN;
         if (s.parts > 1) {
-            float* part = slot_of<ROWS, D>(plan.slots, s, s.part, kvh, nkv);
-            const int row = 32 * wave + col;
+            float* to = slot_of<ROWS, D>(plan.slots, s, s.part, kvh, nkv);
+            const int row = M * wave + col;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int e4 = 0; e4 < 4; ++e4)
-                    *reinterpret_cast<f4*>(part + row * D + 32 * i + 8 * e4 + 4 * hi) =
-                        f4{o[i][4 * e4], o[i][4 * e4 + 1], o[i][4 * e4 + 2], o[i][4 * e4 + 3]};
-            if (hi == 0) {
-                part[ROWS * D + row] = m;
-                part[ROWS * (D + 1) + row] = l;
+                for (int e = 0; e < E; e += 4)
+                    *reinterpret_cast<f4*>(to + row * D + M * i + G::key(e) + 4 * part) =
+                        f4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+            if (part == 0) {
+                to[ROWS * D + row] = m;
+                to[ROWS * (D + 1) + row] = l;
             }
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const int64_t at = (int64_t)(s.q0 + token) * a.ld_out + (int64_t)(kvh * plan.group + head) * D + 4 * hi;
+            // (worked out again, not kept in registers over the loop)
+            int row = w0 + col;
+            asm("" : "+v"(row));
+            const int tk = token_of(plan, row), hd = row - tk * plan.group;
+            const int64_t at = (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + 4 * part;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int e4 = 0; e4 < 4; ++e4)
-                    store4(a, at + 32 * i + 8 * e4,
-                           f4{o[i][4 * e4], o[i][4 * e4 + 1], o[i][4 * e4 + 2], o[i][4 * e4 + 3]} * inv);
+                for (int e = 0; e < E; e += 4)
+                    store4(a, at + M * i + G::key(e), f4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]} * inv);
         }
     }
 }
@@ -805,35 +861,35 @@ constexpr int kJoinRows = 32, kJoinParts = 64;
 // Head dims, waves and stages of the narrow part, waves of the wide one.
 // (MW, MS: of the narrow part beside wide ones)
 template <int D> struct Shape;
-template <> struct Shape<64> { static constexpr int W = 4, S = 4, NW = 4, MW = 4, MS = 2, EU = 2; };
-template <> struct Shape<128> { static constexpr int W = 4, S = 2, NW = 4, MW = 2, MS = 2, EU = 2; };
-template <> struct Shape<256> { static constexpr int W = 2, S = 2, NW = 4, MW = 2, MS = 2, EU = 1; };
+template <> struct Shape<64> { static constexpr int W = 4, S = 4, NW = 4, M = 32, MW = 4, MS = 2, PER_CU = 2; };
+template <> struct Shape<128> { static constexpr int W = 4, S = 2, NW = 4, M = 32, MW = 2, MS = 2, PER_CU = 2; };
+template <> struct Shape<256> { static constexpr int W = 2, S = 2, NW = 8, M = 16, MW = 2, MS = 2, PER_CU = 1; };
 template <int D>
 constexpr int narrow_lds(int w, int s) { return w * s * 2 * kNarrowKeys * 2 * D; }
 template <int D>
 constexpr int wide_lds() { return 4 * kWideKeys * 2 * D; }
 template <int D>
-constexpr int wide_rows() { return 32 * Shape<D>::NW; }
+constexpr int wide_rows() { return Shape<D>::M * Shape<D>::NW; }
 template <int D>
-constexpr int wide_parts() { return 256 * Shape<D>::EU; }
+constexpr int wide_parts() { return 256 * Shape<D>::PER_CU; }
 
 template <int D>
 __global__ __launch_bounds__(64 * Shape<D>::W)
 void rf_paged_attn_narrow_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan plan) {
     __shared__ __align__(1024) uint8_t lds[narrow_lds<D>(Shape<D>::W, Shape<D>::S)];
-    narrow_part<D, Shape<D>::W, Shape<D>::S>(a, c, plan, blockIdx.x + (int64_t)blockIdx.y * gridDim.x, lds);
+    narrow_part<D, Shape<D>::W, Shape<D>::S>(a, c, plan, (int)(blockIdx.x + blockIdx.y * gridDim.x), lds);
 }
 
 // Both kinds in one launch, the wide items first: their workgroups are the
 // longer ones, and the narrow ones fill the CUs that they leave.
 template <int D>
-__global__ __launch_bounds__(64 * Shape<D>::NW) __attribute__((amdgpu_waves_per_eu(Shape<D>::EU)))
+__global__ __launch_bounds__(64 * Shape<D>::NW) __attribute__((amdgpu_waves_per_eu(2)))
 void rf_paged_attn_mixed_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan wide, const Plan narrow) {
     constexpr int MW = Shape<D>::MW, MS = Shape<D>::MS, NEED = narrow_lds<D>(MW, MS);
     __shared__ __align__(1024) uint8_t lds[NEED > wide_lds<D>() ? NEED : wide_lds<D>()];
-    const int64_t item = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+    const int item = (int)(blockIdx.x + blockIdx.y * gridDim.x);
     if (item < wide.items) {
-        wide_part<D, Shape<D>::NW>(a, c, wide, item, lds);
+        wide_part<D, Shape<D>::NW, Shape<D>::M>(a, c, wide, item, lds);
     } else {
         if (threadIdx.x >= 64 * MW) return;      // whole waves, before any barrier
         narrow_part<D, MW, MS>(a, c, narrow, item - wide.items, lds);
@@ -900,7 +956,7 @@ __device__ __forceinline__ void join_part(const rf_paged_attention& a, const rf_
         if (i >= outs) continue;
         for (int k = 1; k < groups; ++k) acc[o] += sums[tid + k * outs];
         const int at = r0 + first + i / (D / 4), d = 4 * (i % (D / 4));
-        const int tk = at / plan.group, hd = at - tk * plan.group;
+        const int tk = token_of(plan, at), hd = at - tk * plan.group;
         store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d, acc[o] * weight[0][i / (D / 4)]);
     }
 }
@@ -943,14 +999,15 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
     const int64_t packed = (int64_t)a.rows * group, positions = (int64_t)a.max_blocks * c.page_size;
     const bool both = (int64_t)a.max_new * group > kNarrowRows;
     float* ws = static_cast<float*>(a.workspace);
-    Plan narrow = {group, 0, both ? kNarrowRows : INT_MAX, kNarrowParts, kNarrowLeast, 0, ws};
-    Plan wide = {group, kNarrowRows, INT_MAX, wide_parts<D>(), kWideLeast, 0, ws + narrow_bytes<D>() / sizeof(float)};
+    const uint32_t inv = packed * group < (1ll << 32) ? (uint32_t)(((1ll << 32) + group - 1) / group) : 0;
+    Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, kNarrowParts, kNarrowLeast, 0, ws};
+    Plan wide = {group, inv, kNarrowRows, INT_MAX, wide_parts<D>(), kWideLeast, 0, ws + narrow_bytes<D>() / sizeof(float)};
     // Items: every tile has a part, and there are at most `parts` parts more (each of them a share
     // long); no more either than the table's width gives room for.
     const auto items = [&](int64_t tiles, const Plan& p, int keys, int64_t* joins) {
         const int64_t most = std::max<int64_t>((positions + keys * p.least - 1) / (keys * p.least), 1);
         *joins = most > 1 ? std::min<int64_t>(tiles, p.parts) : 0;
-        return std::min(tiles + p.parts, tiles * most);
+        return (int)std::min(tiles + p.parts, tiles * most);
     };
     const int64_t some = std::min<int64_t>(a.num_seqs, a.rows);        // requests with rows
     int64_t narrow_joins, wide_joins = 0;
@@ -960,8 +1017,8 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
         // (workgroups i and i + 8 share an XCD's L2, and items i and i + num_kv_heads their K and V)
         wide.items = (wide.items + 8 * nkv - 1) / (8 * nkv) * (8 * nkv);
     }
-    const int64_t total = wide.items + narrow.items;
-    const dim3 grid((unsigned)std::min<int64_t>(total, 1 << 20), (unsigned)((total + (1 << 20) - 1) >> 20));
+    const unsigned total = (unsigned)wide.items + (unsigned)narrow.items;
+    const dim3 grid(std::min(total, 1u << 20), (total + (1u << 20) - 1) >> 20);
     if (both)
         hipLaunchKernelGGL(rf_paged_attn_mixed_kernel<D>, grid, dim3(64 * Shape<D>::NW), 0, stream, a, c, wide, narrow);
     else
@@ -979,7 +1036,7 @@ extern "C" hipError_t rf_paged_attention_launch(const rf_paged_attention* step, 
     const rf_paged_cache& c = *cache;
     if (!rf::cache_ok(c) || a.num_seqs < 0 || a.rows < 0 || a.rows > (1 << 23) || a.max_blocks < 0 ||
         a.num_heads <= 0 || a.num_heads > 65535 || a.num_heads % c.num_kv_heads != 0 ||
-        a.num_heads / c.num_kv_heads > 64 || a.window < 0 || !std::isfinite(a.scale) ||
+        a.num_heads / c.num_kv_heads > 64 || (int64_t)a.rows * a.num_heads > (1 << 27) || a.window < 0 || !std::isfinite(a.scale) ||
         (int64_t)a.max_blocks * c.page_size > (1 << 30))
         return hipErrorInvalidValue;
     if (a.rows == 0 || a.num_seqs == 0) return hipSuccess;
