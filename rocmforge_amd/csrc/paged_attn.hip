@@ -532,6 +532,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
     typedef Geo<M> G;
     typedef typename G::acc Acc;
     constexpr int KS = D / G::DK, NB = D / M, XB = kWideKeys / M, E = G::E, XE = XB * E;
+    constexpr bool BESIDE = M == 32;             // the next tile's scores beside a tile's weights
     static_assert(NI >= 1, "every wave has rows to fetch");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane % M, part = lane / M;   // a lane's packed row, and which keys or dims of it it has
@@ -597,7 +598,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         next = units.page_of((8 * begin & ~63) + lane);
         stage(std::false_type(), begin);
         stage(std::true_type(), begin);
-        stage(std::false_type(), begin + 1);
+        if constexpr (BESIDE) stage(std::false_type(), begin + 1);
     }
     // a negative scale moves its sign to Q (exact), so that the largest S has the largest weight
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
@@ -652,9 +653,10 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         }
     };
     // The softmax of x, a tile's scores, beside the next tile's, and its product with V
-    auto step = [&](auto mask, int tile, Acc (&x)[XB], Acc (&y)[XB]) {
+    auto step = [&](auto mask, int tile, Acc (&x)[XB], Acc (&y)[BESIDE ? XB : 1]) {
         constexpr bool masked = decltype(mask)::value;
         const int k0 = kWideKeys * tile;
+        if constexpr (!BESIDE) scores(tile, x, [](int) {});
         uint32_t vt = va + (uint32_t)(tile & 1) * MAT;
         asm("" : "+v"(vt));
         // V^T (k-step j, block of dims i): the lane takes its dim's keys in the order in which the
@@ -712,7 +714,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
             for (int i = 0; i < 4; ++i) v[f % (AHEAD + 1)][i] = v_frag((4 * f + i) / NB, (4 * f + i) % NB);
         };
         constexpr int TWOS = KS * XB / 2;
-        scores(tile + 1, y, [&](int two) {
+        auto weights = [&](int two) {
 #pragma unroll
             for (int n = 0; n < XE; n += 2) {
                 if (n / 2 * TWOS / (XE / 2) != two) continue;
@@ -726,7 +728,13 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
 #pragma unroll
             for (int f = 0; f < AHEAD; ++f)
                 if (two == TWOS - 1 - AHEAD + f) read_four(f);
-        });
+        };
+        if constexpr (BESIDE) {
+            scores(tile + 1, y, weights);
+        } else {
+#pragma unroll
+            for (int two = 0; two < TWOS; ++two) weights(two);
+        }
         h8 p[STEPS];
 #pragma unroll
         for (int j = 0; j < STEPS; ++j) {
@@ -754,15 +762,16 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         if constexpr (masked) dirty = dirty || !fin.all();
     };
 
-    // K runs a tile ahead of V.  At a tile's start this wave's share
+    // (With the next scores beside, K runs a tile ahead of V.)  At a tile's start this wave's share
     // of what its step reads has landed; past the barrier everyone's has, and the buffers
     // that are filled next have been read.
     auto advance = [&](int tile) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();
         if (tile < begin) return;
+        if constexpr (!BESIDE) stage(std::false_type(), tile + 1);
         stage(std::true_type(), tile + 1);
-        stage(std::false_type(), tile + 2);
+        if constexpr (BESIDE) stage(std::false_type(), tile + 2);
     };
     // the tiles that this wave's rows see, and among them those that all its rows see whole
     const int mine = active ? min(max(u.lo / kWideKeys, begin), end) : end;
@@ -774,9 +783,9 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
 #pragma unroll 1
     for (; tile < mine - 1; ++tile) advance(tile);
     if (mine < mine_end) {
-        Acc x[XB], y[XB];
+        Acc x[XB], y[BESIDE ? XB : 1];
         advance(tile++);
-        scores(mine, x, [](int) {});
+        if constexpr (BESIDE) scores(mine, x, [](int) {});
         // (whole tiles in pairs, so that x and y change places without copies)
         auto run = [&](auto mask, int to) {
             constexpr bool pairs = !decltype(mask)::value;
@@ -784,12 +793,14 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
             for (; tile < to; ++tile) {
                 advance(tile);
                 step(mask, tile, x, y);
-                if (pairs && tile + 1 < to) {
-                    advance(++tile);
-                    step(mask, tile, y, x);
-                } else {
+                if constexpr (BESIDE) {
+                    if (pairs && tile + 1 < to) {
+                        advance(++tile);
+                        step(mask, tile, y, x);
+                    } else {
 #pragma unroll
-                    for (int b = 0; b < XB; ++b) x[b] = y[b];
+                        for (int b = 0; b < XB; ++b) x[b] = y[b];
+                    }
                 }
             }
         };
