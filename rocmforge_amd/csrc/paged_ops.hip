@@ -280,20 +280,19 @@ __global__ __launch_bounds__(256) void rf_paged_rope_kernel(const rf_paged_rope 
 //
 // A workgroup takes kSlice tokens of one row: it starts their loads, counts
 // the history's tokens that fall among them in LDS (integers, so the order of
-// the atomics does not matter), adds the bias list's, and writes the slice in
-// one pass.  The history is read once a slice, from L2.  Bound: 8 bytes a
-// token, and for few rows the latency of history and logits.
+// the atomics does not matter), marks the bias list's, and writes the slice in
+// one pass; a marked token's wave adds up its entries in list order.  The
+// history is read once a slice, from L2.  Bound: 8 bytes a token, and for few
+// rows the latency of history and logits.
 constexpr int kSlice = 4096;
-constexpr uint32_t kMade = 2, kSeen = 1;         // a count in the upper bits, "somewhere" in the lowest
+// of a token in LDS: its place in the history, a mark for the bias list, a count of those not in the prompt
+constexpr uint32_t kSeen = 1, kBiased = 2, kMade = 4;
 
-template <bool VEC, bool BIAS>
+template <bool VEC>
 __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_rules l) {
     __shared__ uint32_t count[kSlice];
-    __shared__ int first[BIAS ? kSlice : 1];     // the list's first entry for a token
-    __shared__ float bias[BIAS ? kSlice : 1];
-    __shared__ int twice;
     constexpr int V = VEC ? 4 : 1, N = kSlice / (256 * V);
-    const int r = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * kSlice;
+    const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, base = blockIdx.x * kSlice;
     const int n = min(kSlice, l.vocab - base);   // tokens of this slice
     const float* x = l.logits + r * l.ld_logits + base;
     float* y = l.out + r * l.ld_out + base;
@@ -314,53 +313,31 @@ __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_ru
         }
     }
     const bool penal = l.repetition != nullptr || l.frequency != nullptr || l.presence != nullptr;
-    for (int i = tid; i < kSlice; i += 256) {
-        count[i] = 0;
-        if constexpr (BIAS) {
-            first[i] = INT_MAX;
-            bias[i] = 0.0f;
-        }
-    }
-    if (tid == 0) twice = 0;
+    const int64_t total = penal ? min((int64_t)max(l.total_lens[r], 0), l.ld_history) : 0;
+    const int prompt = penal ? l.prompt_lens[r] : 0;
+    const int b0 = l.bias_start != nullptr ? max(l.bias_start[r], 0) : 0;
+    const int b1 = l.bias_start != nullptr ? l.bias_start[r + 1] : 0;
+    for (int i = tid; i < kSlice / 4; i += 256) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (penal) {
-        const int64_t total = min((int64_t)max(l.total_lens[r], 0), l.ld_history);
-        const int prompt = l.prompt_lens[r];
-        const int* hist = l.history + r * l.ld_history;
-        for (int64_t i = tid; i < total; i += 256) {
-            const uint32_t id = (uint32_t)hist[i] - (uint32_t)base;
-            if (id < (uint32_t)n) {
-                if (i >= prompt)
-                    atomicAdd(&count[id], kMade);
+    const int* hist = l.history + r * l.ld_history;
+    for (int64_t i0 = tid; i0 < total; i0 += 1024) {
+        uint32_t id[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) id[k] = i0 + 256 * k < total ? (uint32_t)hist[i0 + 256 * k] - (uint32_t)base : ~0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (id[k] < (uint32_t)n) {
+                if (i0 + 256 * k >= prompt)
+                    atomicAdd(&count[id[k]], kMade);
                 else
-                    atomicOr(&count[id], kSeen);
+                    atomicOr(&count[id[k]], kSeen);
             }
-        }
     }
-    int b0 = 0, b1 = 0;
-    if constexpr (BIAS) {
-        b0 = max(l.bias_start[r], 0);
-        b1 = l.bias_start[r + 1];
-        for (int j = b0 + tid; j < b1; j += 256) {
-            const uint32_t id = (uint32_t)l.bias_ids[j] - (uint32_t)base;
-            if (id < (uint32_t)n && atomicMin(&first[id], j) != INT_MAX) twice = 1;
-        }
+    for (int j = b0 + tid; j < b1; j += 256) {
+        const uint32_t id = (uint32_t)l.bias_ids[j] - (uint32_t)base;
+        if (id < (uint32_t)n) atomicOr(&count[id], kBiased);
     }
     __syncthreads();
-    if constexpr (BIAS) {
-        // the thread of a token's first entry adds them all, in list order
-        for (int j = b0 + tid; j < b1; j += 256) {
-            const uint32_t id = (uint32_t)l.bias_ids[j] - (uint32_t)base;
-            if (id < (uint32_t)n && first[id] == j) {
-                float sum = l.bias_values[j];
-                if (twice)
-                    for (int k = j + 1; k < b1; ++k)
-                        if (l.bias_ids[k] == l.bias_ids[j]) sum += l.bias_values[k];
-                bias[id] = sum;
-            }
-        }
-        __syncthreads();
-    }
     const float rep = l.repetition != nullptr ? l.repetition[r] : 1.0f;
     const float freq = l.frequency != nullptr ? l.frequency[r] : 0.0f;
     const float pres = l.presence != nullptr ? l.presence[r] : 0.0f;
@@ -368,21 +345,43 @@ __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_ru
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int e = (i * 256 + tid) * V;
-        if (e >= n) continue;
-        const uint32_t bits = allowed != nullptr ? allowed[e / 32] >> (e % 32) : ~0u;
+        uint32_t c[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) c[k] = count[e + k];
+        const uint32_t bits = allowed != nullptr && e < n ? allowed[e / 32] >> (e % 32) : ~0u;
         float o[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             float z = v[i][k];
-            const uint32_t c = count[e + k];
-            if (c != 0) {
+            if (c[k] & ~kBiased) {
                 if (l.repetition != nullptr) z = z > 0.0f ? z / rep : z * rep;
-                if (c >= kMade) z = (z - freq * (float)(c / kMade)) - pres;
+                if (c[k] >= kMade) z = (z - freq * (float)(c[k] / kMade)) - pres;
             }
-            if constexpr (BIAS)
-                if (first[e + k] != INT_MAX) z += bias[e + k];
-            o[k] = (bits >> k) & 1u ? z : -INFINITY;
+            o[k] = z;
         }
+        if (b1 > b0) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                uint64_t marked = __ballot(c[k] & kBiased);
+                while (marked) {                 // token by token, the wave over the list
+                    const int to = __builtin_ctzll(marked);
+                    marked &= marked - 1;
+                    const int token = base + __shfl(e, to) + k;
+                    float sum = 0.0f;
+                    for (int j0 = b0; j0 < b1; j0 += 64) {
+                        const bool there = j0 + lane < b1;
+                        const bool same = there && l.bias_ids[there ? j0 + lane : b0] == token;
+                        uint64_t hits = __ballot(same);
+                        const float val = same ? l.bias_values[j0 + lane] : 0.0f;
+                        for (; hits; hits &= hits - 1) sum += __shfl(val, __builtin_ctzll(hits));
+                    }
+                    if (lane == to) o[k] += sum;
+                }
+            }
+        }
+        if (e >= n) continue;
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] = (bits >> k) & 1u ? o[k] : -INFINITY;
         if (VEC && e + 3 < n) {
             *reinterpret_cast<float4*>(y + e) = make_float4(o[0], o[V > 1 ? 1 : 0], o[V > 2 ? 2 : 0], o[V > 3 ? 3 : 0]);
         } else {
@@ -501,13 +500,9 @@ extern "C" hipError_t rf_logits_rules_launch(const rf_logits_rules* rules, hipSt
         return hipErrorInvalidValue;
     const bool vec = l.ld_logits % 4 == 0 && l.ld_out % 4 == 0 && aligned(l.logits, 16) && aligned(l.out, 16);
     const dim3 grid((unsigned)((l.vocab + (int64_t)rf::kSlice - 1) / rf::kSlice), l.rows), blk(256);
-    if (vec && bias)
-        hipLaunchKernelGGL((rf::rf_logits_rules_kernel<true, true>), grid, blk, 0, stream, l);
-    else if (vec)
-        hipLaunchKernelGGL((rf::rf_logits_rules_kernel<true, false>), grid, blk, 0, stream, l);
-    else if (bias)
-        hipLaunchKernelGGL((rf::rf_logits_rules_kernel<false, true>), grid, blk, 0, stream, l);
+    if (vec)
+        hipLaunchKernelGGL(rf::rf_logits_rules_kernel<true>, grid, blk, 0, stream, l);
     else
-        hipLaunchKernelGGL((rf::rf_logits_rules_kernel<false, false>), grid, blk, 0, stream, l);
+        hipLaunchKernelGGL(rf::rf_logits_rules_kernel<false>, grid, blk, 0, stream, l);
     return hipGetLastError();
 }
