@@ -49,20 +49,21 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* wave_sums, int
 __device__ __forceinline__ int64_t pages_for(int64_t n, int page) { return (n + page - 1) >> (__ffs(page) - 1); }
 
 // Position and slot of row r, whose request is the last one that starts at or
-// before it (requests of no rows share their start with the next).
-__device__ __forceinline__ void plan_row(const rf_paged_plan& p, int r) {
-    int lo = 0, hi = p.num_seqs;                 // q_start[lo] <= r; r < q_start[hi] unless r is padding
-    if (r < p.q_start[hi]) {
+// before it (requests of no rows share their start with the next).  starts: q_start,
+// in LDS where there is room for it.
+__device__ __forceinline__ void plan_row(const rf_paged_plan& p, const int* starts, int r) {
+    int lo = 0, hi = p.num_seqs;                 // starts[lo] <= r; r < starts[hi] unless r is padding
+    if (r < starts[hi]) {
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (p.q_start[mid] <= r)
+            if (starts[mid] <= r)
                 lo = mid;
             else
                 hi = mid;
         }
         const int n = p.new_lens[lo], kv = p.kv_lens[lo];
         if (kv > 0) {
-            const int pos = kv - n + (r - p.q_start[lo]), sh = __ffs(p.page_size) - 1;
+            const int pos = kv - n + (r - starts[lo]), sh = __ffs(p.page_size) - 1;
             p.positions[r] = pos;
             p.slots[r] = (p.block_tables[(int64_t)lo * p.max_blocks + (pos >> sh)] << sh) + (pos & (p.page_size - 1));
             return;
@@ -72,15 +73,22 @@ __device__ __forceinline__ void plan_row(const rf_paged_plan& p, int r) {
     p.slots[r] = -1;
 }
 
+// ROWS: writes the rows too (then there are at most kPlanThreads requests).
 template <bool ROWS>
 __global__ __launch_bounds__(kPlanThreads) void rf_paged_plan_kernel(const rf_paged_plan p) {
     __shared__ int64_t sums[kPlanWaves];
     __shared__ int64_t page_end[kPlanThreads];   // pages asked for up to and with request b0 + t
     __shared__ int page_first[kPlanThreads];     // its first new column
+    __shared__ int starts[ROWS ? kPlanThreads + 1 : 1];
+    __shared__ int granted_end;                  // pages of the granted requests so far: a prefix of those asked for
     const int t = threadIdx.x;
     const int64_t n_free = min(max(p.free_in[0], 0), p.num_pages);
-    int64_t rows_before = 0, pages_before = 0, taken = 0;
-    if (t == 0) p.q_start[0] = 0;
+    int64_t rows_before = 0, pages_before = 0;
+    if (t == 0) {
+        p.q_start[0] = 0;
+        starts[0] = 0;
+        granted_end = 0;
+    }
     for (int b0 = 0; b0 < p.num_seqs; b0 += kPlanThreads) {
         const int b = b0 + t;
         const bool there = b < p.num_seqs;
@@ -94,27 +102,19 @@ __global__ __launch_bounds__(kPlanThreads) void rf_paged_plan_kernel(const rf_pa
         const int64_t end = pages_before + block_scan(need, sums, &pages);
         const bool granted = fits && (need == 0 || end <= n_free);
         if (there) {
-            p.q_start[b + 1] = (int)min(row_end, (int64_t)p.max_rows);
+            const int start = (int)min(row_end, (int64_t)p.max_rows);
+            p.q_start[b + 1] = start;
+            if constexpr (ROWS) starts[t + 1] = start;
             p.kv_lens[b] = granted ? (int)(ctx + n) : 0;
             p.ctx_out[b] = granted ? (int)(ctx + n) : (int)ctx;
         }
-        // the granted needs are a prefix of the needs: page i of this round belongs to the
-        // first request whose end passes it
         page_end[t] = end;
         page_first[t] = (int)have;
+        if (granted && need > 0) atomicMax(&granted_end, (int)end);
         __syncthreads();
-        const int64_t stop = min(pages_before + pages, n_free);
-        int last = 0, above = kPlanThreads;      // requests [0, last) end at or before stop: none in part
-        while (last < above) {
-            const int mid = (last + above) >> 1;
-            if (page_end[mid] <= stop)
-                last = mid + 1;
-            else
-                above = mid;
-        }
-        const int64_t granted_end = last > 0 ? page_end[last - 1] : taken;
+        // page i of this round belongs to the first request whose end passes it
         for (int64_t i = pages_before + t; i < granted_end; i += kPlanThreads) {
-            int lo = 0, hi = last - 1;
+            int lo = 0, hi = kPlanThreads - 1;
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
                 if (page_end[mid] > i)
@@ -126,21 +126,28 @@ __global__ __launch_bounds__(kPlanThreads) void rf_paged_plan_kernel(const rf_pa
             p.block_tables[(int64_t)(b0 + lo) * p.max_blocks + page_first[lo] + (i - begin)] =
                 p.free_pages[n_free - 1 - i];
         }
-        taken = granted_end;
         rows_before += rows;
         pages_before += pages;
         __syncthreads();                         // page_end is read no more
     }
-    if (t == 0) p.free_out[0] = (int)(n_free - taken);
-    if constexpr (ROWS) {
-        __syncthreads();                         // this workgroup's own global writes, read back below
-        for (int r = t; r < p.max_rows; r += kPlanThreads) plan_row(p, r);
-    }
+    __syncthreads();                             // (no requests: granted_end)
+    if (t == 0) p.free_out[0] = (int)(n_free - granted_end);
+    if constexpr (ROWS)                          // this workgroup's own global writes, read back behind the barrier
+        for (int r = t; r < p.max_rows; r += kPlanThreads) plan_row(p, starts, r);
 }
 
+constexpr int kStartsInLds = 4096;
+
 __global__ __launch_bounds__(256) void rf_paged_rows_kernel(const rf_paged_plan p) {
+    __shared__ int starts[kStartsInLds];
     const int r = blockIdx.x * 256 + threadIdx.x;
-    if (r < p.max_rows) plan_row(p, r);
+    if (p.num_seqs < kStartsInLds) {
+        for (int i = threadIdx.x; i <= p.num_seqs; i += 256) starts[i] = p.q_start[i];
+        __syncthreads();
+        if (r < p.max_rows) plan_row(p, starts, r);
+    } else if (r < p.max_rows) {
+        plan_row(p, p.q_start, r);
+    }
 }
 
 __global__ __launch_bounds__(kPlanThreads) void rf_paged_release_kernel(const int* __restrict__ ended, int* ctx_lens,
@@ -284,13 +291,13 @@ __global__ __launch_bounds__(256) void rf_paged_rope_kernel(const rf_paged_rope 
 // one pass; a marked token's wave adds up its entries in list order.  The
 // history is read once a slice, from L2.  Bound: 8 bytes a token, and for few
 // rows the latency of history and logits.
-constexpr int kSlice = 4096;
 // of a token in LDS: its place in the history, a mark for the bias list, a count of those not in the prompt
 constexpr uint32_t kSeen = 1, kBiased = 2, kMade = 4;
 
-template <bool VEC>
+template <bool VEC, int kSlice>
 __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_rules l) {
     __shared__ uint32_t count[kSlice];
+    constexpr int IDS = 8;                       // of the history in flight a thread
     constexpr int V = VEC ? 4 : 1, N = kSlice / (256 * V);
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, base = blockIdx.x * kSlice;
     const int n = min(kSlice, l.vocab - base);   // tokens of this slice
@@ -320,12 +327,12 @@ __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_ru
     for (int i = tid; i < kSlice / 4; i += 256) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     const int* hist = l.history + r * l.ld_history;
-    for (int64_t i0 = tid; i0 < total; i0 += 1024) {
-        uint32_t id[4];
+    for (int64_t i0 = tid; i0 < total; i0 += 256 * IDS) {
+        uint32_t id[IDS];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) id[k] = i0 + 256 * k < total ? (uint32_t)hist[i0 + 256 * k] - (uint32_t)base : ~0u;
+        for (int k = 0; k < IDS; ++k) id[k] = i0 + 256 * k < total ? (uint32_t)hist[i0 + 256 * k] - (uint32_t)base : ~0u;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < IDS; ++k)
             if (id[k] < (uint32_t)n) {
                 if (i0 + 256 * k >= prompt)
                     atomicAdd(&count[id[k]], kMade);
@@ -411,7 +418,7 @@ extern "C" hipError_t rf_paged_plan_launch(const rf_paged_plan* plan, hipStream_
     if (!p.q_start || !p.free_in || !p.free_out || (p.max_rows > 0 && (!p.positions || !p.slots)) ||
         (p.num_seqs > 0 && (!p.new_lens || !p.ctx_in || !p.ctx_out || !p.kv_lens || !p.block_tables || !p.free_pages)))
         return hipErrorInvalidValue;
-    if (p.max_rows <= kPlanRows) {
+    if (p.max_rows <= kPlanRows && p.num_seqs <= rf::kPlanThreads) {
         hipLaunchKernelGGL(rf::rf_paged_plan_kernel<true>, dim3(1), dim3(rf::kPlanThreads), 0, stream, p);
     } else {
         hipLaunchKernelGGL(rf::rf_paged_plan_kernel<false>, dim3(1), dim3(rf::kPlanThreads), 0, stream, p);
@@ -499,10 +506,17 @@ extern "C" hipError_t rf_logits_rules_launch(const rf_logits_rules* rules, hipSt
         (l.allowed && l.ld_allowed < (l.vocab + (int64_t)31) / 32) || (l.out == l.logits && l.ld_out != l.ld_logits))
         return hipErrorInvalidValue;
     const bool vec = l.ld_logits % 4 == 0 && l.ld_out % 4 == 0 && aligned(l.logits, 16) && aligned(l.out, 16);
-    const dim3 grid((unsigned)((l.vocab + (int64_t)rf::kSlice - 1) / rf::kSlice), l.rows), blk(256);
-    if (vec)
-        hipLaunchKernelGGL(rf::rf_logits_rules_kernel<true>, grid, blk, 0, stream, l);
+    // slices of 4096 tokens (the history is read once each), of 1024 where those leave CUs idle
+    const auto slices = [&](int n) { return (unsigned)((l.vocab + (int64_t)n - 1) / n); };
+    const bool few = (int64_t)l.rows * slices(4096) < rf::device_cu_count();
+    const dim3 grid(slices(few ? 1024 : 4096), l.rows), blk(256);
+    if (vec && few)
+        hipLaunchKernelGGL((rf::rf_logits_rules_kernel<true, 1024>), grid, blk, 0, stream, l);
+    else if (vec)
+        hipLaunchKernelGGL((rf::rf_logits_rules_kernel<true, 4096>), grid, blk, 0, stream, l);
+    else if (few)
+        hipLaunchKernelGGL((rf::rf_logits_rules_kernel<false, 1024>), grid, blk, 0, stream, l);
     else
-        hipLaunchKernelGGL(rf::rf_logits_rules_kernel<false>, grid, blk, 0, stream, l);
+        hipLaunchKernelGGL((rf::rf_logits_rules_kernel<false, 4096>), grid, blk, 0, stream, l);
     return hipGetLastError();
 }
