@@ -297,6 +297,8 @@ constexpr uint32_t kSeen = 1, kBiased = 2, kMade = 4;
 template <bool VEC, int kSlice>
 __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_rules l) {
     __shared__ uint32_t count[kSlice];
+    __shared__ int listed, list_at[64], list_id[64];
+    __shared__ float list_val[64];
     constexpr int IDS = 8;                       // of the history in flight a thread
     constexpr int V = VEC ? 4 : 1, N = kSlice / (256 * V);
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, base = blockIdx.x * kSlice;
@@ -325,6 +327,7 @@ __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_ru
     const int b0 = l.bias_start != nullptr ? max(l.bias_start[r], 0) : 0;
     const int b1 = l.bias_start != nullptr ? l.bias_start[r + 1] : 0;
     for (int i = tid; i < kSlice / 4; i += 256) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) listed = 0;
     __syncthreads();
     const int* hist = l.history + r * l.ld_history;
     for (int64_t i0 = tid; i0 < total; i0 += 256 * IDS) {
@@ -342,9 +345,22 @@ __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_ru
     }
     for (int j = b0 + tid; j < b1; j += 256) {
         const uint32_t id = (uint32_t)l.bias_ids[j] - (uint32_t)base;
-        if (id < (uint32_t)n) atomicOr(&count[id], kBiased);
+        if (id < (uint32_t)n) {
+            atomicOr(&count[id], kBiased);
+            const int k = atomicAdd(&listed, 1);
+            if (k < 64) {
+                list_at[k] = j;
+                list_id[k] = (int)id;
+                list_val[k] = l.bias_values[j];
+            }
+        }
     }
     __syncthreads();
+    // the slice's entries of the bias list, one a lane, in any order
+    const bool short_list = listed <= 64;
+    const bool mine = short_list && lane < listed;
+    const int my_at = mine ? list_at[lane] : INT_MAX, my_id = mine ? list_id[lane] : -1;
+    const float my_val = mine ? list_val[lane] : 0.0f;
     const float rep = l.repetition != nullptr ? l.repetition[r] : 1.0f;
     const float freq = l.frequency != nullptr ? l.frequency[r] : 0.0f;
     const float pres = l.presence != nullptr ? l.presence[r] : 0.0f;
@@ -366,21 +382,33 @@ __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_ru
             }
             o[k] = z;
         }
-        if (b1 > b0) {
+        if (listed > 0) {
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 uint64_t marked = __ballot(c[k] & kBiased);
-                while (marked) {                 // token by token, the wave over the list
+                while (marked) {                 // token by token, its entries in list order
                     const int to = __builtin_ctzll(marked);
                     marked &= marked - 1;
-                    const int token = base + __shfl(e, to) + k;
+                    const int id = __shfl(e, to) + k;
                     float sum = 0.0f;
-                    for (int j0 = b0; j0 < b1; j0 += 64) {
-                        const bool there = j0 + lane < b1;
-                        const bool same = there && l.bias_ids[there ? j0 + lane : b0] == token;
-                        uint64_t hits = __ballot(same);
-                        const float val = same ? l.bias_values[j0 + lane] : 0.0f;
-                        for (; hits; hits &= hits - 1) sum += __shfl(val, __builtin_ctzll(hits));
+                    if (short_list) {
+                        uint64_t hits = __ballot(my_id == id);
+                        while (hits) {
+                            int next = __builtin_ctzll(hits);
+                            for (uint64_t rest = hits & (hits - 1); rest; rest &= rest - 1)
+                                if (__shfl(my_at, __builtin_ctzll(rest)) < __shfl(my_at, next))
+                                    next = __builtin_ctzll(rest);
+                            sum += __shfl(my_val, next);
+                            hits &= ~(1ull << next);
+                        }
+                    } else {
+                        for (int j0 = b0; j0 < b1; j0 += 64) {
+                            const bool there = j0 + lane < b1;
+                            const bool same = there && l.bias_ids[there ? j0 + lane : b0] == base + id;
+                            uint64_t hits = __ballot(same);
+                            const float val = same ? l.bias_values[j0 + lane] : 0.0f;
+                            for (; hits; hits &= hits - 1) sum += __shfl(val, __builtin_ctzll(hits));
+                        }
                     }
                     if (lane == to) o[k] += sum;
                 }

@@ -205,3 +205,18 @@ def test_replays(rf, dev):
         got = c.out.clone()
         c.check()
         assert torch.equal(got, c.out)
+
+
+@pytest.mark.parametrize("entries", [63, 64, 65, 300])
+@pytest.mark.parametrize("vocab", [40, 5000])
+def test_many_biases_on_few_tokens(rf, dev, entries, vocab):
+    # up to 64 entries of a slice are kept beside it, more are read again; the sums go in list order
+    c = Case(2, vocab, penal=(), bias=entries)
+    c.ids[:entries] = torch.randint(0, 30, (entries,), generator=P.gen(entries), device=P.DEV).int()
+    paged.logits_rules(c.args)
+    torch.cuda.synchronize()
+    x = c.x[0].cpu().clone()
+    add = torch.zeros(vocab)
+    for i, v in zip(c.ids[:entries].tolist(), c.val[:entries].cpu()):
+        add[i] = add[i] + v
+    assert torch.equal(c.out[0, :vocab].cpu(), x + add)
