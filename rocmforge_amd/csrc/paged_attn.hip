@@ -578,21 +578,27 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         }
         const uint32_t dst = lds0 + (values ? 2 * MAT : 0) + (uint32_t)(tile & 1) * MAT + 1024u * wave;
         const int u0 = 8 * tile - window;
-        const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
+        auto fetch = [&](auto all) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int row = wave_row + RPI * NW * i;
-            int unit = u0 + (row >> 3);
-            uint32_t off = lane_row + (values ? v_piece : k_piece);
-            if (!whole) {
-                // positions that no row sees are taken from the nearest one that some row sees
-                unit = units.seen(unit + window);
-                off = (uint32_t)(min(max(k0 + row + dr, t.lo), t.hi - 1) - 8 * unit) * stride + (values ? v_piece : k_piece);
-                unit -= window;
+            for (int i = 0; i < NI; ++i) {
+                const int row = wave_row + RPI * NW * i;
+                int unit = u0 + (row >> 3);
+                uint32_t off = lane_row + (values ? v_piece : k_piece);
+                if constexpr (!decltype(all)::value) {
+                    // positions that no row sees are taken from the nearest one that some row sees
+                    unit = units.seen(unit + window);
+                    off = (uint32_t)(min(max(k0 + row + dr, t.lo), t.hi - 1) - 8 * unit) * stride +
+                          (values ? v_piece : k_piece);
+                    unit -= window;
+                }
+                const uint64_t at = read_lane(address, unit) + (values ? v_from_k : 0);
+                lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * NW * i), off, reinterpret_cast<const uint8_t*>(at));
             }
-            const uint64_t at = read_lane(address, unit) + (values ? v_from_k : 0);
-            lds_dma16(__builtin_amdgcn_readfirstlane(dst + 1024u * NW * i), off, reinterpret_cast<const uint8_t*>(at));
-        }
+        };
+        if (k0 >= t.lo && k0 + kWideKeys <= t.hi)
+            fetch(std::true_type());
+        else
+            fetch(std::false_type());
     };
     if (begin < end) {
         next = units.page_of((8 * begin & ~63) + lane);
