@@ -49,11 +49,12 @@ constexpr float kLag = 8.0f;
 
 constexpr int kNarrowRows = 16, kNarrowKeys = 32;
 constexpr int kWideKeys = 64;
-// Parts aimed at over the chip, and the least positions of one, in units of
-// keys.  A tile is cut only where its share is longer than total / parts, so at
-// most twice as many parts are written to the workspace.
-constexpr int kNarrowParts = 512, kNarrowLeast = 4;
-constexpr int kWideLeast = 16;                   // (as many parts as workgroups fit the chip)
+// Least units of keys of a part (a workgroup costs about as much as 4 to 6 units
+// before and behind its loop; wide ones cost more: 4 / 6 / 8 / 16 units, 36.6 / 32.4 /
+// 29.9 / 28.3 us for 30 single tokens and 2 prompts of 300), and the most narrow parts
+// that are aimed at.
+constexpr int kNarrowLeast = 4, kNarrowParts = 512;
+constexpr int kWideLeast = 16;
 
 // ---- which part of which request a workgroup does ---------------------------------------
 
@@ -69,9 +70,9 @@ struct Plan {
     int group;
     uint32_t group_inv;          // 2^32 / group rounded up where r / group is the high word of r group_inv, else 0
     int from_rows, to_rows;      // requests of from_rows < packed rows <= to_rows are this kernel's
-    int parts, least;
+    int parts_log2, least;       // parts aimed at, and the least units of one
     int items;                   // at least as many as there are
-    float* slots;                // the parts' states
+    float* states;               // the parts'
 };
 
 __device__ __forceinline__ int token_of(const Plan& p, int r) {
@@ -110,6 +111,24 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
+// Units a part: total / parts.  A tile is cut only where it is longer, so at most
+// twice as many parts are written.  (In integers: the join has to come to the same.)
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int share_of(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& p,
+                                        const Request& first) {
+    const int lane = threadIdx.x & 63;
+    int64_t mine = (int64_t)first.tiles * first.units;
+    for (int b0 = 64; b0 < a.num_seqs; b0 += 64) {
+        const Request r = request_of<ROWS, KEYS>(a, c, p, b0 + lane);
+        mine += (int64_t)r.tiles * r.units;
+    }
+    const int64_t total = (((int64_t)wave_total((int)(mine >> 24)) << 24) + wave_total((int)(mine & 0xffffff))) *
+                          c.num_kv_heads;
+    return (int)min(max((total + (1 << p.parts_log2) - 1) >> p.parts_log2, (int64_t)p.least), (int64_t)1 << 30);
+}
+
 // Item j: the j-th (part, tile) over the requests, or (merge) the j-th tile of
 // more than one part.  False where there is none.  Wave-uniform.
 template <int ROWS, int KEYS>
@@ -117,14 +136,7 @@ __device__ __forceinline__ bool find_share(const rf_paged_attention& a, const rf
                                            bool merge, Share& s) {
     const int lane = threadIdx.x & 63;
     const Request first = request_of<ROWS, KEYS>(a, c, p, lane);
-    float total = (float)first.tiles * (float)first.units;
-    for (int b0 = 64; b0 < a.num_seqs; b0 += 64) {
-        const Request r = request_of<ROWS, KEYS>(a, c, p, b0 + lane);
-        total += (float)r.tiles * (float)r.units;
-    }
-    // units a part: total / parts rounded up (1.0001: the sum's own roundings)
-    total = xor_sum64(total) * ((float)c.num_kv_heads * 1.0001f);
-    const int share = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(ceilf(total / (float)p.parts), (float)p.least), 1e9f));
+    const int share = share_of<ROWS, KEYS>(a, c, p, first);
     int items_before = 0, slots_before = 0;
     for (int b0 = 0; b0 < a.num_seqs; b0 += 64) {
         const Request r = b0 == 0 ? first : request_of<ROWS, KEYS>(a, c, p, b0 + lane);
@@ -465,7 +477,7 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
     }
     __syncthreads();
     const int live = min(rows - r0, kNarrowRows);
-    float* part = slot_of<kNarrowRows, D>(plan.slots, s, s.part, kvh, nkv);
+    float* part = slot_of<kNarrowRows, D>(plan.states, s, s.part, kvh, nkv);
     for (int i = threadIdx.x; i < live * (D / 4); i += 64 * W) {
         const int row = i / (D / 4), d = 4 * (i % (D / 4));
         float mx = kNone, sum = 0.0f;
@@ -843,7 +855,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         l = xor_sum<32, M>(l);
         if (bad) l = NAN;
         if (s.parts > 1) {
-            float* to = slot_of<ROWS, D>(plan.slots, s, s.part, kvh, nkv);
+            float* to = slot_of<ROWS, D>(plan.states, s, s.part, kvh, nkv);
             const int row = M * wave + col;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
@@ -876,11 +888,13 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
 constexpr int kJoinRows = 32, kJoinParts = 64;
 
 // Head dims, waves and stages of the narrow part, waves of the wide one.
-// (MW, MS: of the narrow part beside wide ones)
+// W, S: of the narrow part by itself, one workgroup a CU; LW, LS: where there are more
+// requests than CUs or wide items beside it, two a CU, so that one's chain of loads runs
+// beside the other's loop (256 requests of 600 positions 157 -> 132 us; one of 2000 9.1 -> 9.6).
 template <int D> struct Shape;
-template <> struct Shape<64> { static constexpr int W = 4, S = 4, NW = 4, M = 32, MW = 4, MS = 2, PER_CU = 2; };
-template <> struct Shape<128> { static constexpr int W = 4, S = 2, NW = 4, M = 32, MW = 2, MS = 2, PER_CU = 2; };
-template <> struct Shape<256> { static constexpr int W = 2, S = 2, NW = 8, M = 16, MW = 2, MS = 2, PER_CU = 1; };
+template <> struct Shape<64> { static constexpr int W = 4, S = 4, LW = 4, LS = 2, NW = 4, M = 32, PER_CU = 2; };
+template <> struct Shape<128> { static constexpr int W = 4, S = 2, LW = 2, LS = 2, NW = 4, M = 32, PER_CU = 2; };
+template <> struct Shape<256> { static constexpr int W = 2, S = 2, LW = 1, LS = 2, NW = 8, M = 16, PER_CU = 1; };
 template <int D>
 constexpr int narrow_lds(int w, int s) { return w * s * 2 * kNarrowKeys * 2 * D; }
 template <int D>
@@ -890,11 +904,12 @@ constexpr int wide_rows() { return Shape<D>::M * Shape<D>::NW; }
 template <int D>
 constexpr int wide_parts() { return 256 * Shape<D>::PER_CU; }
 
-template <int D>
-__global__ __launch_bounds__(64 * Shape<D>::W)
+template <int D, bool LIGHT>
+__global__ __launch_bounds__(64 * (LIGHT ? Shape<D>::LW : Shape<D>::W))
 void rf_paged_attn_narrow_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan plan) {
-    __shared__ __align__(1024) uint8_t lds[narrow_lds<D>(Shape<D>::W, Shape<D>::S)];
-    narrow_part<D, Shape<D>::W, Shape<D>::S>(a, c, plan, (int)(blockIdx.x + blockIdx.y * gridDim.x), lds);
+    constexpr int W = LIGHT ? Shape<D>::LW : Shape<D>::W, S = LIGHT ? Shape<D>::LS : Shape<D>::S;
+    __shared__ __align__(1024) uint8_t lds[narrow_lds<D>(W, S)];
+    narrow_part<D, W, S>(a, c, plan, (int)(blockIdx.x + blockIdx.y * gridDim.x), lds);
 }
 
 // Both kinds in one launch, the wide items first: their workgroups are the
@@ -902,14 +917,14 @@ void rf_paged_attn_narrow_kernel(const rf_paged_attention a, const rf_paged_cach
 template <int D>
 __global__ __launch_bounds__(64 * Shape<D>::NW) __attribute__((amdgpu_waves_per_eu(2)))
 void rf_paged_attn_mixed_kernel(const rf_paged_attention a, const rf_paged_cache c, const Plan wide, const Plan narrow) {
-    constexpr int MW = Shape<D>::MW, MS = Shape<D>::MS, NEED = narrow_lds<D>(MW, MS);
+    constexpr int LW = Shape<D>::LW, LS = Shape<D>::LS, NEED = narrow_lds<D>(LW, LS);
     __shared__ __align__(1024) uint8_t lds[NEED > wide_lds<D>() ? NEED : wide_lds<D>()];
     const int item = (int)(blockIdx.x + blockIdx.y * gridDim.x);
     if (item < wide.items) {
         wide_part<D, Shape<D>::NW, Shape<D>::M>(a, c, wide, item, lds);
     } else {
-        if (threadIdx.x >= 64 * MW) return;      // whole waves, before any barrier
-        narrow_part<D, MW, MS>(a, c, narrow, item - wide.items, lds);
+        if (threadIdx.x >= 64 * LW) return;      // whole waves, before any barrier
+        narrow_part<D, LW, LS>(a, c, narrow, item - wide.items, lds);
     }
 }
 
@@ -929,7 +944,7 @@ __device__ __forceinline__ void join_part(const rf_paged_attention& a, const rf_
     const int live = min(rows - r0 - first, JR);
     if (live <= 0) return;
     const int64_t next = (int64_t)s.tiles * nkv * (ROWS * (D + 2));
-    const float* part0 = slot_of<ROWS, D>(plan.slots, s, 0, kvh, nkv) + first * D;
+    const float* part0 = slot_of<ROWS, D>(plan.states, s, 0, kvh, nkv) + first * D;
     const float* m0 = part0 + (ROWS - first) * D + first;
     const int row = tid / LANES;                 // LANES lanes a row
     float mx = kNone, sum = 0.0f;
@@ -1017,16 +1032,22 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
     const bool both = (int64_t)a.max_new * group > kNarrowRows;
     float* ws = static_cast<float*>(a.workspace);
     const uint32_t inv = packed * group < (1ll << 32) ? (uint32_t)(((1ll << 32) + group - 1) / group) : 0;
-    Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, kNarrowParts, kNarrowLeast, 0, ws};
-    Plan wide = {group, inv, kNarrowRows, INT_MAX, wide_parts<D>(), kWideLeast, 0, ws + narrow_bytes<D>() / sizeof(float)};
-    // Items: every tile has a part, and there are at most `parts` parts more (each of them a share
-    // long); no more either than the table's width gives room for.
-    const auto items = [&](int64_t tiles, const Plan& p, int keys, int64_t* joins) {
-        const int64_t most = std::max<int64_t>((positions + keys * p.least - 1) / (keys * p.least), 1);
-        *joins = most > 1 ? std::min<int64_t>(tiles, p.parts) : 0;
-        return (int)std::min(tiles + p.parts, tiles * most);
-    };
     const int64_t some = std::min<int64_t>(a.num_seqs, a.rows);        // requests with rows
+    // One round of long parts for few tiles, two of shorter ones (which even out a ragged batch) for
+    // more.  us, 256 parts / 512: one request of 16000 positions 20.3 / 26.6, 8 of 2000 18.8 / 22.3, 32 of
+    // 1000 25.9 / 30.9, 48 of 60 to 16000 141 / 126.
+    const bool light = both || some * nkv >= 512;
+    Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, some * nkv <= 256 && !both ? 8 : 9, kNarrowLeast, 0, ws};
+    Plan wide = {group, inv, kNarrowRows, INT_MAX, Shape<D>::PER_CU == 2 ? 9 : 8, kWideLeast, 0,
+                 ws + narrow_bytes<D>() / sizeof(float)};
+    // Items: every tile has a part, and there are at most as many parts more as are aimed at (each of
+    // them a share long); no more either than the table's width gives room for.
+    const auto items = [&](int64_t tiles, const Plan& p, int keys, int64_t* joins) {
+        const int64_t parts = 1ll << p.parts_log2;
+        const int64_t most = std::max<int64_t>((positions + keys * p.least - 1) / (keys * p.least), 1);
+        *joins = most > 1 ? std::min<int64_t>(tiles, parts) : 0;
+        return (int)std::min(tiles + parts, tiles * most);
+    };
     int64_t narrow_joins, wide_joins = 0;
     narrow.items = items((both ? some : packed / kNarrowRows + some) * nkv, narrow, kNarrowKeys, &narrow_joins);
     if (both) {
@@ -1039,7 +1060,8 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
     if (both)
         hipLaunchKernelGGL(rf_paged_attn_mixed_kernel<D>, grid, dim3(64 * Shape<D>::NW), 0, stream, a, c, wide, narrow);
     else
-        hipLaunchKernelGGL(rf_paged_attn_narrow_kernel<D>, grid, dim3(64 * Shape<D>::W), 0, stream, a, c, narrow);
+        hipLaunchKernelGGL((light ? rf_paged_attn_narrow_kernel<D, true> : rf_paged_attn_narrow_kernel<D, false>), grid,
+                           dim3(64 * (light ? Shape<D>::LW : Shape<D>::W)), 0, stream, a, c, narrow);
     const int wide_blocks = (int)wide_joins * (ROWS / kJoinRows);
     if (wide_joins + narrow_joins > 0)
         hipLaunchKernelGGL(rf_paged_attn_join_kernel<D>, dim3((unsigned)(wide_blocks + narrow_joins)), dim3(256), 0,
