@@ -646,7 +646,8 @@ hipError_t rf_gemv_qkv_q4_k_q6_k_v_rmsnorm_launch(const void* w_q, const void* w
  * memory, so captured steps replay with the values they then hold.  The
  * current device must be the stream's.  The launchers allocate nothing, do not
  * synchronise, return hipErrorInvalidValue on a rejected argument and are
- * otherwise as those above.  Zero rows or requests: success, nothing written. */
+ * otherwise as those above.  Zero rows or requests: success, nothing written
+ * (the plan writes unless both are zero). */
 
 /* K and V pages of one layer, fp16 bits.  Position t of a request, head h, dim
  * i: k[page * page_stride + (t % page_size) * row_stride + h * head_stride + i]
@@ -779,7 +780,8 @@ hipError_t rf_paged_rope_write_launch(const rf_paged_rope* step, const rf_paged_
  * outside [0, num_pages) in the positions that it sees may get NaN, and nothing
  * outside the cache is read.  workspace: rf_paged_attention_workspace_bytes
  * bytes, 16-byte aligned (launches that share one must be stream-ordered).
- * q, out 16-byte aligned, ld_q, ld_out multiples of 8; scale finite; window >= 0;
+ * out and workspace overlap no other buffer, q_start does not fall.  q, out 16-byte
+ * aligned, ld_q, ld_out multiples of 8; scale finite; window >= 0;
  * num_heads a multiple of num_kv_heads, at most 64 of them a KV head; rows *
  * num_heads <= 2^27. */
 typedef struct rf_paged_attention {

@@ -450,8 +450,9 @@ extern "C" hipError_t rf_paged_plan_launch(const rf_paged_plan* plan, hipStream_
         hipLaunchKernelGGL(rf::rf_paged_plan_kernel<true>, dim3(1), dim3(rf::kPlanThreads), 0, stream, p);
     } else {
         hipLaunchKernelGGL(rf::rf_paged_plan_kernel<false>, dim3(1), dim3(rf::kPlanThreads), 0, stream, p);
-        hipLaunchKernelGGL(rf::rf_paged_rows_kernel, dim3((unsigned)(((int64_t)p.max_rows + 255) / 256)), dim3(256), 0,
-                           stream, p);
+        if (p.max_rows > 0)
+            hipLaunchKernelGGL(rf::rf_paged_rows_kernel, dim3((unsigned)(((int64_t)p.max_rows + 255) / 256)), dim3(256),
+                               0, stream, p);
     }
     return hipGetLastError();
 }

@@ -126,6 +126,12 @@ def test_rows_and_tables_run_out(rf, dev):
     Step([1, 1], [2000, 3], max_rows=0).check()
 
 
+@pytest.mark.parametrize("seqs", [1024, 1025])
+def test_many_requests_and_no_rows(rf, dev, seqs):
+    Step([0] * seqs, list(range(seqs)), free=0, max_rows=0).check()
+    Step([1] * seqs, [16] * seqs, free=9, max_rows=0).check()
+
+
 def test_bad_lengths_are_refused(rf, dev):
     Step([3, -4, 2, 1], [10, 5, -3, 1], width=4).check()
     Step([1, INT_MAX, 1], [0, 5, 0], width=4, max_rows=9).check()

@@ -83,6 +83,10 @@ def test_attentions(rf, bad):
     refused(paged.attention, attn(**bad), cache())
 
 
+def test_more_rows_and_heads_than_a_launch_counts(rf):
+    refused(paged.attention, attn(rows=1 << 23, num_heads=32, ld_q=4096, ld_out=4096), cache())
+
+
 @pytest.mark.parametrize("bad", [dict(logits=None), dict(out=None), dict(ld_logits=999), dict(ld_out=999),
                                  dict(rows=-1), dict(rows=65536), dict(vocab=-1), dict(bias_ids=None),
                                  dict(bias_start=None), dict(history=None), dict(prompt_lens=None),
