@@ -19,7 +19,7 @@ namespace rf {
 // row.  Bound by latency: a request is two ints and a row two more (57 KB of
 // output at 14 k rows).  One workgroup scans; where there are few rows it
 // writes them as well (one launch), else a second launch spreads them over
-// the chip.
+// the chip.  64 requests of one token 5.7 us; 300 of 14 k rows 5.4 and 3.8.
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
@@ -214,7 +214,8 @@ __global__ void rf_rope_turns_kernel(double* __restrict__ turns, int rot, double
 // reductions).  Lanes u < rot / 8 of a head hold four whole pairs -- elements
 // 4 u .. and rot / 2 + 4 u .. (neox), or 8 u .. -- so a pair never crosses a
 // lane; the others hold 8 elements behind the turned part.  Memory-bound: 4
-// bytes in and 2 out an element, all of it in 16- and 8-byte pieces.
+// bytes in and 2 out an element, all of it in 16- and 8-byte pieces.  4000 rows of
+// 48 heads of 128: 31 us, 4.7 TB/s; one row 3.0 us.
 template <int D, bool NEOX>
 __global__ __launch_bounds__(256) void rf_paged_rope_kernel(const rf_paged_rope s, const rf_paged_cache c) {
     constexpr int LPH = D / 8, HPB = 256 / LPH;
@@ -290,7 +291,8 @@ __global__ __launch_bounds__(256) void rf_paged_rope_kernel(const rf_paged_rope 
 // the atomics does not matter), marks the bias list's, and writes the slice in
 // one pass; a marked token's wave adds up its entries in list order.  The
 // history is read once a slice, from L2.  Bound: 8 bytes a token, and for few
-// rows the latency of history and logits.
+// rows the latency of history and logits.  64 rows of 151936 tokens, masked, 1 to
+// 8000 tokens of history: 23 us, 3.5 TB/s; one row with 4000 6 us.
 // of a token in LDS: its place in the history, a mark for the bias list, a count of those not in the prompt
 constexpr uint32_t kSeen = 1, kBiased = 2, kMade = 4;
 

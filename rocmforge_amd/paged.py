@@ -12,8 +12,8 @@ blocks on its buffers, and runs a step of a batch as
     logits_rules(l)               before a token is picked
 
 with release() for requests that ended.  The argument blocks are the C
-structs; pointer fields take device addresses, torch tensors (kept alive by
-the block) or None.  Launches go to the given stream, else to torch's current
+structs; pointer fields take device addresses, torch tensors of the GPU (kept
+alive by the block) or None.  Launches go to the given stream, else to torch's current
 one, and raise ops.HipApiError where the library refuses the arguments.
 """
 from __future__ import annotations
@@ -41,7 +41,7 @@ class _Block(ctypes.Structure):
     def __setattr__(self, name, value):
         if hasattr(value, "data_ptr"):
             self.__dict__.setdefault("_kept", {})[name] = value
-            value = value.data_ptr()
+            value = _addr(value)
         super().__setattr__(name, value)
 
 
@@ -82,7 +82,11 @@ class LogitsRules(_Block):
 
 
 def _addr(p):
-    return p.data_ptr() if hasattr(p, "data_ptr") else p
+    if not hasattr(p, "data_ptr"):
+        return p
+    if not p.is_cuda:
+        raise ValueError("a tensor that is not on a GPU")
+    return p.data_ptr()
 
 
 def _stream(stream):

@@ -141,6 +141,20 @@ def test_workspaces_of_no_launch(rf, args):
     assert paged.attention_workspace_bytes(*args) == 0
 
 
+def test_tensors_of_the_host(rf):
+    import torch
+    t = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        plan(new_lens=t)
+    p = plan()
+    with pytest.raises(ValueError):
+        p.kv_lens = t
+    with pytest.raises(ValueError):
+        paged.release(t, A, A, A, A, 1, 4, 16, 8, 0)
+    with pytest.raises(ValueError):
+        paged.rope_turns_table(t, 8, 1e4, stream=0)
+
+
 def test_unknown_fields(rf):
     with pytest.raises(TypeError):
         paged.PagedCache(pages=3)
