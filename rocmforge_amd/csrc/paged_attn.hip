@@ -50,11 +50,17 @@ constexpr float kLag = 8.0f;
 constexpr int kNarrowRows = 16, kNarrowKeys = 32;
 constexpr int kWideKeys = 64;
 // Least units of keys of a part (a workgroup costs about as much as 4 to 6 units
-// before and behind its loop; wide ones cost more: 4 / 6 / 8 / 16 units, 36.6 / 32.4 /
-// 29.9 / 28.3 us for 30 single tokens and 2 prompts of 300), and the most narrow parts
-// that are aimed at.
-constexpr int kNarrowLeast = 4, kNarrowParts = 512;
-constexpr int kWideLeast = 16;
+// before and behind its loop; wide ones, and narrow ones beside them, more: 4 prompts of
+// 200 behind 2800 72 us at 16 wide units and 65 at 24, 64 tokens behind 15936 52 and 54),
+// and the most narrow parts that are aimed at.
+constexpr int kNarrowLeast = 4, kBesideLeast = 16, kNarrowParts = 512;
+constexpr int kWideLeast = 24;
+// Where tables are no wider than these many units nothing is cut, and no join is launched: for
+// few narrow tiles (one request of 256 positions 8.4 -> 6.1 us, of 500 9.0 -> 8.6, of 1000 would
+// take 12.6 for 9.0), for 256 and more or beside wide ones (32 requests of 20 to 1000 17.4 -> 15.4,
+// 256 of 600 131 -> 125, 20 of 500 beside two prompts 32 -> 26.6), and for wide tiles (a prompt of
+// 1500 49 -> 41).
+constexpr int kFewWhole = 16, kManyWhole = 32, kWideWhole = 32;
 
 // ---- which part of which request a workgroup does ---------------------------------------
 
@@ -1051,9 +1057,12 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
     // more.  us, 256 parts / 512: one request of 16000 positions 20.3 / 26.6, 8 of 2000 18.8 / 22.3, 32 of
     // 1000 25.9 / 30.9, 48 of 60 to 16000 141 / 126.
     const bool light = both || some * nkv >= 512;
-    Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, some * nkv <= 256 && !both ? 8 : 9, kNarrowLeast, 0, ws};
-    Plan wide = {group, inv, kNarrowRows, INT_MAX, Shape<D>::PER_CU == 2 ? 9 : 8, kWideLeast, 0,
-                 ws + narrow_bytes<D>() / sizeof(float)};
+    const auto least = [&](int keys, int whole, int cut) { return positions <= whole * keys ? whole : cut; };
+    const int narrow_least = least(kNarrowKeys, both || some * nkv >= 256 ? kManyWhole : kFewWhole,
+                                   both ? kBesideLeast : kNarrowLeast);
+    Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, some * nkv <= 256 && !both ? 8 : 9, narrow_least, 0, ws};
+    Plan wide = {group, inv, kNarrowRows, INT_MAX, Shape<D>::PER_CU == 2 ? 9 : 8,
+                 least(kWideKeys, kWideWhole, kWideLeast), 0, ws + narrow_bytes<D>() / sizeof(float)};
     // Items: every tile has a part, and there are at most as many parts more as are aimed at (each of
     // them a share long); no more either than the table's width gives room for.
     const auto items = [&](int64_t tiles, const Plan& p, int keys, int64_t* joins) {
