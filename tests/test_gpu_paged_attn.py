@@ -213,6 +213,18 @@ def test_pages_outside_the_cache_are_not_read(rf, dev, new, kv, bad):
     assert bool((got[new[0]:] == want[new[0]:]).all()) and bool(got[:new[0]].isnan().all())
 
 
+@pytest.mark.parametrize("d,nh,nkv", [(64, 4, 1), (128, 8, 2), (128, 7, 1), (256, 6, 2)])
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("new,kv", [([1], [500]), ([1, 1, 2], [130, 1000, 700]), ([100], [100]), ([3, 90, 1], [200, 2100, 900]),
+                                    ([400], [3500]), ([9, 0, 140, 1], [160, 50, 1700, 3])])
+def test_tables_wider_than_the_lengths(rf, dev, new, kv, window, d, nh, nkv):
+    # (the table's width bounds the parts that a request may be cut into)
+    c = Case(new, kv, nh, nkv, d, window=window)
+    c.tab = torch.nn.functional.pad(c.tab, (0, 6000 - c.tab.shape[1]), value=-3).contiguous()
+    c.args.block_tables, c.args.max_blocks = c.tab, 6000
+    c.check()
+
+
 def test_lengths_beyond_the_table_are_clipped(rf, dev):
     c = Case([1, 60], [100, 100], page=32)
     c.args.max_blocks = 4
