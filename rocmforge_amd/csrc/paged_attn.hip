@@ -76,7 +76,8 @@ struct Plan {
     int group;
     uint32_t group_inv;          // 2^32 / group rounded up where r / group is the high word of r group_inv, else 0
     int from_rows, to_rows;      // requests of from_rows < packed rows <= to_rows are this kernel's
-    int parts_log2, least;       // parts aimed at, and the least units of one
+    int parts, least;            // parts aimed at, and the least units of one
+    uint32_t parts_inv;          // 2^32 / parts, rounded up
     int items;                   // at least as many as there are
     float* states;               // the parts'
 };
@@ -132,7 +133,10 @@ __device__ __forceinline__ int share_of(const rf_paged_attention& a, const rf_pa
     }
     const int64_t total = (((int64_t)wave_total((int)(mine >> 24)) << 24) + wave_total((int)(mine & 0xffffff))) *
                           c.num_kv_heads;
-    return (int)min(max((total + (1 << p.parts_log2) - 1) >> p.parts_log2, (int64_t)p.least), (int64_t)1 << 30);
+    // (rounded up; in 32 bits, in steps of 2^20 where the sum has more)
+    const int sh = total >> 31 ? 20 : 0;
+    const uint32_t steps = (uint32_t)((total + (1 << sh) - 1) >> sh), each = __umulhi(max(steps, 1u) - 1, p.parts_inv) + 1;
+    return (int)min(max((int64_t)each << sh, (int64_t)p.least), (int64_t)1 << 30);
 }
 
 // Item j: the j-th (part, tile) over the requests, or (merge) the j-th tile of
@@ -1051,30 +1055,42 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
     const int64_t packed = (int64_t)a.rows * group, positions = (int64_t)a.max_blocks * c.page_size;
     const bool both = (int64_t)a.max_new * group > kNarrowRows;
     float* ws = static_cast<float*>(a.workspace);
-    const uint32_t inv = packed * group < (1ll << 32) ? (uint32_t)(((1ll << 32) + group - 1) / group) : 0;
+    const auto inverse = [](int n) { return (uint32_t)(((1ll << 32) + n - 1) / n); };
+    const uint32_t inv = packed * group < (1ll << 32) ? inverse(group) : 0;
     const int64_t some = std::min<int64_t>(a.num_seqs, a.rows);        // requests with rows
-    // One round of long parts for few tiles, two of shorter ones (which even out a ragged batch) for
-    // more.  us, 256 parts / 512: one request of 16000 positions 20.3 / 26.6, 8 of 2000 18.8 / 22.3, 32 of
-    // 1000 25.9 / 30.9, 48 of 60 to 16000 141 / 126.
-    const bool light = both || some * nkv >= 512;
+    // The narrow launch.  Fewer than 64 tiles, or up to 256 of short tables: 256 parts, one round of
+    // workgroups with most loads in flight.  Else up to 256: two workgroups a CU, and half a part less for
+    // every tile, since the last part of a tile is half a one on average -- one round again.  Up to 511: two rounds, which even out a
+    // ragged batch.  From 512 tiles on light workgroups again.  us, 256 parts of heavy ones / 512 of
+    // heavy ones / 512 - tiles / 2 of light ones: 2 requests of 8000 (8 KV heads) 19.4 / 24.5 / 20.4;
+    // 8 of 2000 19.2 / 22.8 / 20.3; 8 of 100 to 8000 27.7 / 25.9 / 21.8; 20 of 4000 77.8 / 72.2 / 60.9;
+    // 32 of 100 to 8000 66.5 / 60.6 / 58.9; 48 of 60 to 16000 168 / 146 / 149; 64 of them 241 / 208 / 236;
+    // 32 of 1000 in a table as wide 26.3 / 30.9 / 28.3.
+    const int64_t tiles = some * nkv;
+    const bool few = !both && (tiles < 64 || (tiles <= 256 && positions <= 2048)), some_tiles = !both && !few && tiles <= 256;
+    const bool light = both || some_tiles || tiles >= 512;
+    const int aim = few ? 256 : some_tiles ? kNarrowParts - (int)tiles / 2 : kNarrowParts;
     const auto least = [&](int keys, int whole, int cut) { return positions <= whole * keys ? whole : cut; };
-    const int narrow_least = least(kNarrowKeys, both || some * nkv >= 256 ? kManyWhole : kFewWhole,
+    const int narrow_least = least(kNarrowKeys, both || tiles >= 256 ? kManyWhole : kFewWhole,
                                    both ? kBesideLeast : kNarrowLeast);
-    Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, some * nkv <= 256 && !both ? 8 : 9, narrow_least, 0, ws};
-    Plan wide = {group, inv, kNarrowRows, INT_MAX, Shape<D>::PER_CU == 2 ? 9 : 8,
-                 least(kWideKeys, kWideWhole, kWideLeast), 0, ws + narrow_bytes<D>() / sizeof(float)};
+    Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, aim, narrow_least, inverse(aim), 0, ws};
+    // (fewer parts for many wide tiles likewise: 100 single tokens beside 4 prompts of 300 152 -> 132, and
+    // to half a part less for each, 512 tokens behind 8000 three times 229 -> 240)
+    const int64_t wide_tiles = (packed / ROWS + std::min(some, packed / kNarrowRows)) * nkv;
+    const int wide_aim = (int)std::max<int64_t>(wide_parts<D>() - wide_tiles / 4, wide_parts<D>() / 4);
+    Plan wide = {group, inv, kNarrowRows, INT_MAX, wide_aim, least(kWideKeys, kWideWhole, kWideLeast), inverse(wide_aim), 0,
+                 ws + narrow_bytes<D>() / sizeof(float)};
     // Items: every tile has a part, and there are at most as many parts more as are aimed at (each of
     // them a share long); no more either than the table's width gives room for.
     const auto items = [&](int64_t tiles, const Plan& p, int keys, int64_t* joins) {
-        const int64_t parts = 1ll << p.parts_log2;
         const int64_t most = std::max<int64_t>((positions + keys * p.least - 1) / (keys * p.least), 1);
-        *joins = most > 1 ? std::min<int64_t>(tiles, parts) : 0;
-        return (int)std::min(tiles + parts, tiles * most);
+        *joins = most > 1 ? std::min<int64_t>(tiles, p.parts) : 0;
+        return (int)std::min(tiles + p.parts, tiles * most);
     };
     int64_t narrow_joins, wide_joins = 0;
     narrow.items = items((both ? some : packed / kNarrowRows + some) * nkv, narrow, kNarrowKeys, &narrow_joins);
     if (both) {
-        wide.items = items((packed / ROWS + std::min(some, packed / kNarrowRows)) * nkv, wide, kWideKeys, &wide_joins);
+        wide.items = items(wide_tiles, wide, kWideKeys, &wide_joins);
         // (workgroups i and i + 8 share an XCD's L2, and items i and i + num_kv_heads their K and V)
         wide.items = (wide.items + 8 * nkv - 1) / (8 * nkv) * (8 * nkv);
     }
