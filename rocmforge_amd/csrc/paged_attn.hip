@@ -298,7 +298,7 @@ __device__ __forceinline__ V finite_of(V v) {
 // costs no bytes.  Bound by memory, and for short requests by the chain lengths ->
 // share -> page -> K -> V and the join's launch.  48 requests of 60 to 16000
 // positions (32 heads on 8, head_dim 128, 556 MB): 120 us with the join, 4.6 TB/s
-// where a large copy reaches 5.1; one request of 640: 8.7 us.
+// where a large copy reaches 5.1; one request of 640: 8.8 us.
 template <int D, int W, int S>
 __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan,
                                             int item, uint8_t* lds) {
@@ -530,8 +530,8 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
 // outputs in accumulation registers 79.
 // Bound at head_dim 128 by MFMA, softmax VALU and LDS reads, each about half of
 // the time busy and overlapping across two waves a SIMD: a fresh prompt of 8192
-// (32 heads on 8) 565 to 590 us, 930 to 970 TFLOP/s where a large product reaches
-// 1160; 512 tokens behind 15700 156 to 164 us.  At 256 by LDS reads (4096 clocks
+// (32 heads on 8) 543 to 593 us, 930 to 1010 TFLOP/s where a large product reaches
+// 1160; 512 tokens behind 15700 155 to 164 us.  At 256 by LDS reads (4096 clocks
 // a CU and tile beside 2048 of MFMA): 390 TFLOP/s.
 
 // The two MFMA shapes.  M packed rows a wave; acc: a block of scores or outputs, whose
@@ -910,9 +910,9 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
 constexpr int kJoinRows = 32, kJoinParts = 64;
 
 // Head dims, waves and stages of the narrow part, waves of the wide one.
-// W, S: of the narrow part by itself, one workgroup a CU; LW, LS: where there are more
-// requests than CUs or wide items beside it, two a CU, so that one's chain of loads runs
-// beside the other's loop (256 requests of 600 positions 157 -> 132 us; one of 2000 9.1 -> 9.6).
+// W, S: heavy workgroups of the narrow launch, one a CU; LW, LS: light ones, two a CU, so
+// that one's chain of loads runs beside the other's loop, for many tiles and beside wide
+// items (256 requests of 600 positions 157 -> 132 us; one of 2000 9.1 -> 9.6).
 template <int D> struct Shape;
 template <> struct Shape<64> { static constexpr int W = 4, S = 4, LW = 4, LS = 2, NW = 4, M = 32, PER_CU = 2; };
 template <> struct Shape<128> { static constexpr int W = 4, S = 2, LW = 2, LS = 2, NW = 4, M = 32, PER_CU = 2; };
