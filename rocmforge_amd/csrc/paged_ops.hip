@@ -112,7 +112,7 @@ __global__ __launch_bounds__(kPlanThreads) void rf_paged_plan_kernel(const rf_pa
         page_first[t] = (int)have;
         if (granted && need > 0) atomicMax(&granted_end, (int)end);
         __syncthreads();
-        // page i of this round belongs to the first request whose end passes it
+        // page i belongs to the first of these requests whose end passes it
         for (int64_t i = pages_before + t; i < granted_end; i += kPlanThreads) {
             int lo = 0, hi = kPlanThreads - 1;
             while (lo < hi) {
