@@ -472,7 +472,7 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
             for (int i = 0; i < NB; ++i) {
                 const h4 w = *reinterpret_cast<const h4*>(row + 16 * i), f = finite_of(w);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][e] += seen ? (float)w[e] - (float)f[e] : 0.0f;
+                for (int e = 0; e < 4; ++e) o[i][e] = seen ? o[i][e] + ((float)w[e] - (float)f[e]) : o[i][e];
             }
         }
     }
@@ -851,14 +851,15 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
 #pragma unroll 1
     for (; tile < end; ++tile) advance(tile);
     if (dirty) {
-        // the values that were replaced, to the rows that see them
+        // the values that were replaced, to the rows that see them: those of the tiles that were run masked
         const int psh = units.psh, pmask = units.pmask;
         const int* table = units.table;
         const uint16_t* vc = c.v + kvh * c.head_stride;
 #pragma unroll 1
-        for (int k0 = kWideKeys * begin; k0 < kWideKeys * end; ++k0) {
-            const int k32 = k0 & ~31;
-            if (!(k32 + 31 > u.first || (a.window > 0 && k32 <= u.last - a.window)) || k0 < t.lo || k0 >= t.hi) continue;
+        for (int k0 = kWideKeys * mine; k0 < kWideKeys * mine_end; ++k0) {
+            if (k0 == kWideKeys * full) k0 = kWideKeys * full_end;
+            if (k0 >= kWideKeys * mine_end) break;
+            if (k0 < t.lo || k0 >= t.hi) continue;
             const int page = table[k0 >> psh];
             if ((unsigned)page >= (unsigned)c.num_pages) continue;
             const uint16_t* row = vc + (int64_t)page * c.page_stride + (int64_t)(k0 & pmask) * c.row_stride + 4 * part;
@@ -869,7 +870,8 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
                 for (int e = 0; e < E; e += 4) {
                     const h4 w = *reinterpret_cast<const h4*>(row + M * i + G::key(e)), f = finite_of(w);
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) o[i][e + n] += seen ? (float)w[n] - (float)f[n] : 0.0f;
+                    for (int n = 0; n < 4; ++n)
+                        o[i][e + n] = seen ? o[i][e + n] + ((float)w[n] - (float)f[n]) : o[i][e + n];
                 }
         }
     }
