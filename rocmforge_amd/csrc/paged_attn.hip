@@ -44,7 +44,9 @@ constexpr float kNone = -3.0e+38f;               // the maximum of no scores
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's maximum is left behind until a score passes it by more than 2^8: most
 // tiles then rescale nothing.  Weights reach 256 (fp16 ends at 65504), and since
-// the sum is of the rounded weights, a row of one key still has it exactly.
+// the sum is of the rounded weights, a row of one key still has it exactly.  Each row
+// renews its own: were a wave's rows renewed together, keys that only some of
+// them see would enter the others' roundings.
 constexpr float kLag = 8.0f;
 
 constexpr int kNarrowRows = 16, kNarrowKeys = 32;
@@ -416,9 +418,10 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
                 top = fmaxf(top, x[b][e]);
             }
         top = xor_butterfly<32, 16>(top, max_raw);
-        if (__ballot(top > m + kLag)) {
-            const float mn = max_raw(m, top), f = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
+        const bool up = top > m + kLag;
+        if (__ballot(up)) {
+            const float f = up ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+            m = up ? top : m;
             l *= f;
 #pragma unroll
             for (int i = 0; i < NB; ++i) o[i] *= f;
@@ -724,22 +727,24 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         // exp(x - m) as 2^(x scale - m), one fma: m is a rounded product and the fma's is not, so
         // a row's weights are off by one common factor of 2^(half a step of m).  Far from zero
         // (2^7) scores are rounded as m is, lest the factor leave fp16's range.
+        const bool up = top > m + kLag;
         float mul = scale;
-        if (__ballot(top > m + kLag) || far) {
-            const float mn = max_raw(m, top), f = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
+        if (__ballot(up || far)) {
+            const float f = up ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+            m = up ? top : m;
             l *= f;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[i][e] *= f;
-            far = __ballot(fabsf(m) >= 128.0f && m != kNone) != 0;
-            if (far) {
+            far = fabsf(m) >= 128.0f && m != kNone;
+            if (__ballot(far)) {
+                const float by = far ? scale : 1.0f;
 #pragma unroll
                 for (int b = 0; b < XB; ++b)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) x[b][e] = __fmul_rn(x[b][e], scale);
-                mul = 1.0f;
+                    for (int e = 0; e < E; ++e) x[b][e] = __fmul_rn(x[b][e], by);
+                mul = far ? 1.0f : scale;
             }
         }
         // (past the last tile of K the scores are of what its buffer holds, and are not used)
