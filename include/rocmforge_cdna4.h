@@ -769,7 +769,8 @@ hipError_t rf_paged_rope_write_launch(const rf_paged_rope* step, const rf_paged_
  * new ones) stands at position p = kv - n + i and sees positions max(0, p -
  * window + 1) .. p (window 0: all up to p): out = sum_j softmax_j(scale q . k_j)
  * v_j, query head h on KV head h / (num_heads / num_kv_heads).  A row that sees
- * nothing (p < 0) gets zeros; rows past q_start[num_seqs] are left as they were.
+ * nothing (p < 0) gets zeros, one that sees only scores of -inf NaN; rows past
+ * q_start[num_seqs] are left as they were.
  * What lies in the cache behind a row's position, or in front of its window,
  * does not enter, whatever it holds.  q fp16 bits [row][ld_q], out fp16 bits
  * (rounded once from fp32) or fp32 (out_f32 != 0) [row][ld_out].  The weights are

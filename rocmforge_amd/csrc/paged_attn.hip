@@ -516,8 +516,9 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
             }
         } else {
             const int tk = token_of(plan, r0 + row), hd = r0 + row - tk * plan.group;
+            // (a row in front of position 0 sees nothing; one whose scores are all -inf is 0 / 0)
             store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d,
-                   sum == 0.0f ? f4{0, 0, 0, 0} : acc * (1.0f / sum));
+                   s.kv - s.n + tk < 0 ? f4{0, 0, 0, 0} : acc * (1.0f / sum));
         }
     }
 }
@@ -897,11 +898,11 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
                 to[ROWS * (D + 1) + row] = l;
             }
         } else {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             // (worked out again, not kept in registers over the loop)
             int row = w0 + col;
             asm("" : "+v"(row));
             const int tk = token_of(plan, row), hd = row - tk * plan.group;
+            const float inv = s.kv - s.n + tk < 0 ? 0.0f : 1.0f / l;
             const int64_t at = (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + 4 * part;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
@@ -1009,7 +1010,8 @@ __device__ __forceinline__ void join_part(const rf_paged_attention& a, const rf_
     }
     sum = xor_sum<LANES / 2, 1>(sum);
     __syncthreads();
-    if (row < live && tid % LANES == 0) weight[0][row] = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (row < live && tid % LANES == 0)
+        weight[0][row] = s.kv - s.n + token_of(plan, r0 + first + row) < 0 ? 0.0f : 1.0f / sum;
     sums[tid] = acc[0];
     __syncthreads();
     if (g > 0) return;
