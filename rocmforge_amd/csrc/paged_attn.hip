@@ -644,13 +644,17 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const rf_
         stage(std::true_type(), begin);
         if constexpr (BESIDE) stage(std::false_type(), begin + 1);
     }
-    // a negative scale moves its sign to Q (exact), so that the largest S has the largest weight
+    // a negative scale moves its sign to Q (exact), so that the largest S has the largest weight; a
+    // scale of zero goes to Q whole, so that what is infinite in Q or K gives NaN
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
     const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
     h8 q[KS];
     const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 8 * part;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) q[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qrow + G::DK * k) ^ sign);
+    for (int k = 0; k < KS; ++k) {
+        q[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qrow + G::DK * k) ^ sign);
+        if (a.scale == 0.0f) q[k] *= (_Float16)0;
+    }
     // operand addresses: one base, and an xor for each k-step or block of dims
     const int i16 = lane & 15, vr = 4 * part + (i16 >> 2);
     const uint32_t ka = lds0 + (uint32_t)col * ROWB + 16u * (uint32_t)(part ^ k_swizzle<D>(col));

@@ -67,3 +67,18 @@ def test_fp32_outputs(rf, dev):
     poison(c, range(300))
     got = c.run()
     assert bool(got[:2].isnan().all()) and bool(got[2:].isfinite().all())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new,kv", [(1, 60), (3, 700), (40, 100), (33, 5000)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+def test_a_scale_of_zero(rf, dev, new, kv, d, value):
+    # 0 times an infinite product is NaN; 0 times a finite one is 0
+    c = case(new, kv, d, scale=0.0)
+    c.check()
+    poison(c, [kv // 2 - new // 2], value)
+    got = c.run()
+    pos = torch.arange(kv - new, kv, device=P.DEV)
+    sees = pos >= kv // 2 - new // 2
+    assert bool(sees.any()) and bool(got[:new][sees].isnan().all()) and bool(got[:new][~sees].isfinite().all())
+    assert bool(got[new:].isfinite().all())
