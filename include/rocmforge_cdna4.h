@@ -681,7 +681,8 @@ typedef struct rf_paged_cache {
  * when refused; free_out[0] = free pages left; for every row below max_rows
  * positions[r] = ctx + its index in the request and slots[r] = page *
  * page_size + position % page_size -- rows of refused requests and padding
- * rows get position 0 and slot -1.  ctx_out may be ctx_in and free_out may be
+ * rows get position 0 and slot -1, and slots that pass 32 bits (a table's entry
+ * that names no page) are -1 too.  ctx_out may be ctx_in and free_out may be
  * free_in; no other buffers may overlap.  free_pages holds num_pages entries;
  * a free_in outside [0, num_pages] is taken as the nearer end. */
 typedef struct rf_paged_plan {

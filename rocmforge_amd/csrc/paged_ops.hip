@@ -65,7 +65,10 @@ __device__ __forceinline__ void plan_row(const rf_paged_plan& p, const int* star
         if (kv > 0) {
             const int pos = kv - n + (r - starts[lo]), sh = __ffs(p.page_size) - 1;
             p.positions[r] = pos;
-            p.slots[r] = (p.block_tables[(int64_t)lo * p.max_blocks + (pos >> sh)] << sh) + (pos & (p.page_size - 1));
+            // (an entry that names no page may lie anywhere: in 32 bits its slot could be another page's)
+            const int64_t slot = (int64_t)p.block_tables[(int64_t)lo * p.max_blocks + (pos >> sh)] * p.page_size +
+                                 (pos & (p.page_size - 1));
+            p.slots[r] = slot == (int)slot ? (int)slot : -1;
             return;
         }
     }
