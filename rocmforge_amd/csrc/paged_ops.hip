@@ -301,7 +301,7 @@ constexpr uint32_t kSeen = 1, kBiased = 2, kMade = 4;
 
 template <bool VEC, int kSlice>
 __global__ __launch_bounds__(256) void rf_logits_rules_kernel(const rf_logits_rules l) {
-    __shared__ uint32_t count[kSlice];
+    __shared__ __align__(16) uint32_t count[kSlice];        // (cleared in 16 bytes)
     __shared__ int listed, list_at[64], list_id[64];
     __shared__ float list_val[64];
     constexpr int IDS = 8;                       // of the history in flight a thread
