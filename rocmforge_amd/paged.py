@@ -15,6 +15,12 @@ with release() for requests that ended.  The argument blocks are the C
 structs; pointer fields take device addresses, torch tensors of the GPU (kept
 alive by the block) or None.  Launches go to the given stream, else to torch's current
 one, and raise ops.HipApiError where the library refuses the arguments.
+
+Tensors are looked at before they are launched on, once after each change of a
+block: a ValueError where a type is not the field's (16-bit integers pass for fp16
+bits, the workspace is of any type), where elements do not lie as the field's
+strides say (rows one ld_.. apart and dense in themselves, all else contiguous).
+Addresses are taken as they are, and so are sizes.
 """
 from __future__ import annotations
 
@@ -28,7 +34,43 @@ ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN = 0, 1, 2
 _vp, _i32, _i64, _f, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 
 
+# What a pointer field takes: types of elements, and where these lie ("dense", "last": the last
+# dim is dense, or the field that holds the distance of rows).
+_I32 = (("int32",), "dense")
+_F32 = (("float32",), "dense")
+_HALF = ("float16", "int16", "uint16")
+
+
+def _dense(shape, strides) -> bool:
+    n = 1
+    for size, stride in zip(reversed(shape), reversed(strides)):
+        if size == 0:
+            return True
+        if size > 1 and stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _look(what: str, t, types, layout, ld=None) -> None:
+    kind = str(t.dtype).replace("torch.", "")
+    if types is not None and kind not in types:
+        raise ValueError(f"{what} is {kind}, not {' or '.join(types)}")
+    shape, strides = tuple(t.shape), tuple(t.stride())
+    if layout == "last":
+        ok = not shape or shape[-1] <= 1 or strides[-1] == 1
+    elif layout == "dense" or len(shape) < 2:
+        ok = _dense(shape, strides)
+    else:
+        ok = _dense(shape[1:], strides[1:]) and (shape[0] <= 1 or strides[0] == ld)
+    if not ok:
+        where = f"rows {ld} apart ({layout})" if ld is not None else "dense"
+        raise ValueError(f"{what} has strides {strides}, not {where}")
+
+
 class _Block(ctypes.Structure):
+    _tensors = {}
+
     def __init__(self, **fields):
         super().__init__()
         types = dict(self._fields_)
@@ -39,16 +81,37 @@ class _Block(ctypes.Structure):
             setattr(self, name, value)
 
     def __setattr__(self, name, value):
-        if hasattr(value, "data_ptr"):
-            self.__dict__.setdefault("_kept", {})[name] = value
-            value = _addr(value)
-        super().__setattr__(name, value)
+        tensor = hasattr(value, "data_ptr")
+        if tensor and name not in self._tensors:
+            raise ValueError(f"{type(self).__name__}.{name} is not a pointer")
+        super().__setattr__(name, _addr(value))
+        kept = self.__dict__.setdefault("_kept", {})
+        kept.pop(name, None)
+        if tensor:
+            kept[name] = value
+        self.__dict__.pop("_seen", None)
+
+    def _types(self, name):
+        return self._tensors[name][0]
+
+    def _look(self):
+        for name, t in self.__dict__.get("_kept", {}).items():
+            layout = self._tensors[name][1]
+            _look(f"{type(self).__name__}.{name}", t, self._types(name), layout, getattr(self, layout, None))
+        self.__dict__["_seen"] = True
 
 
 class PagedCache(_Block):
     """K and V pages of one layer (rf_paged_cache)."""
     _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _i64), ("row_stride", _i64), ("head_stride", _i64),
                 ("num_pages", _i32), ("page_size", _i32), ("num_kv_heads", _i32), ("head_dim", _i32)]
+    _tensors = {"k": (_HALF, "last"), "v": (_HALF, "last")}
+
+    def _look(self):
+        kept = self.__dict__.get("_kept", {})
+        if len(kept) == 2 and kept["k"].stride() != kept["v"].stride():
+            raise ValueError(f"PagedCache.v has strides {kept['v'].stride()}, k {kept['k'].stride()}")
+        super()._look()
 
 
 class PagedPlan(_Block):
@@ -56,6 +119,7 @@ class PagedPlan(_Block):
     _fields_ = [(n, _vp) for n in ("new_lens", "ctx_in", "ctx_out", "free_pages", "free_in", "free_out",
                                    "block_tables", "q_start", "kv_lens", "positions", "slots")] + \
                [(n, _i32) for n in ("num_seqs", "max_blocks", "page_size", "max_rows", "num_pages")]
+    _tensors = {n: _I32 for n, t in _fields_ if t is _vp} | {"block_tables": (("int32",), "max_blocks")}
 
 
 class PagedRope(_Block):
@@ -63,6 +127,9 @@ class PagedRope(_Block):
     _fields_ = [(n, _vp) for n in ("q", "k", "v", "q_norm", "k_norm", "q16", "positions", "slots", "turns")] + \
                [(n, _i64) for n in ("ld_q", "ld_k", "ld_v", "ld_q16")] + \
                [(n, _i32) for n in ("rows", "num_heads", "rot_dim", "neox")] + [("eps", _f), ("attn_factor", _f)]
+    _tensors = {n: (("float32",), f"ld_{n}") for n in "qkv"} | {
+        "q_norm": _F32, "k_norm": _F32, "q16": (_HALF, "ld_q16"), "positions": _I32, "slots": _I32,
+        "turns": (("float64",), "dense")}
 
 
 class PagedAttention(_Block):
@@ -71,6 +138,11 @@ class PagedAttention(_Block):
                [("workspace_bytes", _sz), ("ld_q", _i64), ("ld_out", _i64)] + \
                [(n, _i32) for n in ("num_seqs", "max_blocks", "rows", "num_heads", "max_new", "window", "out_f32")] + \
                [("scale", _f)]
+    _tensors = {"q": (_HALF, "ld_q"), "out": (None, "ld_out"), "block_tables": (("int32",), "max_blocks"),
+                "q_start": _I32, "kv_lens": _I32, "workspace": (None, "dense")}
+
+    def _types(self, name):
+        return ((("float32",) if self.out_f32 else _HALF) if name == "out" else super()._types(name))
 
 
 class LogitsRules(_Block):
@@ -79,6 +151,10 @@ class LogitsRules(_Block):
                 ("ld_history", _i64), ("prompt_lens", _vp), ("total_lens", _vp), ("repetition", _vp),
                 ("frequency", _vp), ("presence", _vp), ("bias_start", _vp), ("bias_ids", _vp), ("bias_values", _vp),
                 ("allowed", _vp), ("ld_allowed", _i64), ("rows", _i32), ("vocab", _i32)]
+    _tensors = {"logits": (("float32",), "ld_logits"), "out": (("float32",), "ld_out"),
+                "history": (("int32",), "ld_history"), "prompt_lens": _I32, "total_lens": _I32, "repetition": _F32,
+                "frequency": _F32, "presence": _F32, "bias_start": _I32, "bias_ids": _I32, "bias_values": _F32,
+                "allowed": (("int32", "uint32"), "ld_allowed")}
 
 
 def _addr(p):
@@ -96,32 +172,49 @@ def _stream(stream):
     return getattr(stream, "cuda_stream", stream)
 
 
+def _launch(name: str, stream, *blocks) -> None:
+    for b in blocks:
+        if "_seen" not in b.__dict__:
+            b._look()
+    _check(getattr(load(), name)(*[ctypes.byref(b) for b in blocks], _stream(stream)), name)
+
+
 def _check(rc: int, what: str) -> None:
     if rc != 0:
         raise HipApiError(rc, what)
 
 
+def _addrs(tensors):
+    """Addresses of (name, value, types, layout, rows' distance)."""
+    for name, value, types, layout, ld in tensors:
+        if hasattr(value, "data_ptr"):
+            _look(name, value, types, layout, ld)
+    return [_addr(t[1]) for t in tensors]
+
+
 def plan(step: PagedPlan, stream=None) -> None:
-    _check(load().rf_paged_plan_launch(ctypes.byref(step), _stream(stream)), "rf_paged_plan_launch")
+    _launch("rf_paged_plan_launch", stream, step)
 
 
 def release(ended, ctx_lens, block_tables, free_pages, free_count, num_seqs: int, max_blocks: int, page_size: int,
             num_pages: int, stream=None) -> None:
-    _check(load().rf_paged_release_launch(_addr(ended), _addr(ctx_lens), _addr(block_tables), _addr(free_pages),
-                                          _addr(free_count), num_seqs, max_blocks, page_size, num_pages,
-                                          _stream(stream)), "rf_paged_release_launch")
+    at = _addrs([("ended", ended, *_I32, None), ("ctx_lens", ctx_lens, *_I32, None),
+                 ("block_tables", block_tables, ("int32",), "max_blocks", max_blocks),
+                 ("free_pages", free_pages, *_I32, None), ("free_count", free_count, *_I32, None)])
+    _check(load().rf_paged_release_launch(*at, num_seqs, max_blocks, page_size, num_pages, _stream(stream)),
+           "rf_paged_release_launch")
 
 
 def rope_turns_table(turns, rot_dim: int, theta_base: float, mode: int = ROPE_PLAIN, factor: float = 1.0,
                      orig_positions: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0, freq_scale=None,
                      stream=None) -> None:
-    _check(load().rf_rope_turns_table(_addr(turns), rot_dim, theta_base, mode, factor, orig_positions, beta_fast,
-                                      beta_slow, _addr(freq_scale), _stream(stream)), "rf_rope_turns_table")
+    at = _addrs([("turns", turns, ("float64",), "dense", None), ("freq_scale", freq_scale, *_F32, None)])
+    _check(load().rf_rope_turns_table(at[0], rot_dim, theta_base, mode, factor, orig_positions, beta_fast, beta_slow,
+                                      at[1], _stream(stream)), "rf_rope_turns_table")
 
 
 def rope_write(step: PagedRope, cache: PagedCache, stream=None) -> None:
-    _check(load().rf_paged_rope_write_launch(ctypes.byref(step), ctypes.byref(cache), _stream(stream)),
-           "rf_paged_rope_write_launch")
+    _launch("rf_paged_rope_write_launch", stream, step, cache)
 
 
 def attention_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
@@ -129,9 +222,8 @@ def attention_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int) 
 
 
 def attention(step: PagedAttention, cache: PagedCache, stream=None) -> None:
-    _check(load().rf_paged_attention_launch(ctypes.byref(step), ctypes.byref(cache), _stream(stream)),
-           "rf_paged_attention_launch")
+    _launch("rf_paged_attention_launch", stream, step, cache)
 
 
 def logits_rules(rules: LogitsRules, stream=None) -> None:
-    _check(load().rf_logits_rules_launch(ctypes.byref(rules), _stream(stream)), "rf_logits_rules_launch")
+    _launch("rf_logits_rules_launch", stream, rules)
