@@ -19,8 +19,9 @@ one, and raise ops.HipApiError where the library refuses the arguments.
 Tensors are looked at before they are launched on, once after each change of a
 block: a ValueError where a type is not the field's (16-bit integers pass for fp16
 bits, the workspace is of any type), where elements do not lie as the field's
-strides say (rows one ld_.. apart and dense in themselves, all else contiguous).
-Addresses are taken as they are, and so are sizes.
+strides say (rows one ld_.. apart and dense in themselves, all else contiguous), or
+where a tensor or the stream is not of the current device.  Addresses are taken as
+they are, and so are sizes.
 """
 from __future__ import annotations
 
@@ -89,16 +90,19 @@ class _Block(ctypes.Structure):
         kept.pop(name, None)
         if tensor:
             kept[name] = value
-        self.__dict__.pop("_seen", None)
+        self.__dict__.pop("_on", None)
 
     def _types(self, name):
         return self._tensors[name][0]
 
-    def _look(self):
-        for name, t in self.__dict__.get("_kept", {}).items():
+    def _device(self):
+        """Index of the device of the block's tensors, None without any; they are looked at before."""
+        kept = self.__dict__.get("_kept", {})
+        for name, t in kept.items():
             layout = self._tensors[name][1]
             _look(f"{type(self).__name__}.{name}", t, self._types(name), layout, getattr(self, layout, None))
-        self.__dict__["_seen"] = True
+        on = self.__dict__["_on"] = _one_device([t.device.index for t in kept.values()])
+        return on
 
 
 class PagedCache(_Block):
@@ -107,11 +111,11 @@ class PagedCache(_Block):
                 ("num_pages", _i32), ("page_size", _i32), ("num_kv_heads", _i32), ("head_dim", _i32)]
     _tensors = {"k": (_HALF, "last"), "v": (_HALF, "last")}
 
-    def _look(self):
+    def _device(self):
         kept = self.__dict__.get("_kept", {})
         if len(kept) == 2 and kept["k"].stride() != kept["v"].stride():
             raise ValueError(f"PagedCache.v has strides {kept['v'].stride()}, k {kept['k'].stride()}")
-        super()._look()
+        return super()._device()
 
 
 class PagedPlan(_Block):
@@ -165,18 +169,39 @@ def _addr(p):
     return p.data_ptr()
 
 
-def _stream(stream):
+def _one_device(indexes):
+    on = sorted(set(i for i in indexes if i is not None))
+    if len(on) > 1:
+        raise ValueError("tensors of cuda:" + " and cuda:".join(map(str, on)) + " in one launch")
+    return on[0] if on else None
+
+
+def _stream(stream, on):
+    """The stream's handle.  on: the tensors' device, None where there are addresses only."""
+    import torch
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        stream = torch.cuda.current_stream()
+        current = stream.device_index
+    elif on is None and not hasattr(stream, "cuda_stream"):
+        return stream
+    else:
+        current = torch.cuda.current_device()
+        if getattr(stream, "device_index", current) != current:
+            raise ValueError(f"a stream of cuda:{stream.device_index}, the current device is cuda:{current}")
+    if on is not None and on != current:
+        raise ValueError(f"tensors of cuda:{on}, the current device is cuda:{current}")
     return getattr(stream, "cuda_stream", stream)
 
 
-def _launch(name: str, stream, *blocks) -> None:
-    for b in blocks:
-        if "_seen" not in b.__dict__:
-            b._look()
-    _check(getattr(load(), name)(*[ctypes.byref(b) for b in blocks], _stream(stream)), name)
+def _launch(name: str, stream, step, cache=None) -> None:
+    on = step.__dict__["_on"] if "_on" in step.__dict__ else step._device()
+    if cache is None:
+        _check(getattr(load(), name)(ctypes.byref(step), _stream(stream, on)), name)
+        return
+    cache_on = cache.__dict__["_on"] if "_on" in cache.__dict__ else cache._device()
+    if on != cache_on:
+        on = _one_device([on, cache_on])
+    _check(getattr(load(), name)(ctypes.byref(step), ctypes.byref(cache), _stream(stream, on)), name)
 
 
 def _check(rc: int, what: str) -> None:
@@ -184,12 +209,15 @@ def _check(rc: int, what: str) -> None:
         raise HipApiError(rc, what)
 
 
-def _addrs(tensors):
-    """Addresses of (name, value, types, layout, rows' distance)."""
+def _addrs(stream, tensors):
+    """Addresses of (name, value, types, layout, rows' distance), and the stream's handle."""
+    out, on = [], []
     for name, value, types, layout, ld in tensors:
+        out.append(_addr(value))
         if hasattr(value, "data_ptr"):
             _look(name, value, types, layout, ld)
-    return [_addr(t[1]) for t in tensors]
+            on.append(value.device.index)
+    return out, _stream(stream, _one_device(on))
 
 
 def plan(step: PagedPlan, stream=None) -> None:
@@ -198,19 +226,19 @@ def plan(step: PagedPlan, stream=None) -> None:
 
 def release(ended, ctx_lens, block_tables, free_pages, free_count, num_seqs: int, max_blocks: int, page_size: int,
             num_pages: int, stream=None) -> None:
-    at = _addrs([("ended", ended, *_I32, None), ("ctx_lens", ctx_lens, *_I32, None),
-                 ("block_tables", block_tables, ("int32",), "max_blocks", max_blocks),
-                 ("free_pages", free_pages, *_I32, None), ("free_count", free_count, *_I32, None)])
-    _check(load().rf_paged_release_launch(*at, num_seqs, max_blocks, page_size, num_pages, _stream(stream)),
+    at, handle = _addrs(stream, [("ended", ended, *_I32, None), ("ctx_lens", ctx_lens, *_I32, None),
+                                 ("block_tables", block_tables, ("int32",), "max_blocks", max_blocks),
+                                 ("free_pages", free_pages, *_I32, None), ("free_count", free_count, *_I32, None)])
+    _check(load().rf_paged_release_launch(*at, num_seqs, max_blocks, page_size, num_pages, handle),
            "rf_paged_release_launch")
 
 
 def rope_turns_table(turns, rot_dim: int, theta_base: float, mode: int = ROPE_PLAIN, factor: float = 1.0,
                      orig_positions: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0, freq_scale=None,
                      stream=None) -> None:
-    at = _addrs([("turns", turns, ("float64",), "dense", None), ("freq_scale", freq_scale, *_F32, None)])
+    at, handle = _addrs(stream, [("turns", turns, ("float64",), "dense", None), ("freq_scale", freq_scale, *_F32, None)])
     _check(load().rf_rope_turns_table(at[0], rot_dim, theta_base, mode, factor, orig_positions, beta_fast, beta_slow,
-                                      at[1], _stream(stream)), "rf_rope_turns_table")
+                                      at[1], handle), "rf_rope_turns_table")
 
 
 def rope_write(step: PagedRope, cache: PagedCache, stream=None) -> None:
