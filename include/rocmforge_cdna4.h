@@ -707,8 +707,10 @@ hipError_t rf_paged_plan_launch(const rf_paged_plan* plan, hipStream_t stream);
 
 /* Requests b with ended[b] != 0 give their ceil(ctx_lens[b] / page_size) pages
  * back, in order, onto the stack free_pages[0 .. free_count[0]), and their
- * ctx_lens[b] becomes 0.  All in place.  A request whose pages would take the
- * stack past num_pages entries keeps them (a page was handed back twice). */
+ * ctx_lens[b] becomes 0.  All in place.  Requests that hand nothing back and keep
+ * their length: one whose pages would take the stack past num_pages entries (a
+ * page was handed back twice) and those behind it, one whose ctx_lens[b] is negative, and
+ * one whose pages would be more than max_blocks. */
 hipError_t rf_paged_release_launch(const int32_t* ended, int32_t* ctx_lens, const int32_t* block_tables,
                                    int32_t* free_pages, int32_t* free_count, int num_seqs, int max_blocks,
                                    int page_size, int num_pages, hipStream_t stream);
@@ -821,7 +823,8 @@ hipError_t rf_paged_attention_launch(const rf_paged_attention* step, const rf_pa
  * history when none of the three penalties is given.  Tokens outside [0, vocab)
  * in history or bias are skipped; total_lens is clipped to [0, ld_history].
  * out may be logits itself (with ld_out = ld_logits), else they do not overlap.
- * rows <= 65535. */
+ * rows <= 65535.  Bias lists are meant to be short: beyond about 64 entries in 4096 tokens
+ * (1024 for few rows) the time grows with the square of their length. */
 typedef struct rf_logits_rules {
     const float* logits;
     float* out;

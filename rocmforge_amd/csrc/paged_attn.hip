@@ -52,16 +52,17 @@ constexpr float kLag = 8.0f;
 constexpr int kNarrowRows = 16, kNarrowKeys = 32;
 constexpr int kWideKeys = 64;
 // Least units of keys of a part (a workgroup costs about as much as 4 to 6 units
-// before and behind its loop; wide ones, and narrow ones beside them, more: 4 prompts of
-// 200 behind 2800 72 us at 16 wide units and 65 at 24, 64 tokens behind 15936 52 and 54),
-// and the most narrow parts that are aimed at.
+// before and behind its loop; wide ones, and narrow ones beside them, more), and the
+// most narrow parts that are aimed at.  us, wide parts of at least 4 / 8 / 16 / 24 units: 28 single tokens
+// beside 4 pieces of prompt 39.5 / 33.4 / 28.5 / 28.4; 64 tokens behind 15936 66.1 / 66.2 / 50.7 / 52.9;
+// 4 prompts of 200 behind 2800 64.4 / 64.9 / 64.9 / 64.9.
 constexpr int kNarrowLeast = 4, kBesideLeast = 16, kNarrowParts = 512;
 constexpr int kWideLeast = 24;
-// Where tables are no wider than these many units nothing is cut, and no join is launched: for
-// few narrow tiles (one request of 256 positions 8.4 -> 6.1 us, of 500 9.0 -> 8.6, of 1000 would
-// take 12.6 for 9.0), for 256 and more or beside wide ones (32 requests of 20 to 1000 17.4 -> 15.4,
-// 256 of 600 131 -> 125, 20 of 500 beside two prompts 32 -> 26.6), and for wide tiles (a prompt of
-// 1500 49 -> 41).
+// Where tables are no wider than these many units nothing is cut, and no join is launched.  us, cut ->
+// whole, in tables of just these widths: few narrow tiles (one request of 256 positions 8.2 -> 5.9, of
+// 500 8.8 -> 8.4, 8 of 500 9.7 -> 8.6), 256 tiles and more (32 requests of 20 to 1000 17.2 -> 15.3, 256 of 600
+// 132 -> 126), beside wide ones (20 of 500 beside two prompts 28.0 -> 26.2), and wide tiles: a prompt of 1500
+// 41.4 -> 41.0, but pieces behind a context lose by it (2 of 100 behind 1900 36.3 -> 46.0).
 constexpr int kFewWhole = 16, kManyWhole = 32, kWideWhole = 32;
 
 // ---- which part of which request a workgroup does ---------------------------------------
@@ -300,7 +301,7 @@ __device__ __forceinline__ V finite_of(V v) {
 // costs no bytes.  Bound by memory, and for short requests by the chain lengths ->
 // share -> page -> K -> V and the join's launch.  48 requests of 60 to 16000
 // positions (32 heads on 8, head_dim 128, 556 MB): 120 us with the join, 4.6 TB/s
-// where a large copy reaches 5.1; one request of 640: 8.8 us.
+// where a large copy reaches 5.1; one request of 640: 8.6 us.
 template <int D, int W, int S>
 __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const rf_paged_cache& c, const Plan& plan,
                                             int item, uint8_t* lds) {
@@ -530,12 +531,12 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
 // beside the weights of the one before (MFMA beside exp), so K runs a tile ahead.
 // M = 32 where a wave's queries and outputs fit its registers (head_dim 64 and
 // 128); at 256 they would take 192 of them, and M = 16 has two waves a SIMD: a
-// step of three windowed prompts 70 us, with 32 rows a wave, one wave a SIMD and
+// step of three windowed prompts 71 us, with 32 rows a wave, one wave a SIMD and
 // outputs in accumulation registers 79.
 // Bound at head_dim 128 by MFMA, softmax VALU and LDS reads, each about half of
 // the time busy and overlapping across two waves a SIMD: a fresh prompt of 8192
 // (32 heads on 8) 543 to 593 us, 930 to 1010 TFLOP/s where a large product reaches
-// 1160; 512 tokens behind 15700 155 to 164 us.  At 256 by LDS reads (4096 clocks
+// 1160; 512 tokens behind 15700 153 to 164 us.  At 256 by LDS reads (4096 clocks
 // a CU and tile beside 2048 of MFMA): 390 TFLOP/s.
 
 // The two MFMA shapes.  M packed rows a wave; acc: a block of scores or outputs, whose
@@ -924,7 +925,7 @@ constexpr int kJoinRows = 32, kJoinParts = 64;
 // Head dims, waves and stages of the narrow part, waves of the wide one.
 // W, S: heavy workgroups of the narrow launch, one a CU; LW, LS: light ones, two a CU, so
 // that one's chain of loads runs beside the other's loop, for many tiles and beside wide
-// items (256 requests of 600 positions 157 -> 132 us; one of 2000 9.1 -> 9.6).
+// items (256 requests of 600 positions 148 -> 126 us; one of 2000 9.0 -> 9.5).
 template <int D> struct Shape;
 template <> struct Shape<64> { static constexpr int W = 4, S = 4, LW = 4, LS = 2, NW = 4, M = 32, PER_CU = 2; };
 template <> struct Shape<128> { static constexpr int W = 4, S = 2, LW = 2, LS = 2, NW = 4, M = 32, PER_CU = 2; };
@@ -1073,12 +1074,26 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
     const int64_t some = std::min<int64_t>(a.num_seqs, a.rows);        // requests with rows
     // The narrow launch.  Fewer than 64 tiles, or up to 256 of short tables: 256 parts, one round of
     // workgroups with most loads in flight.  Else up to 256: two workgroups a CU, and half a part less for
-    // every tile, since the last part of a tile is half a one on average -- one round again.  Up to 511: two rounds, which even out a
-    // ragged batch.  From 512 tiles on light workgroups again.  us, 256 parts of heavy ones / 512 of
-    // heavy ones / 512 - tiles / 2 of light ones: 2 requests of 8000 (8 KV heads) 19.4 / 24.5 / 20.4;
-    // 8 of 2000 19.2 / 22.8 / 20.3; 8 of 100 to 8000 27.7 / 25.9 / 21.8; 20 of 4000 77.8 / 72.2 / 60.9;
-    // 32 of 100 to 8000 66.5 / 60.6 / 58.9; 48 of 60 to 16000 168 / 146 / 149; 64 of them 241 / 208 / 236;
-    // 32 of 1000 in a table as wide 26.3 / 30.9 / 28.3.
+    // every tile, since the last part of a tile is half a one on average -- one round again.  Up to 511: two rounds
+    // of heavy workgroups.  From 512 tiles on 512 parts of light ones.  us (graph, 8 KV heads of 128 unless
+    // said), 256 parts of heavy ones / 512 of heavy ones / 512 of light ones / 512 - tiles / 2 of light ones:
+    //   up to 63 tiles        2 requests of 8000         19.1 / 24.0 / 20.0 / 20.1
+    //   64 to 256             8 of 100 to 8000           20.1 / 18.8 / 15.9 / 15.9
+    //                         20 of 4000                 76.5 / 71.1 / 75.3 / 59.8
+    //                         32 of 100 to 8000          82.5 / 75.5 / 83.3 / 69.7
+    //     in a short table    8 of 2000                  18.8 / 22.2 / 18.5 / 19.7
+    //                         32 of 1000                 25.8 / 30.9 / 27.6 / 27.6
+    //   257 to 511            48 of 60 to 16000           134 /  125 /  140 /  128
+    //                         the same, heads of 64      86.7 / 77.5 / 67.8 / 64.8
+    //                         the same, heads of 256      249 /  206 /  233 /  225
+    //   from 512 on           256 of 600                  149 /  149 /  126 /  126
+    //                         64 of 2000                 98.0 / 98.5 / 96.0 / 95.7
+    //                         300 of 20 to 4000           203 /  208 /  201 /  196
+    //                         128 of 20 to 8000           168 /  149 /  160 /  201
+    //                         the same, heads of 64       137 /  124 /  102 /  133
+    //                         the same, heads of 256      379 /  322 /  352 /  522
+    // So from 257 tiles on no choice wins throughout: very ragged batches of 512 tiles and more would run up to 9 %
+    // faster with heavy workgroups, even ones 18 % slower, and heads of 64 in the band before with light ones.
     const int64_t tiles = some * nkv;
     const bool few = !both && (tiles < 64 || (tiles <= 256 && positions <= 2048)), some_tiles = !both && !few && tiles <= 256;
     const bool light = both || some_tiles || tiles >= 512;
@@ -1087,8 +1102,8 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
     const int narrow_least = least(kNarrowKeys, both || tiles >= 256 ? kManyWhole : kFewWhole,
                                    both ? kBesideLeast : kNarrowLeast);
     Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, aim, narrow_least, inverse(aim), 0, ws};
-    // (fewer parts for many wide tiles likewise: 100 single tokens beside 4 prompts of 300 152 -> 132, and
-    // to half a part less for each, 512 tokens behind 8000 three times 229 -> 240)
+    // (fewer parts for many wide tiles likewise, a quarter of one a tile.  us, none less / a quarter / half of one:
+    // 100 single tokens beside 4 prompts of 300 159 / 144 / 137, 512 tokens behind 8000 three times 223 / 224 / 235)
     const int64_t wide_tiles = (packed / ROWS + std::min(some, packed / kNarrowRows)) * nkv;
     const int wide_aim = (int)std::max<int64_t>(wide_parts<D>() - wide_tiles / 4, wide_parts<D>() / 4);
     Plan wide = {group, inv, kNarrowRows, INT_MAX, wide_aim, least(kWideKeys, kWideWhole, kWideLeast), inverse(wide_aim), 0,
