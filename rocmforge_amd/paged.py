@@ -112,9 +112,10 @@ class PagedCache(_Block):
     _tensors = {"k": (_HALF, "last"), "v": (_HALF, "last")}
 
     def _device(self):
-        kept = self.__dict__.get("_kept", {})
-        if len(kept) == 2 and kept["k"].stride() != kept["v"].stride():
-            raise ValueError(f"PagedCache.v has strides {kept['v'].stride()}, k {kept['k'].stride()}")
+        k, v = [self.__dict__.get("_kept", {}).get(n) for n in "kv"]
+        if k is not None and v is not None and len(k.shape) == len(v.shape) and any(
+                m > 1 and n > 1 and a != b for m, n, a, b in zip(k.shape, v.shape, k.stride(), v.stride())):
+            raise ValueError(f"PagedCache.v has strides {v.stride()}, k {k.stride()}")
         return super()._device()
 
 

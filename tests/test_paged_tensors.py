@@ -188,6 +188,9 @@ def test_pages_in_either_order(rf):
         paged.attention(attn(rows=-1), ok, stream=0)
     with pytest.raises(ValueError, match="v"):
         paged.attention(attn(), cache(v=by_head), stream=0)
+    one_page = OnGpu(torch.zeros(9, 16, 2, 128, dtype=torch.float16)[::9])
+    with pytest.raises(HipApiError):
+        paged.attention(attn(rows=-1), cache(k=f16(1, 16, 2, 128), v=one_page, num_pages=1), stream=0)
     dims_apart = OnGpu(torch.zeros(4, 16, 128, 2, dtype=torch.float16).transpose(2, 3))
     with pytest.raises(ValueError):
         paged.attention(attn(), cache(k=dims_apart, v=dims_apart), stream=0)
