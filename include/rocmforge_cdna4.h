@@ -641,6 +641,11 @@ hipError_t rf_gemv_qkv_q4_k_q6_k_v_rmsnorm_launch(const void* w_q, const void* w
  *   rf_logits_rules_launch     before a token is picked
  *   rf_paged_release_launch    the pages of ended requests back to the free ones
  *
+ * A layer whose pages hold 8 bits a value (rf_paged_cache8) takes
+ * rf_paged_rope_write8_launch and rf_paged_attention8_launch in their places;
+ * rf_paged_read8_launch takes requests out of such pages, and rf_lora_add_launch
+ * adds the requests' low-rank adapters to a projection.
+ *
  * Arguments come as a struct (a caller keeps one per layer and step shape);
  * it is read during the call only.  Lengths, positions and tables are device
  * memory, so captured steps replay with the values they then hold.  The
@@ -809,6 +814,107 @@ typedef struct rf_paged_attention {
 } rf_paged_attention;
 size_t rf_paged_attention_workspace_bytes(int num_heads, int num_kv_heads, int head_dim);
 hipError_t rf_paged_attention_launch(const rf_paged_attention* step, const rf_paged_cache* cache, hipStream_t stream);
+
+/* K and V pages of one layer in 8 bits: k[page * page_stride + (t % page_size) *
+ * row_stride + h * head_stride + i] is an e4m3 code (sign, 4 bits of exponent of bias
+ * 7, 3 of mantissa; 0x7f and 0xff NaN, no infinities), strides in bytes.  A block of
+ * B = min(page_size, 16) positions of a page shares an exponent a KV head:
+ * k_scale[(page * (page_size / B) + (t % page_size) / B) * num_kv_heads + h] = e + 127, and
+ * code c stands for c 2^e; v alike.  e is in [-15, 7], so that each such value is one of
+ * fp16's; bytes outside 112 .. 134 are taken as the nearer end.  Strides > 0 and
+ * multiples of 16, row_stride <= 2^27; k and v 16-byte aligned; the rest as for
+ * rf_paged_cache. */
+typedef struct rf_paged_cache8 {
+    uint8_t* k;
+    uint8_t* v;
+    uint8_t* k_scale;
+    uint8_t* v_scale;
+    int64_t page_stride;
+    int64_t row_stride;
+    int64_t head_stride;
+    int32_t num_pages;
+    int32_t page_size;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+} rf_paged_cache8;
+
+/* rf_paged_rope_write_launch into 8-bit pages: q16 alike, k and v (fp32, not rounded
+ * before) as codes.  For each block and head that rows of the call lie in, with amax the
+ * largest magnitude among these rows' finite values and e' the smallest exponent in
+ * [-15, 7] with amax <= 448 2^e' (7 where there is none):
+ *   the block's first position is among the rows:  e = e'
+ *   else:                                          e = max(e', e as it was)
+ * Values become the nearest code of value 2^-e (ties to even; beyond 448 +-448,
+ * infinities and NaN NaN).  Where e has grown, the block's positions in front of the
+ * first of these rows become the nearest code of what they stood for; those behind the
+ * rows stay as they are, to be written before they are read.  The slots of one call are distinct,
+ * and rows of one block stand one behind the other with rising slots (as a plan's do). */
+hipError_t rf_paged_rope_write8_launch(const rf_paged_rope* step, const rf_paged_cache8* cache, hipStream_t stream);
+
+/* What requests hold in 8-bit pages, as fp16 bits (exact): row r in [row_start[b],
+ * row_start[b + 1]) is position first[b] + r - row_start[b] of request b (first null: 0):
+ * k[r * ld_out + h * head_dim + i], v alike (either may be null to skip).  Skipped, and
+ * their rows left as they were: positions < 0 or >= max_blocks * page_size, those whose
+ * table entry names no page, and rows past row_start[num_seqs].  row_start does not fall, its
+ * entries are clipped to [0, rows]; k and v 16-byte aligned, ld_out >= num_kv_heads *
+ * head_dim, a multiple of 8; rows <= 2^27; outputs overlap nothing. */
+typedef struct rf_paged_read {
+    uint16_t* k;
+    uint16_t* v;
+    const int32_t* block_tables;
+    const int32_t* row_start;
+    const int32_t* first;
+    int64_t ld_out;
+    int32_t num_seqs;
+    int32_t max_blocks;
+    int32_t rows;
+} rf_paged_read;
+hipError_t rf_paged_read8_launch(const rf_paged_read* read, const rf_paged_cache8* cache, hipStream_t stream);
+
+/* rf_paged_attention_launch over 8-bit pages: keys and values are what the codes stand
+ * for, and everything else is as there, the workspace's size too. */
+hipError_t rf_paged_attention8_launch(const rf_paged_attention* step, const rf_paged_cache8* cache, hipStream_t stream);
+
+/* Low-rank adapters beside a projection, each request with its own: for the rows r of
+ * request b (q_start as for the attention) with adapter i = adapters[b], and each target
+ *   y[r * ld_y + n] = base[r * ld_base + n] + scales[i] sum_j b_i[n, j] sum_k a_i[j, k] x[r * ld_x + k]
+ * over j < ranks[i]; i outside [0, num_adapters): y = base.  Targets share x, the adapters
+ * and their ranks (q, k and v; gate and up).  a_i[j, k] = a[i * a_stride + j * in_dim + k]
+ * (j < max_rank) and b_i[n, j] = b[i * b_stride + n * max_rank + j] are fp16 bits; parts of
+ * them behind an adapter's rank are not used, whatever they hold.  ranks are clipped to [0, max_rank].
+ * x is fp32, or fp16 bits (x_f16 != 0): fp32 values are taken as two of fp16's (22 bits; beyond
+ * 65504 NaN or infinite sums), the inner sums as two of fp16's against the row's largest, products
+ * are added in fp32.  y may be base itself (with ld_y = ld_base), else they do not overlap;
+ * rows past q_start[num_seqs] are left as they were, q_start does not fall.
+ * in_dim a multiple of 8, max_rank of 8 and at most 128, out_dim, ld_base and ld_y of 4, ld_x (in
+ * elements) of 8 (fp16) or 4, a_stride and b_stride of 8; pointers to x, a, b, base and y 16-byte
+ * aligned; in_dim, out_dim <= 2^20; rows <= 2^23; num_targets 1 to 3.  targets is read during the call only. */
+typedef struct rf_lora {
+    const void* x;
+    const int32_t* adapters;
+    const int32_t* q_start;
+    const int32_t* ranks;
+    const float* scales;
+    int64_t ld_x;
+    int32_t rows;
+    int32_t num_seqs;
+    int32_t num_adapters;
+    int32_t max_rank;
+    int32_t in_dim;
+    int32_t x_f16;
+} rf_lora;
+typedef struct rf_lora_target {
+    const uint16_t* a;
+    const uint16_t* b;
+    const float* base;
+    float* y;
+    int64_t a_stride;
+    int64_t b_stride;
+    int64_t ld_base;
+    int64_t ld_y;
+    int32_t out_dim;
+} rf_lora_target;
+hipError_t rf_lora_add_launch(const rf_lora* step, const rf_lora_target* targets, int num_targets, hipStream_t stream);
 
 /* Rules on the logits of each row before a token is picked.  With the row's
  * history history[r * ld_history + i], i < total_lens[r], of which the first

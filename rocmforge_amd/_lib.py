@@ -104,6 +104,10 @@ SIGNATURES = {
     "rf_rope_turns_table": [_vp, _i, _d, _i, _d, _d, _d, _d, _vp, _vp],
     "rf_paged_rope_write_launch": [_vp, _vp, _vp],
     "rf_paged_attention_launch": [_vp, _vp, _vp],
+    "rf_paged_rope_write8_launch": [_vp, _vp, _vp],
+    "rf_paged_read8_launch": [_vp, _vp, _vp],
+    "rf_paged_attention8_launch": [_vp, _vp, _vp],
+    "rf_lora_add_launch": [_vp, _vp, _i, _vp],
     "rf_logits_rules_launch": [_vp, _vp],
     "rf_q8_0_quantize_launch": [_vp, _vp, _vp, _vp, _i, _vp],
     "rf_q4_k_q8_int_dots_launch": [_vp, _vp, _vp, _i, _i, _vp],

@@ -19,7 +19,7 @@ BUILD = PKG / "_build"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 SOURCES = ["runtime.hip", "gemv_q4k.hip", "gemv_q6k.hip", "gemm_qk.hip", "model_ops.hip", "paged_ops.hip",
-           "paged_attn.hip", "mfma_peak.hip", "dispatch.cpp"]
+           "paged_attn.hip", "paged8_ops.hip", "paged8_attn.hip", "lora.hip", "mfma_peak.hip", "dispatch.cpp"]
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -27,11 +27,12 @@ FLAGS = [
 ]
 
 
-# Per-source extras.  model_ops.hip, paged_attn.hip: the prefill attention (the
+# Per-source extras.  model_ops.hip, paged_attn.hip, paged8_attn.hip: the prefill attention (the
 # only MFMA kernels there) rescales and reads its accumulators with VALU every key tile; with
 # them in AGPRs each tile paid ~350 accvgpr moves, in VGPRs none.
 EXTRA = {"model_ops.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-         "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+         "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "paged8_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _run(cmd: list[str]) -> None:

@@ -11,7 +11,9 @@ blocks on its buffers, and runs a step of a batch as
         attention(a, cache)       the new rows over their requests' pages
     logits_rules(l)               before a token is picked
 
-with release() for requests that ended.  The argument blocks are the C
+with release() for requests that ended.  Layers whose pages hold 8 bits a value
+have a PagedCache8 and call rope_write8 and attention8; read8 takes requests out of
+such pages.  (lora.py: the requests' adapters beside the layers' projections.)  The argument blocks are the C
 structs; pointer fields take device addresses, torch tensors of the GPU (kept
 alive by the block) or None.  Launches go to the given stream, else to torch's current
 one, and raise ops.HipApiError where the library refuses the arguments.
@@ -40,6 +42,8 @@ _vp, _i32, _i64, _f, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctyp
 _I32 = (("int32",), "dense")
 _F32 = (("float32",), "dense")
 _HALF = ("float16", "int16", "uint16")
+_CODES = ("float8_e4m3fn", "uint8", "int8")
+_EXPONENTS = ("uint8", "float8_e8m0fnu")
 
 
 def _dense(shape, strides) -> bool:
@@ -105,18 +109,31 @@ class _Block(ctypes.Structure):
         return on
 
 
-class PagedCache(_Block):
-    """K and V pages of one layer (rf_paged_cache)."""
-    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _i64), ("row_stride", _i64), ("head_stride", _i64),
-                ("num_pages", _i32), ("page_size", _i32), ("num_kv_heads", _i32), ("head_dim", _i32)]
-    _tensors = {"k": (_HALF, "last"), "v": (_HALF, "last")}
-
+class _Pages(_Block):
     def _device(self):
         k, v = [self.__dict__.get("_kept", {}).get(n) for n in "kv"]
         if k is not None and v is not None and len(k.shape) == len(v.shape) and any(
                 m > 1 and n > 1 and a != b for m, n, a, b in zip(k.shape, v.shape, k.stride(), v.stride())):
-            raise ValueError(f"PagedCache.v has strides {v.stride()}, k {k.stride()}")
+            raise ValueError(f"{type(self).__name__}.v has strides {v.stride()}, k {k.stride()}")
         return super()._device()
+
+
+_PAGES = [("page_stride", _i64), ("row_stride", _i64), ("head_stride", _i64), ("num_pages", _i32), ("page_size", _i32),
+          ("num_kv_heads", _i32), ("head_dim", _i32)]
+
+
+class PagedCache(_Pages):
+    """K and V pages of one layer (rf_paged_cache)."""
+    _fields_ = [("k", _vp), ("v", _vp)] + _PAGES
+    _tensors = {"k": (_HALF, "last"), "v": (_HALF, "last")}
+
+
+class PagedCache8(_Pages):
+    """K and V pages of one layer in 8 bits (rf_paged_cache8): e4m3 codes, strides in bytes, and
+    exponents [num_pages][page_size / min(page_size, 16)][num_kv_heads], + 127."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)] + _PAGES
+    _tensors = {"k": (_CODES, "last"), "v": (_CODES, "last"), "k_scale": (_EXPONENTS, "dense"),
+                "v_scale": (_EXPONENTS, "dense")}
 
 
 class PagedPlan(_Block):
@@ -148,6 +165,14 @@ class PagedAttention(_Block):
 
     def _types(self, name):
         return ((("float32",) if self.out_f32 else _HALF) if name == "out" else super()._types(name))
+
+
+class PagedRead(_Block):
+    """What requests hold in 8-bit pages, as fp16 (rf_paged_read)."""
+    _fields_ = [(n, _vp) for n in ("k", "v", "block_tables", "row_start", "first")] + [("ld_out", _i64)] + \
+               [(n, _i32) for n in ("num_seqs", "max_blocks", "rows")]
+    _tensors = {"k": (_HALF, "ld_out"), "v": (_HALF, "ld_out"), "block_tables": (("int32",), "max_blocks"),
+                "row_start": _I32, "first": _I32}
 
 
 class LogitsRules(_Block):
@@ -205,6 +230,13 @@ def _launch(name: str, stream, step, cache=None) -> None:
     _check(getattr(load(), name)(ctypes.byref(step), ctypes.byref(cache), _stream(stream, on)), name)
 
 
+def _pages(cache, kind):
+    """The cache, which is one of the kind that the launch reads."""
+    if not isinstance(cache, kind):
+        raise TypeError(f"a {type(cache).__name__}, not a {kind.__name__}")
+    return cache
+
+
 def _check(rc: int, what: str) -> None:
     if rc != 0:
         raise HipApiError(rc, what)
@@ -243,7 +275,15 @@ def rope_turns_table(turns, rot_dim: int, theta_base: float, mode: int = ROPE_PL
 
 
 def rope_write(step: PagedRope, cache: PagedCache, stream=None) -> None:
-    _launch("rf_paged_rope_write_launch", stream, step, cache)
+    _launch("rf_paged_rope_write_launch", stream, step, _pages(cache, PagedCache))
+
+
+def rope_write8(step: PagedRope, cache: PagedCache8, stream=None) -> None:
+    _launch("rf_paged_rope_write8_launch", stream, step, _pages(cache, PagedCache8))
+
+
+def read8(read: PagedRead, cache: PagedCache8, stream=None) -> None:
+    _launch("rf_paged_read8_launch", stream, read, _pages(cache, PagedCache8))
 
 
 def attention_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
@@ -251,7 +291,11 @@ def attention_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int) 
 
 
 def attention(step: PagedAttention, cache: PagedCache, stream=None) -> None:
-    _launch("rf_paged_attention_launch", stream, step, cache)
+    _launch("rf_paged_attention_launch", stream, step, _pages(cache, PagedCache))
+
+
+def attention8(step: PagedAttention, cache: PagedCache8, stream=None) -> None:
+    _launch("rf_paged_attention8_launch", stream, step, _pages(cache, PagedCache8))
 
 
 def logits_rules(rules: LogitsRules, stream=None) -> None:

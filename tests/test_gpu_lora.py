@@ -1,0 +1,226 @@
+"""Low-rank adapters of many requests (rf_lora_add_launch) against float64: ranks, widths,
+batches from single tokens to prompts, several targets, padding, and what must not enter."""
+import math
+
+import pytest
+import torch
+
+from rocmforge_amd import lora
+
+from . import paged_util as P
+
+pytestmark = pytest.mark.gpu
+
+
+class Case:
+    def __init__(self, new, of, ranks, max_rank=16, k=256, widths=(192,), x16=False, pad=0, wide=0, inplace=False, seed=0,
+                 size=1.0):
+        g = P.gen(seed + 13 * sum(new) + k + max_rank)
+        r = lambda *s: torch.randn(*s, generator=g, device=P.DEV)
+        rows, n = sum(new) + pad, len(ranks)
+        x = size * r(rows, k + wide)
+        self.x = (x.half() if x16 else x)[:, :k]
+        self.new, self.of, self.ranks, self.scales = new, of, ranks, [0.5 + 0.25 * i for i in range(n)]
+        starts = [0]
+        for m in new:
+            starts.append(starts[-1] + m)
+        self.a, self.b, self.base, self.y, self.t = [], [], [], [], []
+        for w in widths:
+            a, b = (r(n, max_rank, k) / math.sqrt(k)).half(), r(n, w, max_rank).half()
+            for i, q in enumerate(ranks):                    # behind an adapter's rank: NaN
+                a[i, max(min(q, max_rank), 0):] = math.nan
+                b[i, :, max(min(q, max_rank), 0):] = math.nan
+            base = r(rows, w + wide)
+            y = base.clone() if inplace else torch.full((rows, w + wide), 7.0, device=P.DEV)
+            self.a.append(a)
+            self.b.append(b)
+            self.base.append(base)
+            self.y.append(y)
+            self.t.append(lora.LoraTarget(a=a, b=b, base=y if inplace else base, y=y, a_stride=max_rank * k,
+                                          b_stride=w * max_rank, ld_base=w + wide, ld_y=w + wide, out_dim=w))
+        self.inplace, self.widths = inplace, widths
+        self.q_start, self.of_t = P.ints(starts), P.ints(of)
+        self.step = lora.LoraStep(x=self.x, adapters=self.of_t, q_start=self.q_start, ranks=P.ints(ranks),
+                                  scales=torch.tensor(self.scales, device=P.DEV), ld_x=k + wide, rows=rows,
+                                  num_seqs=len(new), num_adapters=n, max_rank=max_rank, in_dim=k, x_f16=int(x16))
+
+    def run(self):
+        print(f"[gpu] lora rows {self.new[:6]} of {self.of[:6]} ranks {self.ranks[:6]} x {tuple(self.x.shape)} {self.widths}",
+              flush=True)
+        lora.add(self.step, self.t)
+        torch.cuda.synchronize()
+
+    def want(self, j):
+        """(value, bound), float64."""
+        w, k = self.widths[j], self.x.shape[1]
+        y = (self.base[j] if self.inplace else torch.full_like(self.y[j], 7.0)).double()
+        bound = torch.zeros_like(y)
+        at = 0
+        for m, i in zip(self.new, self.of):
+            rows = slice(at, at + m)
+            y[rows, :w] = self.base[j][rows, :w].double()
+            q = min(max(self.ranks[i], 0), self.a[j].shape[1]) if 0 <= i < len(self.ranks) else 0
+            if q > 0:
+                a, b, x = self.a[j][i, :q].double(), self.b[j][i, :, :q].double(), self.x[rows].double()
+                h, ha = x @ a.t().contiguous(), x.abs() @ a.abs().t().contiguous()
+                y[rows, :w] += self.scales[i] * (h @ b.t().contiguous())
+                # x in 22 bits or whole (2^-22), fp32 sums of k products in any order (at most k + 4 roundings of the
+                # sums' size, in the mean far fewer: sqrt(k) + 8), A x in 22 bits of its row's largest, sums over the ranks
+                # alike, and three roundings of the result
+                e = 2.0 ** -22 + (math.sqrt(k) + 8) * 2.0 ** -24
+                top = h.abs().amax(1, keepdim=True) * 2.0 ** -22
+                off = (e * ha + top) @ b.abs().t().contiguous()
+                off += (math.sqrt(q) + 8) * 2.0 ** -24 * (h.abs() @ b.abs().t().contiguous())
+                bound[rows, :w] = abs(self.scales[i]) * off + 3 * 2.0 ** -24 * (y[rows, :w].abs() + self.base[j][rows, :w].double().abs())
+            at += m
+        return y, bound
+
+    def check(self):
+        self.run()
+        for j in range(len(self.widths)):
+            want, bound = self.want(j)
+            off = (self.y[j].double() - want).abs()
+            assert bool((off <= bound).all()), (j, (off / bound).nan_to_num(0.0).max().item())
+
+
+@pytest.mark.parametrize("max_rank", [8, 16, 24, 32, 40, 64, 72, 128])
+@pytest.mark.parametrize("x16", [False, True])
+@pytest.mark.parametrize("new", [[1], [1, 1, 1], [5, 40], [100]])
+def test_ranks(rf, dev, new, max_rank, x16):
+    of = list(range(len(new)))
+    Case(new, of, [max_rank, max_rank - 1, 1][:max(len(new), 1)], max_rank, x16=x16).check()
+
+
+@pytest.mark.parametrize("k", [8, 16, 24, 32, 40, 120, 128, 136, 264, 1000, 4096, 12288])
+@pytest.mark.parametrize("x16", [False, True])
+@pytest.mark.parametrize("new", [[1, 1], [1, 33]])
+def test_widths_of_x(rf, dev, new, k, x16):
+    Case(new, [1, 0], [16, 9], k=k, x16=x16).check()
+
+
+@pytest.mark.parametrize("w", [4, 8, 12, 16, 20, 60, 64, 68, 1024, 4100, 12288])
+@pytest.mark.parametrize("new", [[1, 1], [1, 33], [300]])
+def test_widths_of_y(rf, dev, new, w):
+    Case(new, [1, 0][:len(new)], [16, 9], widths=(w,)).check()
+
+
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 47, 64, 65, 127, 128, 129, 500, 2000])
+@pytest.mark.parametrize("x16", [False, True])
+def test_rows(rf, dev, n, x16):
+    Case([n, 1, n], [0, 1, 1], [16, 32], 32, x16=x16, pad=5).check()
+
+
+@pytest.mark.parametrize("widths", [(256, 64), (512, 128, 128), (4, 4096, 64)])
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [30, 1, 200, 4]])
+def test_targets_strides_and_place(rf, dev, widths, inplace, new):
+    Case(new, [2, -1, 0, 1], [8, 16, 3], widths=widths, inplace=inplace, wide=8, pad=7).check()
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("x16", [False, True])
+def test_requests_without_an_adapter(rf, dev, inplace, x16):
+    # none, numbers of no adapter, adapters of no rank (or less), requests without rows, more than the rank there is
+    Case([1, 0, 20, 3, 1, 0, 17, 2, 2], [-1, 0, 5, 1 << 30, -(1 << 31), 1, 1, 2, 3], [8, 0, -4, 1000], inplace=inplace,
+         x16=x16, pad=2).check()
+
+
+def test_no_adapters(rf, dev):
+    c = Case([3, 20], [0, 1], [8, 8], pad=3)
+    c.step.num_adapters, c.step.ranks, c.step.scales = 0, None, None
+    c.t[0].a = c.t[0].b = None
+    c.run()
+    assert torch.equal(c.y[0][:23], c.base[0][:23]) and bool((c.y[0][23:] == 7.0).all())
+
+
+@pytest.mark.parametrize("seqs", [63, 64, 65, 200, 1000])
+def test_many_requests(rf, dev, seqs):
+    Case([1 + (i % 9 == 0) * (i % 37) for i in range(seqs)], [(7 * i) % 11 - 1 for i in range(seqs)],
+         [1 + i for i in range(10)]).check()
+    Case([1] * seqs, [(5 * i) % 10 for i in range(seqs)], [16 - i for i in range(10)], x16=True).check()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 3e-3, 100.0, 10000.0])
+@pytest.mark.parametrize("new", [[2, 1], [40]])
+def test_sizes_of_x(rf, dev, size, new):
+    # (fp16's range ends at 65504, and hi + 2^-11 lo has 2^-36 for its smallest step)
+    c = Case(new, [0, 1], [16, 5], size=size)
+    c.run()
+    want, bound = c.want(0)
+    a, b = c.a[0].double().nan_to_num(0.0), c.b[0].double().nan_to_num(0.0)
+    tiny = 2.0 ** -37 * a.abs().sum((1, 2)).max() * b.abs().max() * max(c.scales)
+    assert bool(((c.y[0].double() - want).abs() <= bound + tiny).all())
+
+
+def test_rows_do_not_meet(rf, dev):
+    # NaN and infinities in a row stay in it
+    for x16 in (False, True):
+        c = Case([20, 3], [0, 1], [16, 16], x16=x16)
+        c.run()
+        want = c.y[0].clone()
+        c.x[4, 100], c.x[7, 3], c.x[21, 0] = math.nan, math.inf, math.nan
+        c.run()
+        for r in range(23):
+            if r in (4, 7, 21):
+                assert bool((~c.y[0][r].isfinite()).all())
+            else:
+                assert torch.equal(c.y[0][r], want[r])
+
+
+def test_row_ranges_are_clipped(rf, dev):
+    c = Case([30, 40], [0, 1], [16, 16])
+    c.run()
+    want = c.y[0].clone()
+    c.y[0].fill_(7.0)
+    c.step.rows = 50
+    c.run()
+    assert torch.equal(c.y[0][:50], want[:50]) and bool((c.y[0][50:] == 7.0).all())
+
+
+def test_every_run_gives_the_same_bits(rf, dev):
+    c = Case([1, 100, 1], [0, 1, 0], [64, 33], 64, k=4096, widths=(4096,))
+    c.run()
+    want = c.y[0].clone()
+    for _ in range(3):
+        c.y[0].fill_(7.0)
+        c.run()
+        assert torch.equal(c.y[0], want)
+
+
+def test_far_into_many_adapters(rf, dev):
+    # element offsets beyond 32 bits
+    k, w, rank = 4096, 256, 128
+    n = 5 * (1 << 30) // (rank * k)
+    a = torch.empty(n, rank, k, dtype=torch.float16, device=P.DEV)
+    b = torch.empty(n, w, rank, dtype=torch.float16, device=P.DEV)
+    c = Case([1, 30], [0, 1], [128, 100], rank, k=k, widths=(w,))
+    c.run()
+    want = c.y[0].clone()
+    a[n - 2:], b[n - 2:] = c.a[0], c.b[0]
+    c.t[0].a, c.t[0].b = a, b
+    full = lambda v, t: torch.cat([torch.zeros(n - 2, dtype=t, device=P.DEV), torch.tensor(v, dtype=t, device=P.DEV)])
+    c.step.ranks, c.step.scales, c.step.num_adapters = full([128, 100], torch.int32), full(c.scales, torch.float32), n
+    c.of_t += n - 2
+    c.run()
+    assert torch.equal(c.y[0], want)
+
+
+@pytest.mark.parametrize("new", [[1] * 6, [1, 70, 1, 0, 200, 3]])
+def test_replays(rf, dev, new):
+    c = Case(new, [0, 1, 2, 0, 1, 2], [8, 16, 5], widths=(128, 64), pad=4)
+    c.run()
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        lora.add(c.step, c.t)
+    for i in range(3):
+        c.of = [(j * (i + 2)) % 4 - 1 for j in range(6)]
+        c.of_t.copy_(P.ints(c.of))
+        c.x.normal_(generator=P.gen(i))
+        for y in c.y:
+            y.fill_(7.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        got = [y.clone() for y in c.y]
+        c.check()
+        assert all(torch.equal(p, q) for p, q in zip(got, c.y))
