@@ -26,16 +26,6 @@ __device__ __forceinline__ int v_swizzle8(int row) {
     return D == 64 ? ((row >> 2) & 1) | (far << 1) : D == 128 ? ((row >> 1) & 3) | (far << 2) : (row & 7) | (far << 3);
 }
 
-// 16 codes times a power of two, as two MFMA operands
-__device__ __forceinline__ void values_of(u32x4 w, float scale, h8& lo, h8& hi) {
-    auto four = [&](uint32_t a, uint32_t b) {
-        return join(__builtin_shufflevector(two_of<false>(a, scale), two_of<true>(a, scale), 0, 1, 2, 3),
-                    __builtin_shufflevector(two_of<false>(b, scale), two_of<true>(b, scale), 0, 1, 2, 3));
-    };
-    lo = four(w[0], w[1]);
-    hi = four(w[2], w[3]);
-}
-
 // 16 bytes a lane from each lane's own address into LDS at m0 + 16 lane
 __device__ __forceinline__ void lds_dma16_at(uint32_t lds_dst, uint64_t at) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_dst), "v"(at) : "memory", "m0");
@@ -300,26 +290,56 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
 
 // ---- the launches -------------------------------------------------------------------------
 
+// Waves and stages of the narrow part, waves of the wide one and their packed rows.
 template <int D> struct Shape8;
-template <> struct Shape8<64> { static constexpr int W = 4, S = 4; };
-template <> struct Shape8<128> { static constexpr int W = 4, S = 3; };
-template <> struct Shape8<256> { static constexpr int W = 4, S = 2; };
-constexpr int kParts8 = 512;
+template <> struct Shape8<64> { static constexpr int W = 4, S = 4, LW = 4, LS = 4, NW = 4, M = 32, PER_CU = 2; };
+template <> struct Shape8<128> { static constexpr int W = 4, S = 3, LW = 4, LS = 2, NW = 4, M = 32, PER_CU = 2; };
+template <> struct Shape8<256> { static constexpr int W = 4, S = 2, LW = 2, LS = 2, NW = 8, M = 16, PER_CU = 1; };
+constexpr int kNarrowLeast8 = 4, kBesideLeast8 = 16, kWideLeast8 = 24;
+constexpr int kFewWhole8 = 16, kManyWhole8 = 32, kWideWhole8 = 32;
+template <int D>
+constexpr int narrow8_lds(int w, int s) { return w * s * 2 * kNarrowKeys * D; }
+template <int D>
+constexpr int wide8_lds() { return 4 * kWideKeys * 2 * D; }
+template <int D>
+constexpr int wide8_rows() { return Shape8<D>::M * Shape8<D>::NW; }
+template <int D>
+constexpr int wide8_parts() { return 256 * Shape8<D>::PER_CU; }
 
 template <int D>
 __global__ __launch_bounds__(64 * Shape8<D>::W)
 void rf_paged8_attn_narrow_kernel(const rf_paged_attention a, const rf_paged_cache8 c, const Plan plan) {
     constexpr int W = Shape8<D>::W, S = Shape8<D>::S;
-    __shared__ __align__(1024) uint8_t lds[W * S * 2 * kNarrowKeys * D];
+    __shared__ __align__(1024) uint8_t lds[narrow8_lds<D>(W, S)];
     narrow8_part<D, W, S>(a, c, plan, (int)(blockIdx.x + blockIdx.y * gridDim.x), lds);
+}
+
+// Both kinds in one launch, the wide items first: their workgroups are the
+// longer ones, and the narrow ones fill the CUs that they leave.
+template <int D>
+__global__ __launch_bounds__(64 * Shape8<D>::NW) __attribute__((amdgpu_waves_per_eu(2)))
+void rf_paged8_attn_mixed_kernel(const rf_paged_attention a, const rf_paged_cache8 c, const Plan wide, const Plan narrow) {
+    constexpr int LW = Shape8<D>::LW, LS = Shape8<D>::LS, NEED = narrow8_lds<D>(LW, LS);
+    __shared__ __align__(1024) uint8_t lds[NEED > wide8_lds<D>() ? NEED : wide8_lds<D>()];
+    const int item = (int)(blockIdx.x + blockIdx.y * gridDim.x);
+    if (item < wide.items) {
+        wide_part<D, Shape8<D>::NW, Shape8<D>::M>(a, c, wide, item, lds);
+    } else {
+        if (threadIdx.x >= 64 * LW) return;      // whole waves, before any barrier
+        narrow8_part<D, LW, LS>(a, c, narrow, item - wide.items, lds);
+    }
 }
 
 template <int D>
 __global__ __launch_bounds__(256) void rf_paged8_attn_join_kernel(const rf_paged_attention a, const rf_paged_cache8 c,
-                                                                  const Plan narrow) {
+                                                                  const Plan wide, const Plan narrow, int wide_items) {
     __shared__ float weight[kJoinParts][kJoinRows];
     __shared__ f4 sums[256];
-    join_part<D, kNarrowRows, kNarrowKeys>(a, c, narrow, blockIdx.x, weight, sums);
+    const int item = blockIdx.x;
+    if (item < wide_items)
+        join_part<D, wide8_rows<D>(), kWideKeys>(a, c, wide, item, weight, sums);
+    else
+        join_part<D, kNarrowRows, kNarrowKeys>(a, c, narrow, item - wide_items, weight, sums);
 }
 
 }  // namespace rf
@@ -327,21 +347,48 @@ __global__ __launch_bounds__(256) void rf_paged8_attn_join_kernel(const rf_paged
 template <int D>
 static void attn8_go(const rf_paged_attention& a, const rf_paged_cache8& c, hipStream_t stream) {
     using namespace rf;
+    constexpr int ROWS = wide8_rows<D>();
     const int nkv = c.num_kv_heads, group = a.num_heads / nkv;
     const int64_t packed = (int64_t)a.rows * group, positions = (int64_t)a.max_blocks * c.page_size;
+    const bool both = (int64_t)a.max_new * group > kNarrowRows;
+    float* ws = static_cast<float*>(a.workspace);
     const auto inverse = [](int n) { return (uint32_t)(((1ll << 32) + n - 1) / n); };
     const uint32_t inv = packed * group < (1ll << 32) ? inverse(group) : 0;
     const int64_t some = std::min<int64_t>(a.num_seqs, a.rows);        // requests with rows
-    const int aim = kParts8;
-    Plan narrow = {group, inv, 0, INT_MAX, aim, 4, inverse(aim), 0, static_cast<float*>(a.workspace)};
-    const int64_t tiles = (packed / kNarrowRows + some) * nkv;
-    const int64_t most = std::max<int64_t>((positions + kNarrowKeys * narrow.least - 1) / (kNarrowKeys * narrow.least), 1);
-    const int64_t joins = most > 1 ? std::min<int64_t>(tiles, narrow.parts) : 0;
-    const unsigned total = (unsigned)std::min(tiles + narrow.parts, tiles * most);
+    const int64_t tiles = some * nkv;
+    const int aim = kNarrowParts;
+    const auto least = [&](int keys, int whole, int cut) { return positions <= whole * keys ? whole : cut; };
+    const int narrow_least = least(kNarrowKeys, both || tiles >= 256 ? kManyWhole8 : kFewWhole8,
+                                   both ? kBesideLeast8 : kNarrowLeast8);
+    Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, aim, narrow_least, inverse(aim), 0, ws};
+    const int64_t wide_tiles = (packed / ROWS + std::min(some, packed / kNarrowRows)) * nkv;
+    const int wide_aim = (int)std::max<int64_t>(wide8_parts<D>() - wide_tiles / 4, wide8_parts<D>() / 4);
+    Plan wide = {group, inv, kNarrowRows, INT_MAX, wide_aim, least(kWideKeys, kWideWhole8, kWideLeast8), inverse(wide_aim), 0,
+                 ws + narrow_bytes<D>() / sizeof(float)};
+    // Items: every tile has a part, and there are at most as many parts more as are aimed at (each of
+    // them a share long); no more either than the table's width gives room for.
+    const auto items = [&](int64_t tiles, const Plan& p, int keys, int64_t* joins) {
+        const int64_t most = std::max<int64_t>((positions + keys * p.least - 1) / (keys * p.least), 1);
+        *joins = most > 1 ? std::min<int64_t>(tiles, p.parts) : 0;
+        return (int)std::min(tiles + p.parts, tiles * most);
+    };
+    int64_t narrow_joins, wide_joins = 0;
+    narrow.items = items((both ? some : packed / kNarrowRows + some) * nkv, narrow, kNarrowKeys, &narrow_joins);
+    if (both) {
+        wide.items = items(wide_tiles, wide, kWideKeys, &wide_joins);
+        // (workgroups i and i + 8 share an XCD's L2, and items i and i + num_kv_heads their K and V)
+        wide.items = (wide.items + 8 * nkv - 1) / (8 * nkv) * (8 * nkv);
+    }
+    const unsigned total = (unsigned)wide.items + (unsigned)narrow.items;
     const dim3 grid(std::min(total, 1u << 20), (total + (1u << 20) - 1) >> 20);
-    hipLaunchKernelGGL((rf_paged8_attn_narrow_kernel<D>), grid, dim3(64 * Shape8<D>::W), 0, stream, a, c, narrow);
-    if (joins > 0)
-        hipLaunchKernelGGL(rf_paged8_attn_join_kernel<D>, dim3((unsigned)joins), dim3(256), 0, stream, a, c, narrow);
+    if (both)
+        hipLaunchKernelGGL(rf_paged8_attn_mixed_kernel<D>, grid, dim3(64 * Shape8<D>::NW), 0, stream, a, c, wide, narrow);
+    else
+        hipLaunchKernelGGL(rf_paged8_attn_narrow_kernel<D>, grid, dim3(64 * Shape8<D>::W), 0, stream, a, c, narrow);
+    const int wide_blocks = (int)wide_joins * (ROWS / kJoinRows);
+    if (wide_joins + narrow_joins > 0)
+        hipLaunchKernelGGL(rf_paged8_attn_join_kernel<D>, dim3((unsigned)(wide_blocks + narrow_joins)), dim3(256), 0,
+                           stream, a, c, wide, narrow, wide_blocks);
 }
 
 extern "C" hipError_t rf_paged_attention8_launch(const rf_paged_attention* step, const rf_paged_cache8* cache,

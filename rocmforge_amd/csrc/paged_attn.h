@@ -25,6 +25,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "paged8.h"
 #include "paged_common.h"
 #include "qk_common.h"
 
@@ -39,6 +40,8 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) const h8* lds_h8;
 typedef __attribute__((address_space(3))) s4* lds_s4;
 typedef __attribute__((address_space(3))) const h4* lds_h4;
+typedef __attribute__((address_space(3))) h8* lds_h8w;
+typedef __attribute__((address_space(1))) const u32x4* global_u4;
 
 constexpr float kNone = -3.0e+38f;               // the maximum of no scores
 constexpr float kLog2e = 1.4426950408889634f;
@@ -51,6 +54,7 @@ constexpr float kLag = 8.0f;
 
 constexpr int kNarrowRows = 16, kNarrowKeys = 32;
 constexpr int kWideKeys = 64;
+constexpr int kNarrowParts = 512;                // the most narrow parts that are aimed at
 // ---- which part of which request a workgroup does ---------------------------------------
 
 struct Share {
@@ -250,7 +254,16 @@ __device__ __forceinline__ h4 read_tr(uint32_t at) {
 
 __device__ __forceinline__ h8 join(h4 a, h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+// 16 codes times a power of two, as two MFMA operands
+__device__ __forceinline__ void values_of(u32x4 w, float scale, h8& lo, h8& hi) {
+    auto four = [&](uint32_t a, uint32_t b) {
+        return join(__builtin_shufflevector(two_of<false>(a, scale), two_of<true>(a, scale), 0, 1, 2, 3),
+                    __builtin_shufflevector(two_of<false>(b, scale), two_of<true>(b, scale), 0, 1, 2, 3));
+    };
+    lo = four(w[0], w[1]);
+    hi = four(w[2], w[3]);
+}
+
 // l + the eight weights, products with one in fp32.
 __device__ __forceinline__ float sum8(h8 p, float l) {
     const h2 one = {1, 1};
@@ -325,6 +338,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
     typedef typename G::acc Acc;
     constexpr int KS = D / G::DK, NB = D / M, XB = kWideKeys / M, E = G::E, XE = XB * E;
     constexpr bool BESIDE = M == 32;             // the next tile's scores beside a tile's weights
+    constexpr bool CODES = std::is_same_v<C, rf_paged_cache8>;
     static_assert(NI >= 1, "every wave has rows to fetch");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane % M, part = lane / M;   // a lane's packed row, and which keys or dims of it it has
@@ -359,7 +373,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
     const uint32_t k_piece = 16u * (uint32_t)(ds ^ k_swizzle<D>(wave_row + dr));
     const uint32_t v_piece = 16u * (uint32_t)(ds ^ v_swizzle<D>(wave_row + dr));
     // this wave's rows of a tile of K or V into its buffer; K goes first and moves the window
-    auto stage = [&](auto which, int tile) {
+    [[maybe_unused]] auto stage = [&](auto which, int tile) {
         constexpr bool values = decltype(which)::value;
         if (tile < begin || tile >= end) return;
         const int k0 = kWideKeys * tile;
@@ -392,11 +406,87 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
         else
             fetch(std::false_type());
     };
+    // Codes come through registers and are written to LDS as the fp16 values that they stand for, each once:
+    // fetch a tile's (this wave's share), put them a tile later.
+    constexpr int LPC = D / 16, RPC = 64 / LPC, NC = CODES ? kWideKeys / (RPC * NW) : 1;
+    static_assert(!CODES || NC >= 1, "every wave has rows to fetch");
+    u32x4 k_codes[NC], v_codes[NC];
+    int scales = 0, scales_before = 0;           // a unit's exponents, V's << 8: of this window and of the one before
+    const int cr = lane / LPC, cp = lane % LPC;
+    // the unit of the wave's i-th group of rows, from the tile's first on; for heads of 64 of its first half
+    auto group_unit = [&](int i) { return RPC * (wave + NW * i) >> 3; };
+    auto fetch = [&](auto which, int tile) {
+        constexpr bool values = decltype(which)::value;
+        if constexpr (CODES) {
+            if (tile < begin || tile >= end) return;
+            if (!values && (8 * tile & ~63) != window) {
+                window = 8 * tile & ~63;
+                const int page = next;
+                address = units.address(window + lane, page, bad);
+                next = units.page_of(window + 64 + lane);
+                const int64_t at = scale_at(c, (unsigned)page >= (unsigned)c.num_pages ? 0 : page,
+                                            (8 * units.seen(window + lane)) & units.pmask, block_shift(c)) + kvh;
+                scales_before = scales;
+                scales = c.k_scale[at] | (c.v_scale[at] << 8);
+            }
+            const int u0 = 8 * tile - window, k0 = kWideKeys * tile;
+            const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int row = RPC * (wave + NW * i) + cr;
+                // positions that no row sees are taken from the nearest one that some row sees
+                const int key = whole ? k0 + row : min(max(k0 + row, t.lo), t.hi - 1);
+                int unit = 8 * tile + group_unit(i);
+                uint64_t at;
+                if constexpr (RPC > 8) {         // two units
+                    const uint64_t lo = read_lane(address, u0 + group_unit(i)), hi = read_lane(address, u0 + group_unit(i) + 1);
+                    unit = units.seen(unit + (lane >> 5));
+                    at = lane < 32 ? lo : hi;
+                } else {
+                    unit = units.seen(unit);
+                    at = read_lane(address, unit - window);
+                }
+                at += (uint64_t)((uint32_t)(key - 8 * unit) * (uint32_t)c.row_stride + 16u * (uint32_t)cp);
+                (values ? v_codes : k_codes)[i] = *(global_u4)(at + (values ? v_from_k : 0));
+            }
+        }
+    };
+    auto put = [&](auto which, int tile) {
+        constexpr bool values = decltype(which)::value;
+        if constexpr (CODES) {
+            if (tile < begin || tile >= end) return;
+            const int w0 = 8 * tile & ~63, held = w0 == window ? scales : scales_before;
+            const uint32_t dst = lds0 + (values ? 2 * MAT : 0) + (uint32_t)(tile & 1) * MAT;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int unit = 8 * tile + group_unit(i), row = RPC * (wave + NW * i) + cr;
+                int byte = __builtin_amdgcn_readlane(held, units.seen(unit) - w0);
+                if constexpr (RPC > 8) byte = lane < 32 ? byte : __builtin_amdgcn_readlane(held, units.seen(unit + 1) - w0);
+                h8 lo, hi;
+                values_of((values ? v_codes : k_codes)[i], pow2_of(scale_byte((values ? byte >> 8 : byte) & 0xff)), lo, hi);
+                const uint32_t to = dst + (uint32_t)row * ROWB +
+                                    16u * (uint32_t)((2 * cp) ^ (values ? v_swizzle<D>(row) : k_swizzle<D>(row)));
+                *(lds_h8w)(to) = lo;
+                *(lds_h8w)(to ^ 16u) = hi;
+            }
+        }
+    };
     if (begin < end) {
         next = units.page_of((8 * begin & ~63) + lane);
-        stage(std::false_type(), begin);
-        stage(std::true_type(), begin);
-        if constexpr (BESIDE) stage(std::false_type(), begin + 1);
+        if constexpr (CODES) {
+            fetch(std::false_type(), begin);
+            fetch(std::true_type(), begin);
+            put(std::false_type(), begin);
+            put(std::true_type(), begin);
+            fetch(std::false_type(), begin + 1);
+            if constexpr (BESIDE) put(std::false_type(), begin + 1);
+            fetch(std::true_type(), begin + 1);
+            if constexpr (BESIDE) fetch(std::false_type(), begin + 2);
+        } else {
+            stage(std::false_type(), begin);
+            stage(std::true_type(), begin);
+            if constexpr (BESIDE) stage(std::false_type(), begin + 1);
+        }
     }
     // a negative scale moves its sign to Q (exact), so that the largest S has the largest weight; a
     // scale of zero goes to Q whole, so that what is infinite in Q or K gives NaN
@@ -570,6 +660,17 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
     // of what its step reads has landed; past the barrier everyone's has, and the buffers
     // that are filled next have been read.
     auto advance = [&](int tile) {
+        if constexpr (CODES) {
+            lds_barrier();                       // (this wave's values are written, and the next ones still on their way)
+            if (tile < begin) return;
+            if constexpr (!BESIDE) put(std::false_type(), tile + 1);
+            put(std::true_type(), tile + 1);
+            if constexpr (BESIDE) put(std::false_type(), tile + 2);
+            if constexpr (!BESIDE) fetch(std::false_type(), tile + 2);
+            fetch(std::true_type(), tile + 2);
+            if constexpr (BESIDE) fetch(std::false_type(), tile + 3);
+            return;
+        }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();
         if (tile < begin) return;
@@ -618,7 +719,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
         // the values that were replaced, to the rows that see them: those of the tiles that were run masked
         const int psh = units.psh, pmask = units.pmask;
         const int* table = units.table;
-        const uint16_t* vc = c.v + kvh * c.head_stride;
+        const auto* vc = c.v + kvh * c.head_stride;
 #pragma unroll 1
         for (int k0 = kWideKeys * mine; k0 < kWideKeys * mine_end; ++k0) {
             if (k0 == kWideKeys * full) k0 = kWideKeys * full_end;
@@ -626,16 +727,23 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
             if (k0 < t.lo || k0 >= t.hi) continue;
             const int page = table[k0 >> psh];
             if ((unsigned)page >= (unsigned)c.num_pages) continue;
-            const uint16_t* row = vc + (int64_t)page * c.page_stride + (int64_t)(k0 & pmask) * c.row_stride + 4 * part;
+            const auto* row = vc + (int64_t)page * c.page_stride + (int64_t)(k0 & pmask) * c.row_stride + 4 * part;
             const bool seen = k0 <= pos && (a.window == 0 || k0 > pos - a.window);
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int e = 0; e < E; e += 4) {
-                    const h4 w = *reinterpret_cast<const h4*>(row + M * i + G::key(e)), f = finite_of(w);
+                    if constexpr (CODES) {       // (NaN is all that a code can stand for beside what is finite)
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(row + M * i + G::key(e));
 #pragma unroll
-                    for (int n = 0; n < 4; ++n)
-                        o[i][e + n] = seen ? o[i][e + n] + ((float)w[n] - (float)f[n]) : o[i][e + n];
+                        for (int n = 0; n < 4; ++n)
+                            o[i][e + n] = seen && ((w >> (8 * n)) & 0x7f) == 0x7f ? NAN : o[i][e + n];
+                    } else {
+                        const h4 w = *reinterpret_cast<const h4*>(row + M * i + G::key(e)), f = finite_of(w);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+                            o[i][e + n] = seen ? o[i][e + n] + ((float)w[n] - (float)f[n]) : o[i][e + n];
+                    }
                 }
         }
     }
@@ -742,6 +850,10 @@ __device__ __forceinline__ void join_part(const rf_paged_attention& a, const C& 
         store4(a, (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d, acc[o] * weight[0][i / (D / 4)]);
     }
 }
+
+// Bytes of the narrow parts of a launch: twice as many as are aimed at; the wide ones' lie behind them.
+template <int D>
+constexpr size_t narrow_bytes() { return (size_t)2 * kNarrowParts * kNarrowRows * (D + 2) * sizeof(float); }
 
 // ---- what the launchers refuse -------------------------------------------------------------
 

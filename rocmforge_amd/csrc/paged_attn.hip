@@ -8,11 +8,10 @@
 namespace rf {
 
 // Least units of keys of a part (a workgroup costs about as much as 4 to 6 units
-// before and behind its loop; wide ones, and narrow ones beside them, more), and the
-// most narrow parts that are aimed at.  us, wide parts of at least 4 / 8 / 16 / 24 units: 28 single tokens
+// before and behind its loop; wide ones, and narrow ones beside them, more).  us, wide parts of at least 4 / 8 / 16 / 24 units: 28 single tokens
 // beside 4 pieces of prompt 39.5 / 33.4 / 28.5 / 28.4; 64 tokens behind 15936 66.1 / 66.2 / 50.7 / 52.9;
 // 4 prompts of 200 behind 2800 64.4 / 64.9 / 64.9 / 64.9.
-constexpr int kNarrowLeast = 4, kBesideLeast = 16, kNarrowParts = 512;
+constexpr int kNarrowLeast = 4, kBesideLeast = 16;
 constexpr int kWideLeast = 24;
 // Where tables are no wider than these many units nothing is cut, and no join is launched.  us, cut ->
 // whole, in tables of just these widths: few narrow tiles (one request of 256 positions 8.2 -> 5.9, of
@@ -312,18 +311,16 @@ __global__ __launch_bounds__(256) void rf_paged_attn_join_kernel(const rf_paged_
 
 }  // namespace rf
 
-// Bytes of the narrow and the wide parts of a launch.
-template <int D>
-static constexpr size_t narrow_bytes() { return (size_t)2 * rf::kNarrowParts * rf::kNarrowRows * (D + 2) * sizeof(float); }
+// Bytes of the wide parts of a launch.
 template <int D>
 static constexpr size_t wide_bytes() { return (size_t)2 * rf::wide_parts<D>() * rf::wide_rows<D>() * (D + 2) * sizeof(float); }
 
 extern "C" size_t rf_paged_attention_workspace_bytes(int num_heads, int num_kv_heads, int head_dim) {
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0) return 0;
     switch (head_dim) {
-    case 64: return narrow_bytes<64>() + wide_bytes<64>();
-    case 128: return narrow_bytes<128>() + wide_bytes<128>();
-    case 256: return narrow_bytes<256>() + wide_bytes<256>();
+    case 64: return rf::narrow_bytes<64>() + wide_bytes<64>();
+    case 128: return rf::narrow_bytes<128>() + wide_bytes<128>();
+    case 256: return rf::narrow_bytes<256>() + wide_bytes<256>();
     default: return 0;
     }
 }
@@ -374,7 +371,7 @@ static void attn_go(const rf_paged_attention& a, const rf_paged_cache& c, hipStr
     const int64_t wide_tiles = (packed / ROWS + std::min(some, packed / kNarrowRows)) * nkv;
     const int wide_aim = (int)std::max<int64_t>(wide_parts<D>() - wide_tiles / 4, wide_parts<D>() / 4);
     Plan wide = {group, inv, kNarrowRows, INT_MAX, wide_aim, least(kWideKeys, kWideWhole, kWideLeast), inverse(wide_aim), 0,
-                 ws + narrow_bytes<D>() / sizeof(float)};
+                 ws + rf::narrow_bytes<D>() / sizeof(float)};
     // Items: every tile has a part, and there are at most as many parts more as are aimed at (each of
     // them a share long); no more either than the table's width gives room for.
     const auto items = [&](int64_t tiles, const Plan& p, int keys, int64_t* joins) {
