@@ -884,17 +884,21 @@ hipError_t rf_paged_attention8_launch(const rf_paged_attention* step, const rf_p
  * them behind an adapter's rank are not used, whatever they hold.  ranks are clipped to [0, max_rank].
  * x is fp32, or fp16 bits (x_f16 != 0): fp32 values are taken as two of fp16's (22 bits; beyond
  * 65504 NaN or infinite sums), the inner sums as two of fp16's against the row's largest, products
- * are added in fp32.  y may be base itself (with ld_y = ld_base), else they do not overlap;
+ * are added in fp32, in an order that goes by the batch.  y may be base itself (with ld_y = ld_base), else they do not overlap;
  * rows past q_start[num_seqs] are left as they were, q_start does not fall.
  * in_dim a multiple of 8, max_rank of 8 and at most 128, out_dim, ld_base and ld_y of 4, ld_x (in
  * elements) of 8 (fp16) or 4, a_stride and b_stride of 8; pointers to x, a, b, base and y 16-byte
- * aligned; in_dim, out_dim <= 2^20; rows <= 2^23; num_targets 1 to 3.  targets is read during the call only. */
+ * aligned; in_dim, out_dim <= 2^20; rows <= 2^23; num_targets 1 to 3.  targets is read during the call only.
+ * workspace: rf_lora_workspace_bytes bytes (it depends on the numbers of both blocks, not on what their
+ * buffers hold; 0: none is needed), 16-byte aligned; launches that share one must be stream-ordered. */
 typedef struct rf_lora {
     const void* x;
     const int32_t* adapters;
     const int32_t* q_start;
     const int32_t* ranks;
     const float* scales;
+    void* workspace;
+    size_t workspace_bytes;
     int64_t ld_x;
     int32_t rows;
     int32_t num_seqs;
@@ -914,6 +918,7 @@ typedef struct rf_lora_target {
     int64_t ld_y;
     int32_t out_dim;
 } rf_lora_target;
+size_t rf_lora_workspace_bytes(const rf_lora* step, const rf_lora_target* targets, int num_targets);
 hipError_t rf_lora_add_launch(const rf_lora* step, const rf_lora_target* targets, int num_targets, hipStream_t stream);
 
 /* Rules on the logits of each row before a token is picked.  With the row's

@@ -142,5 +142,7 @@ def load() -> ctypes.CDLL:
     lib.rf_flash_attn_decode_workspace_bytes.restype = _sz
     lib.rf_paged_attention_workspace_bytes.argtypes = [_i, _i, _i]
     lib.rf_paged_attention_workspace_bytes.restype = _sz
+    lib.rf_lora_workspace_bytes.argtypes = [_vp, _vp, _i]
+    lib.rf_lora_workspace_bytes.restype = _sz
     _LIB = lib
     return lib

@@ -99,20 +99,6 @@ __device__ __forceinline__ Request request_of(const rf_paged_attention& a, const
     return r;
 }
 
-// Inclusive prefix sum over the wave: within rows of 16 lanes, then the rows' last lanes
-// into the rows behind them.
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);      // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);      // row_bcast 15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);      // row_bcast 31 into rows 2 and 3
-    return v;
-}
-
-__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
-
 // Units a part: total / parts.  A tile is cut only where it is longer, so at most
 // twice as many parts are written.  (In integers: the join has to come to the same.)
 template <int ROWS, int KEYS, class C>

@@ -168,13 +168,10 @@ def test_rows_do_not_meet(rf, dev):
 
 
 def test_row_ranges_are_clipped(rf, dev):
+    # (the order of a row's sums goes by how many rows its tile has: within the bound, not to the bit)
     c = Case([30, 40], [0, 1], [16, 16])
-    c.run()
-    want = c.y[0].clone()
-    c.y[0].fill_(7.0)
-    c.step.rows = 50
-    c.run()
-    assert torch.equal(c.y[0][:50], want[:50]) and bool((c.y[0][50:] == 7.0).all())
+    c.step.rows, c.new = 50, [30, 20]
+    c.check()
 
 
 def test_every_run_gives_the_same_bits(rf, dev):
@@ -203,6 +200,54 @@ def test_far_into_many_adapters(rf, dev):
     c.of_t += n - 2
     c.run()
     assert torch.equal(c.y[0], want)
+
+
+@pytest.mark.parametrize("new", [[1] * 5, [3, 40, 1, 200, 9]])
+def test_workspaces_of_the_caller(rf, dev, new):
+    # what lies in it, or behind it, does not matter
+    c = Case(new, [0, 1, 2, 0, 1], [16, 5, 30], 32, widths=(128, 64))
+    c.run()
+    want = [y.clone() for y in c.y]
+    n = lora.workspace_bytes(c.step, c.t)
+    ws = torch.full((n // 4 + 64,), math.nan, device=P.DEV)
+    c.step.workspace, c.step.workspace_bytes = ws, n
+    for y in c.y:
+        y.fill_(7.0)
+    c.run()
+    assert all(torch.equal(a, b) for a, b in zip(c.y, want)) and bool(ws[n // 4:].isnan().all())
+
+
+def test_streams(rf, dev):
+    # steps on streams of their own, each with memory of its own: torch's, handles and the default one
+    cases = [Case([1, 30, 2], [0, 1, 0], [16, 9], seed=i) for i in range(4)]
+    for c in cases:
+        c.run()
+    want = [c.y[0].clone() for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream(), None, 0]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, s in zip(cases, streams):
+            lora.add(c.step, c.t, s.cuda_stream if s is streams[1] else s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(c.y[0], w) for c, w in zip(cases, want))
+
+
+@pytest.mark.parametrize("rows,seqs", [(700, 3), (800, 70), (2000, 5), (2600, 40), (4000, 1)])
+@pytest.mark.parametrize("x16", [False, True])
+@pytest.mark.parametrize("max_rank", [16, 32, 64, 128])
+def test_many_rows(rf, dev, rows, seqs, x16, max_rank):
+    # tiles of 16, 32 and 64 rows, of one request and of several
+    new = [rows // seqs + (i % 5 - 2) * (seqs > 4) for i in range(seqs)]
+    Case(new, [(3 * i) % 5 - 1 for i in range(seqs)], [max_rank, 3, max_rank - 5, 17], max_rank, k=520, widths=(72, 128),
+         x16=x16, pad=3).check()
+
+
+@pytest.mark.parametrize("seqs", [3, 64, 100, 300])
+def test_requests_of_one_adapter(rf, dev, seqs):
+    # their rows share tiles
+    Case([1 + i % 3 for i in range(seqs)], [0] * seqs, [16]).check()
+    Case([1] * seqs, [i % 2 for i in range(seqs)], [16, 8], k=1024).check()
+    Case([(i % 4) * 40 for i in range(seqs)], [i % 3 - 1 for i in range(seqs)], [16, 8], x16=True).check()
 
 
 @pytest.mark.parametrize("new", [[1] * 6, [1, 70, 1, 0, 200, 3]])

@@ -86,6 +86,17 @@ def test_adapter_targets(rf, bad):
     refused(lora.add, step(), [target(), target(**bad)])
 
 
+def test_workspaces(rf):
+    big = dict(rows=100, ld_x=256)
+    n = lora.workspace_bytes(step(**big), target())
+    assert n > 0 and lora.workspace_bytes(step(**big), [target()] * 3) > n
+    assert lora.workspace_bytes(step(), target()) == 0                   # few rows: one launch
+    for bad in (dict(), dict(workspace=A), dict(workspace=A, workspace_bytes=n - 1), dict(workspace=ODD, workspace_bytes=n)):
+        assert rf.rf_lora_add_launch(ctypes.byref(step(**big, **bad)), ctypes.byref(target()), 1, None) == 1
+    assert lora.workspace_bytes(step(rows=-1), target()) == 0
+    assert lora.workspace_bytes(step(**big), []) == 0
+
+
 def test_numbers_of_targets(rf):
     refused(lora.add, step(), [])
     refused(lora.add, step(), [target()] * 4)
