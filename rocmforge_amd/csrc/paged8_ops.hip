@@ -169,14 +169,14 @@ __global__ __launch_bounds__(256) void rf_paged_rope8_kernel(const rf_paged_rope
 
 // ---- reading back ----------------------------------------------------------------------------
 //
-// A workgroup takes kReadRows rows: where they lie is found once, and then 16 codes a
-// thread become 32 bytes.  Memory-bound, one byte in and two out a value.
+// A workgroup takes kReadRows rows: where they lie is found once, and then 8 codes a
+// thread become 16 bytes.  Memory-bound, one byte in and two out a value.
 constexpr int kReadRows = 16;
 
 __global__ __launch_bounds__(256) void rf_paged_read8_kernel(const rf_paged_read s, const rf_paged_cache8 c, uint32_t inv) {
     __shared__ int64_t codes_at[kReadRows], scales_at[kReadRows];
     const int tid = threadIdx.x, lane = tid & 63, r0 = kReadRows * blockIdx.x;
-    const int bsh = block_shift(c), dsh = __ffs(c.head_dim) - 5;         // pieces of 16 a head
+    const int bsh = block_shift(c), dsh = __ffs(c.head_dim) - 4;         // pieces of 8 a head
     const int pieces = c.num_kv_heads << dsh;
     if (tid < 64) {
         // the last request that starts at or before row r0, by 64 probes at a time
@@ -209,26 +209,41 @@ __global__ __launch_bounds__(256) void rf_paged_read8_kernel(const rf_paged_read
         }
     }
     __syncthreads();
-    for (int i = tid; i < kReadRows * pieces; i += 256) {
-        const int r = inv ? (int)__umulhi((uint32_t)i, inv) : i / pieces, piece = i - r * pieces;
-        const int64_t at = codes_at[r];
-        if (at < 0) continue;
-        const int h = piece >> dsh, d = 16 * (piece & ((1 << dsh) - 1));
+    constexpr int U = 4;
+    for (int i0 = tid; i0 < kReadRows * pieces; i0 += 256 * U) {
+        u32x2 w[U][2];
+        int byte[U][2];
+        int64_t to[U];
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            uint16_t* out = v ? s.v : s.k;
-            if (out == nullptr) continue;
-            const u32x4 w = *reinterpret_cast<const u32x4*>((v ? c.v : c.k) + at + h * c.head_stride + d);
-            const float scale = pow2_of(scale_byte((v ? c.v_scale : c.k_scale)[scales_at[r] + h]));
-            u32x4 o[2];
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 256 * u;
+            const int r = min(inv ? (int)__umulhi((uint32_t)i, inv) : i / pieces, kReadRows - 1), piece = i - r * pieces;
+            const int64_t at = i < kReadRows * pieces ? codes_at[r] : -1;
+            const int h = piece >> dsh, d = 8 * (piece & ((1 << dsh) - 1));
+            to[u] = at < 0 ? -1 : (int64_t)(r0 + r) * s.ld_out + (int64_t)h * c.head_dim + d;
+            if (at >= 0)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                o[k >> 1][2 * (k & 1)] = __builtin_bit_cast(uint32_t, two_of<false>(w[k], scale));
-                o[k >> 1][2 * (k & 1) + 1] = __builtin_bit_cast(uint32_t, two_of<true>(w[k], scale));
+                for (int v = 0; v < 2; ++v) {
+                    w[u][v] = *reinterpret_cast<const u32x2*>((v ? c.v : c.k) + at + h * c.head_stride + d);
+                    byte[u][v] = (v ? c.v_scale : c.k_scale)[scales_at[r] + h];
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (to[u] < 0) continue;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                uint16_t* out = v ? s.v : s.k;
+                if (out == nullptr) continue;
+                const float scale = pow2_of(scale_byte(byte[u][v]));
+                u32x4 o;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    o[2 * k] = __builtin_bit_cast(uint32_t, two_of<false>(w[u][v][k], scale));
+                    o[2 * k + 1] = __builtin_bit_cast(uint32_t, two_of<true>(w[u][v][k], scale));
+                }
+                *reinterpret_cast<u32x4*>(out + to[u]) = o;
             }
-            u32x4* dst = reinterpret_cast<u32x4*>(out + (int64_t)(r0 + r) * s.ld_out + (int64_t)h * c.head_dim + d);
-            dst[0] = o[0];
-            dst[1] = o[1];
         }
     }
 }
@@ -281,9 +296,9 @@ extern "C" hipError_t rf_paged_read8_launch(const rf_paged_read* read, const rf_
     const int64_t width = (int64_t)cache->num_kv_heads * cache->head_dim;
     if (!s.block_tables || !s.row_start || !aligned(s.k, 16) || !aligned(s.v, 16) || s.ld_out < width || s.ld_out % 8)
         return hipErrorInvalidValue;
-    // (i / pieces is the high word of i inv while 16 pieces^2 <= 2^32)
-    const uint32_t pieces = (uint32_t)(width / 16);
-    const uint32_t inv = pieces <= 16384 ? (uint32_t)(((1ull << 32) + pieces - 1) / pieces) : 0;
+    // (i / pieces is the high word of i inv while 16 pieces^2 and what a pass reads past the end stay below 2^32)
+    const uint32_t pieces = (uint32_t)(width / 8);
+    const uint32_t inv = pieces <= 8192 ? (uint32_t)(((1ull << 32) + pieces - 1) / pieces) : 0;
     hipLaunchKernelGGL(rf::rf_paged_read8_kernel, dim3((unsigned)((s.rows + rf::kReadRows - 1) / rf::kReadRows)), dim3(256),
                        0, stream, s, *cache, inv);
     return hipGetLastError();
