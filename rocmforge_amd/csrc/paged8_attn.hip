@@ -290,11 +290,15 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
 
 // ---- the launches -------------------------------------------------------------------------
 
-// Waves and stages of the narrow part, waves of the wide one and their packed rows.
+// Waves and stages of the narrow part, waves of the wide one and their packed rows.  Two
+// stages a wave, so that two and more workgroups share a CU: 48 requests of 60 to 16000 positions
+// (head_dim 128) 52.4 us, with three stages and one workgroup a CU 67; at 64 a third stage is even
+// (47.7 and 48.1 us, 64 requests of 2000).  At 256 two waves, for the same reason: 256 requests
+// of 600 138 us, with four waves 166.
 template <int D> struct Shape8;
-template <> struct Shape8<64> { static constexpr int W = 4, S = 4, LW = 4, LS = 4, NW = 4, M = 32, PER_CU = 2; };
-template <> struct Shape8<128> { static constexpr int W = 4, S = 3, LW = 4, LS = 2, NW = 4, M = 32, PER_CU = 2; };
-template <> struct Shape8<256> { static constexpr int W = 4, S = 2, LW = 2, LS = 2, NW = 8, M = 16, PER_CU = 1; };
+template <> struct Shape8<64> { static constexpr int W = 4, S = 2, LW = 4, LS = 4, NW = 4, M = 32, PER_CU = 2; };
+template <> struct Shape8<128> { static constexpr int W = 4, S = 2, LW = 4, LS = 2, NW = 4, M = 32, PER_CU = 2; };
+template <> struct Shape8<256> { static constexpr int W = 2, S = 2, LW = 2, LS = 2, NW = 8, M = 16, PER_CU = 1; };
 constexpr int kNarrowLeast8 = 4, kBesideLeast8 = 16, kWideLeast8 = 24;
 constexpr int kFewWhole8 = 16, kManyWhole8 = 32, kWideWhole8 = 32;
 template <int D>
@@ -356,7 +360,10 @@ static void attn8_go(const rf_paged_attention& a, const rf_paged_cache8& c, hipS
     const uint32_t inv = packed * group < (1ll << 32) ? inverse(group) : 0;
     const int64_t some = std::min<int64_t>(a.num_seqs, a.rows);        // requests with rows
     const int64_t tiles = some * nkv;
-    const int aim = kNarrowParts;
+    // Few tiles in a part a CU, more in nearly two, as the joins cost little beside the ragged
+    // end then (head_dim 128): one request of 16000 positions 17.3 us at 256 parts and 18.9 at 400,
+    // 20 of 4000 49.1 and 44.1, 48 of 60 to 16000 56.9, 52.4 and, at 512, 57.8.
+    const int aim = tiles < 64 ? 256 : 400;
     const auto least = [&](int keys, int whole, int cut) { return positions <= whole * keys ? whole : cut; };
     const int narrow_least = least(kNarrowKeys, both || tiles >= 256 ? kManyWhole8 : kFewWhole8,
                                    both ? kBesideLeast8 : kNarrowLeast8);
