@@ -12,170 +12,189 @@ namespace rf {
 // ---- the rotary step into the pages --------------------------------------------------------
 //
 // A block's exponent needs all its new rows, so a workgroup takes whole runs of rows that
-// share a block: those that start among 16 rows, at most 31 of them (a prompt's 16, or
-// 16 requests' single tokens).  D / 8 lanes a row, 8 elements a lane, the rows of a head at
-// once and one head after the other; a lane's four pairs turn by the same angles in all
-// heads, so it takes their cosines once.  A run's largest value meets through LDS.
-constexpr int kRunRows = 16;                     // first rows of runs a workgroup looks at
+// share a block: those that start among 16 rows (32 at head_dim 64), up to 15 more with the
+// last one's (a prompt's 16, or 16 requests' single tokens).  D / 8 lanes a row, 8 elements a
+// lane, the rows of a head at once and one head after the other; a lane's four pairs turn by
+// the same angles in all heads, so it takes their cosines once.  A run's largest value meets
+// through LDS.  Where the runs have more rows than the threads take, the last one goes by itself.
+constexpr int kRunRows = 16;                     // the most rows of a run
+template <int D>
+constexpr int rope8_threads() { return D == 256 ? 512 : 256; }
+template <int D>
+constexpr int start_rows() { return rope8_threads<D>() / (D / 8); }
 
 template <int D, bool NEOX>
-__global__ __launch_bounds__(256) void rf_paged_rope8_kernel(const rf_paged_rope s, const rf_paged_cache8 c, int per) {
-    constexpr int LPH = D / 8, RPP = 256 / LPH, PASSES = (2 * kRunRows - 1 + RPP - 1) / RPP;
-    __shared__ float tops[2][2 * kRunRows];      // a row's largest finite value
-    __shared__ int olds[2][2 * kRunRows];        // the exponent before, at a run's first row
+__global__ __launch_bounds__(rope8_threads<D>(), 5)
+void rf_paged_rope8_kernel(const rf_paged_rope s, const rf_paged_cache8 c, int per) {
+    constexpr int ROWS = start_rows<D>(), LPH = D / 8;
+    static_assert(ROWS >= kRunRows && ROWS + kRunRows < 64, "the threads take a run, a wave's ballot all rows");
+    __shared__ float tops[2][ROWS];              // a row's largest finite value
+    __shared__ int olds[2][ROWS];                // the exponent before, at a run's first row
     const int tid = threadIdx.x, lane = tid & 63, u = tid % LPH;
-    const int bsh = block_shift(c), slots = c.num_pages * c.page_size;
-    const int r0 = kRunRows * blockIdx.x;
+    const int bsh = block_shift(c), slots = c.num_pages * c.page_size, psh = __ffs(c.page_size) - 1;
+    const int r0 = ROWS * blockIdx.x;
     // a run: rows one behind the other with rising slots of one block
     const int at = r0 + lane;
-    const bool there = lane < 3 * kRunRows && at < s.rows;
+    const bool there = lane < ROWS + kRunRows && at < s.rows;
     const int now = there ? s.slots[at] : -1, before = there && at > 0 ? s.slots[at - 1] : -1;
     const bool lead = !there || (unsigned)now >= (unsigned)slots || (unsigned)before >= (unsigned)slots ||
                       now <= before || (now >> bsh) != (before >> bsh);
-    const uint64_t leads = __ballot(lead);
-    if ((leads & 0xffffu) == 0) return;
-    const int a0 = __builtin_ctzll(leads), first = r0 + a0;
-    const int n = min(kRunRows + __builtin_ctzll(leads >> kRunRows), s.rows - r0) - a0;
-    if (n <= 0) return;
+    const uint64_t leads = __ballot(lead), mine = leads & ((1ull << ROWS) - 1);
+    if (mine == 0) return;
+    const int a0 = __builtin_ctzll(mine), last = 63 - __builtin_clzll(mine);
+    const int a2 = min(ROWS + __builtin_ctzll(leads >> ROWS), s.rows - r0);      // (rows from r0 on)
+    if (a2 <= a0) return;
+    const int a1 = a2 - a0 <= ROWS ? a2 : last;
 
     const int half = s.rot_dim / 2, heads = s.num_heads + 2 * c.num_kv_heads;
     const bool turned = u < s.rot_dim / 8;
     const int e0 = NEOX && turned ? 4 * u : 8 * u, e1 = NEOX && turned ? half + 4 * u : e0 + 4;
     const int h0 = blockIdx.y * per, h1 = min(h0 + per, heads);
-    int row[PASSES], slot[PASSES], run[PASSES], end[PASSES];     // run, end: rows of this row's run, from `first` on
-    float4 a[PASSES], b[PASSES];
-    auto load = [&](int h, int p) {
-        const int64_t r = first + row[p];
-        const float* src = h < s.num_heads ? s.q + r * s.ld_q + (int64_t)h * D
-                           : h < s.num_heads + c.num_kv_heads
-                               ? s.k + r * s.ld_k + (int64_t)(h - s.num_heads) * D
-                               : s.v + r * s.ld_v + (int64_t)(h - s.num_heads - c.num_kv_heads) * D;
-        a[p] = *reinterpret_cast<const float4*>(src + e0);
-        b[p] = *reinterpret_cast<const float4*>(src + e1);
-    };
-    float2 cs[PASSES][4];
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        row[p] = RPP * p + tid / LPH;
-        slot[p] = -1;
-        if (row[p] >= n) continue;
-        const int r = first + row[p], bit = a0 + row[p];
-        slot[p] = s.slots[r];
-        if ((unsigned)slot[p] >= (unsigned)slots) {
-            slot[p] = -1;
-            continue;
-        }
-        load(h0, p);
-        run[p] = 63 - __builtin_clzll(leads & ((2ull << bit) - 1)) - a0;
-        end[p] = min(bit + 1 + __builtin_ctzll(leads >> (bit + 1)) - a0, n);
-        if (turned)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const double turn = (double)s.positions[r] * s.turns[4 * u + i];
-                float sn, co;
-                sincospif(2.0f * (float)(turn - rint(turn)), &sn, &co);
-                cs[p][i] = make_float2(co * s.attn_factor, sn * s.attn_factor);
-            }
-    }
-    for (int h = h0; h < h1; ++h) {
-        const bool is_q = h < s.num_heads, is_v = h >= s.num_heads + c.num_kv_heads;
-        const int kvh = is_v ? h - s.num_heads - c.num_kv_heads : h - s.num_heads;
-        const float* w = is_v ? nullptr : is_q ? s.q_norm : s.k_norm;
-        uint8_t* codes = (is_v ? c.v : c.k) + (is_q ? 0 : kvh) * c.head_stride;
-        uint8_t* scales = (is_v ? c.v_scale : c.k_scale) + (is_q ? 0 : kvh);
-        const int buf = h & 1;
-        float y[PASSES][8];
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            if (slot[p] < 0) continue;
-            float x[8] = {a[p].x, a[p].y, a[p].z, a[p].w, b[p].x, b[p].y, b[p].z, b[p].w};
-            if (h + 1 < h1) load(h + 1, p);
-            // (every lane of a row takes the same way, and rows do not share lanes)
-            if (w != nullptr) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ss = __fmaf_rn(x[i], x[i], ss);
-                ss = xor_sum<LPH / 2, 1>(ss);
-                const float inv = 1.0f / sqrtf(ss * (1.0f / D) + s.eps);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[(i < 4 ? e0 : e1 - 4) + i];
-            }
-            if (!is_v && turned) {
+    int buf = 0;
+    for (int begin = a0, n = a1 - a0; n > 0; begin += n, n = a2 - begin) {
+        const int first = r0 + begin;
+        const int row = tid / LPH;               // from `first` on, as run and end, its run's
+        int slot = -1, run = 0, end = 0, from = 0;       // from: place in the block of the run's first row
+        float4 a, b;
+        auto load = [&](int h) {
+            const int64_t r = first + row;
+            const float* src = h < s.num_heads ? s.q + r * s.ld_q + (int64_t)h * D
+                               : h < s.num_heads + c.num_kv_heads
+                                   ? s.k + r * s.ld_k + (int64_t)(h - s.num_heads) * D
+                                   : s.v + r * s.ld_v + (int64_t)(h - s.num_heads - c.num_kv_heads) * D;
+            a = *reinterpret_cast<const float4*>(src + e0);
+            b = *reinterpret_cast<const float4*>(src + e1);
+        };
+        float2 cs[4];
+        const int r = first + row, bit = begin + row;
+        if (row < n) slot = s.slots[r];
+        const bool live = (unsigned)slot < (unsigned)slots;
+        if (live) {
+            load(h0);
+            run = 63 - __builtin_clzll(leads & ((2ull << bit) - 1)) - begin;
+            end = min(bit + 1 + __builtin_ctzll(leads >> (bit + 1)) - begin, n);
+            from = s.slots[first + run] & ((1 << bsh) - 1);
+            if (turned)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 t = cs[p][i];
-                    constexpr int P = NEOX ? 1 : 2, Q = NEOX ? 4 : 1;
-                    const float f = x[P * i], g = x[P * i + Q];
-                    x[P * i] = __fmaf_rn(f, t.x, -(g * t.y));
-                    x[P * i + Q] = __fmaf_rn(f, t.y, g * t.x);
+                    const double turn = (double)s.positions[r] * s.turns[4 * u + i];
+                    float sn, co;
+                    sincospif(2.0f * (float)(turn - rint(turn)), &sn, &co);
+                    cs[i] = make_float2(co * s.attn_factor, sn * s.attn_factor);
                 }
-            }
-            if (is_q) {
-                uint16_t* dst = s.q16 + (int64_t)(first + row[p]) * s.ld_q16 + (int64_t)h * D;
-                uint32_t o[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    o[i] = (uint32_t)f16_bits_rn(x[2 * i]) | ((uint32_t)f16_bits_rn(x[2 * i + 1]) << 16);
-                *reinterpret_cast<uint2*>(dst + e0) = make_uint2(o[0], o[1]);
-                *reinterpret_cast<uint2*>(dst + e1) = make_uint2(o[2], o[3]);
-                continue;
-            }
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                y[p][i] = x[i];
-                top = fmaxf(top, nan_unless_finite(x[i]) == 0.0f ? fabsf(x[i]) : 0.0f);
-            }
-            top = xor_max<LPH / 2, 1>(top);
-            if (u == 0) {
-                tops[buf][row[p]] = top;
-                // (one lane reads it, and writes it again below)
-                if (run[p] == row[p])
-                    olds[buf][row[p]] = scale_byte(scales[(int64_t)(slot[p] >> bsh) * c.num_kv_heads]);
-            }
         }
-        if (is_q) continue;
-        __syncthreads();                         // (of the other buffer's readers all have passed the barrier before)
+        float4 w0 = {1, 1, 1, 1}, w1 = w0;       // the norm's weights
+        for (int h = h0; h < h1; ++h) {
+            const bool is_q = h < s.num_heads, is_v = h >= s.num_heads + c.num_kv_heads;
+            const int kvh = is_v ? h - s.num_heads - c.num_kv_heads : h - s.num_heads;
+            const float* w = is_v ? nullptr : is_q ? s.q_norm : s.k_norm;
+            if (w != nullptr && (h == h0 || h == s.num_heads)) {
+                w0 = *reinterpret_cast<const float4*>(w + e0);
+                w1 = *reinterpret_cast<const float4*>(w + e1);
+            }
+            uint8_t* codes = (is_v ? c.v : c.k) + (is_q ? 0 : kvh) * c.head_stride;
+            uint8_t* scales = (is_v ? c.v_scale : c.k_scale) + (is_q ? 0 : kvh);
+            float y[8];
+            if (live) {
+                float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                if (h + 1 < h1) load(h + 1);
+                // (every lane of a row takes the same way, and rows do not share lanes)
+                if (w != nullptr) {
+                    float ss = 0.0f;
 #pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            if (slot[p] < 0) continue;
-            float top = 0.0f;
-            for (int i = run[p]; i < end[p]; ++i) top = fmaxf(top, tops[buf][i]);
-            // the place in the block of the run's first row: rows of a run need not be all of its rows
-            const int from = s.slots[first + run[p]] & ((1 << bsh) - 1);
-            const int old = olds[buf][run[p]], fit = scale_for(top), e = from == 0 ? fit : max(fit, old);
-            const float by = pow2_of(254 - e);
-            uint8_t* dst = codes + (int64_t)(slot[p] / c.page_size) * c.page_stride +
-                           (int64_t)(slot[p] % c.page_size) * c.row_stride;
-            const float lo[4] = {y[p][0], y[p][1], y[p][2], y[p][3]}, hi[4] = {y[p][4], y[p][5], y[p][6], y[p][7]};
-            *reinterpret_cast<uint32_t*>(dst + e0) = codes_of(lo, by);
-            *reinterpret_cast<uint32_t*>(dst + e1) = codes_of(hi, by);
-            if (run[p] == row[p]) {
-                if (from > 0 && e > old) {
-                    const float less = pow2_of(127 + old - e);
-                    for (int i = 1; i <= from; ++i) {
-                        uint8_t* was = dst - i * c.row_stride;
-                        uint32_t* w0 = reinterpret_cast<uint32_t*>(was + e0);
-                        uint32_t* w1 = reinterpret_cast<uint32_t*>(was + e1);
-                        *w0 = recoded(*w0, less);
-                        *w1 = recoded(*w1, less);
+                    for (int i = 0; i < 8; ++i) ss = __fmaf_rn(x[i], x[i], ss);
+                    ss = xor_sum<LPH / 2, 1>(ss);
+                    const float inv = 1.0f / sqrtf(ss * (1.0f / D) + s.eps);
+                    const float by[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * by[i];
+                }
+                if (!is_v && turned) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 t = cs[i];
+                        constexpr int P = NEOX ? 1 : 2, Q = NEOX ? 4 : 1;
+                        const float f = x[P * i], g = x[P * i + Q];
+                        x[P * i] = __fmaf_rn(f, t.x, -(g * t.y));
+                        x[P * i + Q] = __fmaf_rn(f, t.y, g * t.x);
                     }
                 }
-                if (u == 0) scales[(int64_t)(slot[p] >> bsh) * c.num_kv_heads] = (uint8_t)e;
+                if (is_q) {
+                    uint16_t* dst = s.q16 + (int64_t)(first + row) * s.ld_q16 + (int64_t)h * D;
+                    uint32_t o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[i] = (uint32_t)f16_bits_rn(x[2 * i]) | ((uint32_t)f16_bits_rn(x[2 * i + 1]) << 16);
+                    *reinterpret_cast<uint2*>(dst + e0) = make_uint2(o[0], o[1]);
+                    *reinterpret_cast<uint2*>(dst + e1) = make_uint2(o[2], o[3]);
+                } else {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        y[i] = x[i];
+                        top = fmaxf(top, nan_unless_finite(x[i]) == 0.0f ? fabsf(x[i]) : 0.0f);
+                    }
+                    top = xor_max<LPH / 2, 1>(top);
+                    if (u == 0) {
+                        tops[buf][row] = top;
+                        // (one lane reads it, and writes it again below)
+                        if (run == row) olds[buf][row] = scale_byte(scales[(int64_t)(slot >> bsh) * c.num_kv_heads]);
+                    }
+                }
             }
+            if (is_q) continue;
+            __syncthreads();                     // (of the other buffer's readers all have passed the barrier before)
+            if (live) {
+                float top = 0.0f;
+                for (int i = run + u; i < end; i += LPH) top = fmaxf(top, tops[buf][i]);
+                top = xor_max<LPH / 2, 1>(top);
+                const int old = olds[buf][run], fit = scale_for(top), e = from == 0 ? fit : max(fit, old);
+                const float by = pow2_of(254 - e);
+                uint8_t* dst = codes + (int64_t)(slot >> psh) * c.page_stride +
+                               (int64_t)(slot & (c.page_size - 1)) * c.row_stride;
+                const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
+                *reinterpret_cast<uint32_t*>(dst + e0) = codes_of(lo, by);
+                *reinterpret_cast<uint32_t*>(dst + e1) = codes_of(hi, by);
+                if (run == row) {
+                    if (from > 0 && e > old) {
+                        // the block's rows before, two at a time (more cost registers, and so the prompts time)
+                        const float less = pow2_of(127 + old - e);
+                        constexpr int AT_ONCE = 2;
+                        for (int i0 = 1; i0 <= from; i0 += AT_ONCE) {
+                            uint32_t was[AT_ONCE][2];
+#pragma unroll
+                            for (int i = 0; i < AT_ONCE; ++i) {
+                                const uint8_t* src = dst - min(i0 + i, from) * c.row_stride;
+                                was[i][0] = *reinterpret_cast<const uint32_t*>(src + e0);
+                                was[i][1] = *reinterpret_cast<const uint32_t*>(src + e1);
+                            }
+#pragma unroll
+                            for (int i = 0; i < AT_ONCE; ++i) {
+                                if (i0 + i > from) continue;
+                                uint8_t* to = dst - (i0 + i) * c.row_stride;
+                                *reinterpret_cast<uint32_t*>(to + e0) = recoded(was[i][0], less);
+                                *reinterpret_cast<uint32_t*>(to + e1) = recoded(was[i][1], less);
+                            }
+                        }
+                    }
+                    if (u == 0) scales[(int64_t)(slot >> bsh) * c.num_kv_heads] = (uint8_t)e;
+                }
+            }
+            buf ^= 1;
         }
     }
 }
 
 // ---- reading back ----------------------------------------------------------------------------
 //
-// A workgroup takes kReadRows rows: where they lie is found once, and then 8 codes a
+// A workgroup takes a few rows: where they lie is found once, and then 8 codes a
 // thread become 16 bytes.  Memory-bound, one byte in and two out a value.
-constexpr int kReadRows = 16;
+constexpr int kReadRows = 4;                     // at most
 
-__global__ __launch_bounds__(256) void rf_paged_read8_kernel(const rf_paged_read s, const rf_paged_cache8 c, uint32_t inv) {
+__global__ __launch_bounds__(256) void rf_paged_read8_kernel(const rf_paged_read s, const rf_paged_cache8 c, int per,
+                                                            uint32_t inv) {
     __shared__ int64_t codes_at[kReadRows], scales_at[kReadRows];
-    const int tid = threadIdx.x, lane = tid & 63, r0 = kReadRows * blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, r0 = per * blockIdx.x;
     const int bsh = block_shift(c), dsh = __ffs(c.head_dim) - 4;         // pieces of 8 a head
     const int pieces = c.num_kv_heads << dsh;
     if (tid < 64) {
@@ -188,10 +207,18 @@ __global__ __launch_bounds__(256) void rf_paged_read8_kernel(const rf_paged_read
             lo += k;
             len = min(step, len - k);
         }
-        if (lane < kReadRows) {
+        // and how many more start by each of the others, 64 starts at a time
+        int b = lo;
+        for (int b0 = lo + 1;; b0 += 64) {
+            const int start = lane <= s.num_seqs - b0 ? s.row_start[b0 + lane] : INT_MAX;
+            for (int i = 0; i < per; ++i) {
+                const int more = __popcll(__ballot(start <= r0 + i));
+                if (lane == i) b += more;
+            }
+            if (__builtin_amdgcn_readlane(start, 63) >= r0 + per) break;
+        }
+        if (lane < per) {
             const int r = r0 + lane;
-            int b = lo;
-            while (b < s.num_seqs && s.row_start[b + 1] <= r) ++b;
             int64_t at = -1;
             if (r < s.rows && b < s.num_seqs && s.row_start[b] <= r) {
                 const int64_t pos = (int64_t)(s.first != nullptr ? s.first[b] : 0) + (r - max(s.row_start[b], 0));
@@ -210,22 +237,25 @@ __global__ __launch_bounds__(256) void rf_paged_read8_kernel(const rf_paged_read
     }
     __syncthreads();
     constexpr int U = 4;
-    for (int i0 = tid; i0 < kReadRows * pieces; i0 += 256 * U) {
+    // (what is not asked for is not read: its loads are the other's again)
+    const uint8_t* from[2] = {s.k ? c.k : c.v, s.v ? c.v : c.k};
+    const uint8_t* bytes[2] = {s.k ? c.k_scale : c.v_scale, s.v ? c.v_scale : c.k_scale};
+    for (int i0 = tid; i0 < per * pieces; i0 += 256 * U) {
         u32x2 w[U][2];
         int byte[U][2];
         int64_t to[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + 256 * u;
-            const int r = min(inv ? (int)__umulhi((uint32_t)i, inv) : i / pieces, kReadRows - 1), piece = i - r * pieces;
-            const int64_t at = i < kReadRows * pieces ? codes_at[r] : -1;
+            const int r = min(inv ? (int)__umulhi((uint32_t)i, inv) : i / pieces, per - 1), piece = i - r * pieces;
+            const int64_t at = i < per * pieces ? codes_at[r] : -1;
             const int h = piece >> dsh, d = 8 * (piece & ((1 << dsh) - 1));
             to[u] = at < 0 ? -1 : (int64_t)(r0 + r) * s.ld_out + (int64_t)h * c.head_dim + d;
             if (at >= 0)
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    w[u][v] = *reinterpret_cast<const u32x2*>((v ? c.v : c.k) + at + h * c.head_stride + d);
-                    byte[u][v] = (v ? c.v_scale : c.k_scale)[scales_at[r] + h];
+                    w[u][v] = *reinterpret_cast<const u32x2*>(from[v] + at + h * c.head_stride + d);
+                    byte[u][v] = bytes[v][scales_at[r] + h];
                 }
         }
 #pragma unroll
@@ -268,16 +298,18 @@ extern "C" hipError_t rf_paged_rope_write8_launch(const rf_paged_rope* step, con
         !aligned(s.k_norm, 16) || !aligned(s.turns, 8) || s.ld_q % 4 || s.ld_k % 4 || s.ld_v % 4 || s.ld_q16 % 8 ||
         s.ld_q < 0 || s.ld_k < 0 || s.ld_v < 0 || s.ld_q16 < (int64_t)s.num_heads * cache->head_dim)
         return hipErrorInvalidValue;
-    const int heads = s.num_heads + 2 * cache->num_kv_heads, chunks = (s.rows + rf::kRunRows - 1) / rf::kRunRows;
-    // as many heads a workgroup as leave eight of them a CU, so that cosines are shared
-    const int64_t most = 8ll * rf::device_cu_count();
+    const int heads = s.num_heads + 2 * cache->num_kv_heads, starts = cache->head_dim == 64 ? rf::start_rows<64>() : rf::start_rows<128>();
+    const int chunks = (s.rows + starts - 1) / starts;
+    // as many heads a workgroup as leave sixteen of them a CU, so that cosines are shared: 4000 rows
+    // of 48 heads 36 us, with eight a CU 40, with one head a workgroup 48
+    const int64_t most = 16ll * rf::device_cu_count();
     const int per = (int)std::min<int64_t>(std::max<int64_t>(((int64_t)chunks * heads + most - 1) / most, (heads + 65534) / 65535), heads);
-    const dim3 grid(chunks, (heads + per - 1) / per), blk(256);
+    const dim3 grid(chunks, (heads + per - 1) / per);
 #define ROPE_GO(D)                                                                                         \
     if (s.neox)                                                                                            \
-        hipLaunchKernelGGL((rf::rf_paged_rope8_kernel<D, true>), grid, blk, 0, stream, s, *cache, per);    \
+        hipLaunchKernelGGL((rf::rf_paged_rope8_kernel<D, true>), grid, dim3(rf::rope8_threads<D>()), 0, stream, s, *cache, per);    \
     else                                                                                                   \
-        hipLaunchKernelGGL((rf::rf_paged_rope8_kernel<D, false>), grid, blk, 0, stream, s, *cache, per);
+        hipLaunchKernelGGL((rf::rf_paged_rope8_kernel<D, false>), grid, dim3(rf::rope8_threads<D>()), 0, stream, s, *cache, per);
     switch (cache->head_dim) {
     case 64: ROPE_GO(64) break;
     case 128: ROPE_GO(128) break;
@@ -299,7 +331,10 @@ extern "C" hipError_t rf_paged_read8_launch(const rf_paged_read* read, const rf_
     // (i / pieces is the high word of i inv while 16 pieces^2 and what a pass reads past the end stay below 2^32)
     const uint32_t pieces = (uint32_t)(width / 8);
     const uint32_t inv = pieces <= 8192 ? (uint32_t)(((1ull << 32) + pieces - 1) / pieces) : 0;
-    hipLaunchKernelGGL(rf::rf_paged_read8_kernel, dim3((unsigned)((s.rows + rf::kReadRows - 1) / rf::kReadRows)), dim3(256),
-                       0, stream, s, *cache, inv);
+    // few rows in twos (640 rows of 8 heads of 128 3.5 us, in fours 3.7, in sixteens 6.4), many in fours (48
+    // ragged requests 210 us, in sixteens 214)
+    const int per = s.rows <= 4096 ? 2 : rf::kReadRows;
+    hipLaunchKernelGGL(rf::rf_paged_read8_kernel, dim3((unsigned)((s.rows + per - 1) / per)), dim3(256), 0, stream, s,
+                       *cache, per, inv);
     return hipGetLastError();
 }

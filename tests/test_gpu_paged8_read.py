@@ -65,7 +65,8 @@ class Case:
 
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("nkv", [1, 3, 8])
-@pytest.mark.parametrize("lens", [[1], [640], [15, 16, 17], [0, 5, 0, 0, 33, 0], [1] * 70, [3 + i % 40 for i in range(200)]])
+@pytest.mark.parametrize("lens", [[1], [640], [15, 16, 17], [0, 5, 0, 0, 33, 0], [1] * 70, [3 + i % 40 for i in range(200)],
+                                  [0] * 100 + [1] + [0] * 150 + [2, 1, 0, 1] + [0] * 70 + [9], [40] * 120, [5000, 1, 1, 0, 1]])
 def test_lengths_and_heads(rf, dev, lens, nkv, d):
     Case(lens, nkv=nkv, d=d).check()
 

@@ -158,6 +158,19 @@ def test_single_tokens(rf, dev, rows):
     Step([16 * ((7 * i) % rows) + i % 16 for i in range(rows)], pages=rows, old=0.05).check()
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("singles", [1, 14, 15, 16, 30, 31, 32])
+def test_long_runs_behind_single_tokens(rf, dev, singles, d):
+    # more rows start in a group than its threads take at once
+    slots = [16 * (4 + i) + i % 16 for i in range(singles)] + list(range(32)) + [35, 37, 39]
+    Step(slots, d=d, pages=40, old=0.05).check()
+    Step(slots, d=d, pages=80, page=8, rot=d, norm=True).check()
+
+
+def test_heads_of_all_kinds_in_a_workgroup(rf, dev):
+    Step(list(range(7, 1507)), 33, 8, rot=128, norm=True, pages=100).check()
+
+
 def test_many_rows(rf, dev):
     # heads shared among few workgroups a row
     s = Step(list(range(7, 3007)), 8, 2, 64, pages=200)
