@@ -12,6 +12,7 @@ namespace rf {
 typedef int i2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i2* lds_i2;
 typedef __attribute__((address_space(3))) const u32x4* lds_u4;
+typedef __attribute__((address_space(3))) float* lds_f;
 
 // A row of D codes in LDS lies as in memory, its 16-byte pieces permuted so that neither
 // K's reads (one piece of 16 rows) nor V's transposing ones (one piece of the rows 8 i .. 8 i + 7
@@ -288,25 +289,409 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
     }
 }
 
+// ---- pieces of prompt, heads of 256 ---------------------------------------------------------
+//
+// Two waves share 32 packed rows: each has the scores of half of a tile's 64 positions and the
+// outputs of half of the dims, and they swap weights through LDS, in the registers' order.  So a
+// wave's queries and outputs take 128 registers, two waves fit a SIMD, and an operand that is
+// read from LDS meets 32 rows.  Codes stay codes in LDS and become fp16 on their way into the MFMAs:
+// an operand's conversion is 16 clocks of VALU beside the 32 of its MFMA.
+//
+// A row's maximum is rounded up to a whole number, so that the two waves' weights come to the
+// larger one by powers of two, exactly.  No weight of a row need be one of fp16's then, so the sum is
+// of the weights before they are rounded: an output is off by their roundings, 2^-11 of sum w |v|
+// at most, where a sum of rounded weights would let two comparable ones err by twice that.
+constexpr int kPairRows = 32, kPairStages = 3;
+template <int D, int NW>
+constexpr int pair8_lds() { return 2 * kPairStages * kWideKeys * D + NW * (2 * 2048 + 3 * 4 * kPairRows); }
+
+// Dims of 4 part + {0 .. 3, 8 .. 11} positions of 16: rows of 16 bytes, the 16 lanes' 8 rows and the
+// next piece's in other banks.
+__device__ __forceinline__ int pair_swizzle(int row) { return 2 * ((row & 3) | ((row >> 1) & 4)); }
+
+template <int D, int NW>
+__device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf_paged_cache8& c, const Plan& plan,
+                                           int item, uint8_t* lds) {
+    static_assert(D == 256, "a row of 16 pieces, its half a wave's outputs");
+    constexpr int M = kPairRows, ROWS = M * NW / 2, MAT = kWideKeys * D, KS = D / 16, NB = D / 2 / M;
+    constexpr int RPI = 4, NI = kWideKeys / (RPI * NW);          // rows an instruction, a wave's instructions a tile
+    typedef Geo<M> G;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = wave & 1, col = lane % M, part = lane / M;
+    // (what a lane works out from this, it works out where it is used: registers are scarce in the loop,
+    // and a reload of one waits for the tiles that are on their way)
+    auto lane_here = [&] {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        return l;
+    };
+    const int nkv = c.num_kv_heads;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    const uint32_t weights0 = lds0 + 2 * kPairStages * MAT, tops0 = weights0 + 2 * NW * 2048, sums0 = tops0 + 2 * NW * 4 * M;
+
+    Share s;
+    const int kvh = item % nkv;
+    if (!find_share<ROWS, kWideKeys>(a, c, plan, item / nkv, false, s)) return;
+    const int rows = s.n * plan.group, r0 = ROWS * s.tile;
+    const Span t = span_of(plan, s, r0, min(r0 + ROWS, rows) - 1, a.window);
+    const int w0 = r0 + M * (wave >> 1);
+    const bool active = w0 < rows;
+    const Span u = span_of(plan, s, min(w0, rows - 1), min(w0 + M, rows) - 1, a.window);
+    const int p0 = t.lo / kWideKeys, p1 = (t.hi + kWideKeys - 1) / kWideKeys;
+    const int each = (max(p1 - p0, 0) + s.parts - 1) / s.parts;
+    const int begin = p0 + s.part * each, end = min(begin + each, p1);
+    const int r = min(w0 + col, rows - 1), token = token_of(plan, r), head = r - token * plan.group;
+    const int pos = s.kv - s.n + token;
+    // the addresses and exponents (K's, V's << 8) of 64 units, and the pages of the next 64
+    const Units<rf_paged_cache8> units(a, c, s.b, kvh, t.lo, t.hi);
+    const int bsh = block_shift(c);
+    bool bad = false;
+    int next = 0, window = -1, k_byte = 0, v_byte = 0;   // the bytes as loaded: they are waited for where they are used
+    uint64_t address = 0;
+    const uint64_t v_from_k = (uint64_t)c.v - (uint64_t)c.k;
+    const uint32_t stride = (uint32_t)c.row_stride;
+    auto buffer = [&](int tile) { return (uint32_t)tile % kPairStages * MAT; };
+    // this wave's rows of a tile of K or V into its buffer; K goes ahead and moves the window
+    auto stage = [&](auto which, int tile) {
+        constexpr bool values = decltype(which)::value;
+        if (tile < begin || tile >= end) return;
+        const int k0 = kWideKeys * tile;
+        if (!values && (8 * tile & ~63) != window) {
+            window = 8 * tile & ~63;
+            const int page = next;
+            address = units.address(window + lane, page, bad);
+            next = units.page_of(window + 64 + lane);
+            const int64_t at = scale_at(c, (unsigned)page >= (unsigned)c.num_pages ? 0 : page,
+                                        (8 * units.seen(window + lane)) & units.pmask, bsh) + kvh;
+            k_byte = c.k_scale[at];
+            v_byte = c.v_scale[at];
+        }
+        const uint32_t dst = lds0 + (values ? kPairStages * MAT : 0) + buffer(tile);
+        const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
+        const int ln = lane_here(), dr = ln / 16, ds = ln % 16;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int row0 = RPI * (wave + NW * i), row = row0 + dr;
+            const uint32_t piece = 16u * (uint32_t)(ds ^ (values ? pair_swizzle(row) : k_swizzle8<D>(row)));
+            int unit = 8 * tile + (row0 >> 3);
+            uint32_t off = (uint32_t)((row0 & 7) + dr) * stride;
+            if (!whole) {
+                // positions that no row sees are taken from the nearest one that some row sees
+                const int seen = units.seen(unit);
+                off = (uint32_t)(min(max(k0 + row, t.lo), t.hi - 1) - 8 * seen) * stride;
+            }
+            const uint64_t at = read_lane(address, unit - window) + (values ? v_from_k : 0);
+            lds_dma16(__builtin_amdgcn_readfirstlane(dst + (uint32_t)row0 * D), off + piece, reinterpret_cast<const uint8_t*>(at));
+        }
+    };
+    int scales = 0, scales_before = 0;           // the exponents of a tile's units (V's << 8), and of the 64 before
+    auto turn = [&] {
+        scales_before = scales;
+        scales = scale_byte(k_byte) | (scale_byte(v_byte) << 8);
+    };
+    if (begin < end) {
+        next = units.page_of((8 * begin & ~63) + lane);
+        stage(std::false_type(), begin);
+        stage(std::true_type(), begin);
+        turn();
+        stage(std::false_type(), begin + 1);
+    }
+    // the sign and a zero of the scale go to Q, as in wide_part
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+    // dims 32 j + 16 part + {0 .. 7, 8 .. 15} are this lane's of k-steps 2 j and 2 j + 1, as K's 16-byte reads have them
+    h8 q[KS];
+    const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 16 * part;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+        q[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qrow + 32 * (k >> 1) + 8 * (k & 1)) ^ sign);
+        if (a.scale == 0.0f) q[k] *= (_Float16)0;
+    }
+    // operand addresses: one base, and an xor for each piece
+    const int krow = M * half + col;
+    const uint32_t ka = lds0 + (uint32_t)krow * D + 16u * (uint32_t)(part ^ k_swizzle8<D>(krow));
+    const int i16 = lane & 15, vr = 4 * part + ((i16 >> 1) & 3) + 8 * (i16 >> 3);
+    const uint32_t va = lds0 + kPairStages * MAT + (uint32_t)vr * D +
+                        16u * (uint32_t)((8 * half + ((lane >> 4) & 1)) ^ pair_swizzle(vr)) + 8u * (uint32_t)(i16 & 1);
+    // a wave's weights and maxima of a tile
+    auto weights_at = [&](int wave, int tile, int ln) { return weights0 + (uint32_t)((tile & 1) * NW + wave) * 2048 + 16u * ln; };
+    auto top_at = [&](int wave, int tile, int ln) { return tops0 + (uint32_t)((tile & 1) * NW + wave) * (4 * M) + 4u * (ln % M); };
+    f16v o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+    // m: of the outputs, both waves'; own: of this wave's newest weights and of l
+    float m = kNone, own = kNone, l = 0.0f, mul = scale;
+    bool dirty = false;
+    h8 p[4];                                     // the weights of this half's positions, and of the other's
+
+    // S^T of this wave's half of a tile
+    auto scores = [&](int tile, f16v& x) {
+        uint32_t kt = ka + buffer(tile);
+        asm("" : "+v"(kt));
+        const float ks = pow2_of(__builtin_amdgcn_ds_bpermute(4 * ((8 * tile & 63) + 4 * half + (lane_here() % M >> 3)), scales) & 0xff);
+        auto codes = [&](int j) { return *(lds_u4)(kt ^ (32u * j)); };
+        constexpr int AHEAD = 2;
+        u32x4 w[AHEAD + 1];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) w[j] = codes(j);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KS / 2; ++j) {
+            if (j + AHEAD < KS / 2) w[(j + AHEAD) % (AHEAD + 1)] = codes(j + AHEAD);
+            h8 lo, hi;
+            values_of(w[j % (AHEAD + 1)], ks, lo, hi);
+            x = G::mfma(lo, q[2 * j], x);
+            x = G::mfma(hi, q[2 * j + 1], x);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Both halves' weights of a tile, under one maximum.
+    auto meet = [&](int tile) {
+        const int ln = lane_here();
+        const uint32_t at = weights_at(wave ^ 1, tile, ln);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) p[2 + i] = *(lds_h8)(at + 1024u * i);
+        const float other = *(lds_f)(top_at(wave ^ 1, tile, ln));
+        const float most = fmaxf(own, other);
+        if (__ballot(most != m || most != own || most != other)) {
+            const float f = __builtin_amdgcn_exp2f(m - most), g = __builtin_amdgcn_exp2f(own - most);
+            const _Float16 mine = (_Float16)g, others = (_Float16)__builtin_amdgcn_exp2f(other - most);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                p[i] *= mine;
+                p[2 + i] *= others;
+            }
+            l *= g;
+            m = own = most;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= f;
+        }
+    };
+    // The softmax of x, a tile's scores, in two steps: the maximum, and the 2 n-th and next weight.
+    auto maximum = [&](auto mask, int tile, f16v& x) {
+        if constexpr (decltype(mask)::value) {
+            const int ahead = pos - kWideKeys * tile - M * half - 4 * part, behind = a.window > 0 ? ahead - a.window : INT_MIN;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (G::key(e) > ahead || G::key(e) <= behind) x[e] = -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
+        top = xor_butterfly<32, 32>(top, max_raw) * scale;
+        const bool up = top > m + kLag;
+        own = up ? ceilf(top) : m;
+        if (__ballot(up)) l *= up ? __builtin_amdgcn_exp2f(m - own) : 1.0f;
+        // a score times the scale less the maximum in one fma; past 2^23, where the maximum was itself
+        // rounded by a half and more, the product is rounded as it was
+        const bool far = fabsf(own) >= 0x1p23f && own != kNone;
+        mul = scale;
+        if (__ballot(far)) {
+            const float by = far ? scale : 1.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], by);
+            mul = far ? 1.0f : scale;
+        }
+    };
+    u32x4 w[2];
+    auto weights = [&](int n, const f16v& x) {
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) f[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * n + i], mul, -own));
+        w[n >> 2][n & 3] = __builtin_bit_cast(uint32_t, h2{(_Float16)f[0], (_Float16)f[1]});
+        asm volatile("" : "+v"(w[n >> 2][n & 3]));               // here, not where it is used
+        l += f[0] + f[1];
+    };
+    auto give = [&](int tile) {
+        const int ln = lane_here();
+        const uint32_t at = weights_at(wave, tile, ln);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            p[i] = __builtin_bit_cast(h8, w[i]);
+            *(lds_h8w)(at + 1024u * i) = p[i];
+        }
+        if (ln < M) *(lds_f)(top_at(wave, tile, ln)) = own;
+    };
+    // O^T += V^T P^T of a tile; beside(n): what is done beside the n-th product
+    auto product = [&](auto mask, int tile, auto beside) {
+        // (the scores are a tile ahead)
+        const int at = 8 * tile & 63, held = at == 56 ? scales_before : scales;
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {            // 16 positions each, this wave's half first
+            const int side = f < 2 ? half : 1 - half;
+            uint32_t vt = va + buffer(tile) + (uint32_t)(M * side + 16 * (f & 1)) * D;
+            asm("" : "+v"(vt));
+            float vs[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                vs[i] = pow2_of(__builtin_amdgcn_readlane(held, at + 4 * side + 2 * (f & 1) + i) >> 8);
+            i2 codes[NB];
+#pragma unroll
+            for (int d = 0; d < NB; ++d) codes[d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2)(vt ^ (32u * d)));
+            if constexpr (decltype(mask)::value) {
+                // NaN among values that some rows do not see must not meet their zero weights: zeros
+                // take its place, and the rows that see it get it at the end
+                i2 nan = {0, 0};
+#pragma unroll
+                for (int d = 0; d < NB; ++d) nan |= (codes[d] & 0x7f7f7f7f) + 0x01010101;
+                if (__ballot(((nan[0] | nan[1]) & 0x80808080) != 0)) {
+                    dirty = true;
+#pragma unroll
+                    for (int d = 0; d < NB; ++d) {
+                        const i2 one = (((codes[d] & 0x7f7f7f7f) + 0x01010101) >> 7) & 0x01010101;
+                        codes[d] &= ~((one << 8) - one);
+                    }
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < NB; ++d) {
+                const i2 k = codes[d];
+                const h8 v = join(__builtin_shufflevector(two_of<false>(k[0], vs[0]), two_of<true>(k[0], vs[0]), 0, 1, 2, 3),
+                                  __builtin_shufflevector(two_of<false>(k[1], vs[1]), two_of<true>(k[1], vs[1]), 0, 1, 2, 3));
+                o[d] = G::mfma(v, p[f], o[d]);
+                beside(NB * f + d);
+            }
+        }
+    };
+
+    // the tiles that this pair's rows see, and among them those that all its rows see whole
+    const int mine = active ? min(max(u.lo / kWideKeys, begin), end) : end;
+    const int mine_end = active ? max(min((u.hi + kWideKeys - 1) / kWideKeys, end), mine) : end;
+    const int behind = a.window > 0 ? max(u.last - a.window + kWideKeys, 0) / kWideKeys : 0;
+    const int full = min(max(behind, mine), mine_end);
+    const int full_end = min(max((u.first + 1) / kWideKeys, full), mine_end);
+    f16v x;
+    // A turn: a tile's product beside the scores and the softmax of the next one.  At its start this
+    // wave's share of what is read has landed (all but what the turn before has asked for); past the
+    // barrier everyone's has, the weights are there, and the buffers that are filled next have been read.
+    auto start = [&](int tile) {
+        if (tile + 2 < end)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();
+        if (tile >= begin && (tile + 1) % 8 == 0) turn();
+        stage(std::true_type(), tile + 2);
+        stage(std::false_type(), tile + 3);
+    };
+    int tile = begin - 1;
+    while (true) {
+        const int whole = full_end - 1;          // turns from full on have whole tiles on both sides
+        const int stop = tile < full && full < whole ? full : end;
+#pragma unroll 1
+        for (; tile < stop; ++tile) {
+            start(tile);
+            const bool more = tile + 1 >= mine && tile + 1 < mine_end;
+            if (more) scores(tile + 1, x);
+            if (tile >= mine && tile < mine_end) {
+                meet(tile);
+                product(std::true_type(), tile, [](int) {});
+            }
+            if (more) {
+                maximum(std::true_type(), tile + 1, x);
+#pragma unroll
+                for (int n = 0; n < 8; ++n) weights(n, x);
+                give(tile + 1);
+            }
+        }
+        if (tile >= end) break;
+#pragma unroll 1
+        for (; tile < whole; ++tile) {
+            start(tile);
+            meet(tile);
+            scores(tile + 1, x);
+            product(std::false_type(), tile, [&](int n) {
+                // (the scores have settled beside the first four)
+                if (n == 3) maximum(std::false_type(), tile + 1, x);
+                if (n >= 4 && n < 12) weights(n - 4, x);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            give(tile + 1);
+        }
+    }
+    if (dirty) {
+        // the NaN that were replaced, to the rows that see them: those of the tiles that were run masked
+        const uint8_t* vc = c.v + kvh * c.head_stride + D / 2 * half + 4 * part;
+#pragma unroll 1
+        for (int k0 = kWideKeys * mine; k0 < kWideKeys * mine_end; ++k0) {
+            if (k0 == kWideKeys * full) k0 = kWideKeys * max(full, full_end - 1);
+            if (k0 >= kWideKeys * mine_end) break;
+            if (k0 < t.lo || k0 >= t.hi) continue;
+            const int page = units.table[k0 >> units.psh];
+            if ((unsigned)page >= (unsigned)c.num_pages) continue;
+            const uint8_t* row = vc + (int64_t)page * c.page_stride + (int64_t)(k0 & units.pmask) * c.row_stride;
+            const bool seen = k0 <= pos && (a.window == 0 || k0 > pos - a.window);
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const uint32_t codes = *reinterpret_cast<const uint32_t*>(row + M * i + G::key(e));
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        o[i][e + n] = seen && ((codes >> (8 * n)) & 0x7f) == 0x7f ? NAN : o[i][e + n];
+                }
+        }
+    }
+    // both halves' sums
+    l = xor_sum<32, 32>(l);
+    if (bad) l = NAN;
+    const uint32_t sum_at = sums0 + 4u * col;
+    if (part == 0) *(lds_f)(sum_at + 4u * M * wave) = l;
+    lds_barrier();
+    l += *(lds_f)(sum_at + 4u * M * (wave ^ 1));
+    if (!active || w0 + col >= rows) return;
+    const int d0 = D / 2 * half + 4 * part;
+    if (s.parts > 1) {
+        float* to = slot_of<ROWS, D>(plan.states, s, s.part, kvh, nkv);
+        const int row = M * (wave >> 1) + col;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<f4*>(to + row * D + d0 + M * i + G::key(e)) = f4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+        if (half == 0 && part == 0) {
+            to[ROWS * D + row] = m;
+            to[ROWS * (D + 1) + row] = l;
+        }
+    } else {
+        // (worked out again, not kept in registers over the loop)
+        int row = w0 + col;
+        asm("" : "+v"(row));
+        const int tk = token_of(plan, row), hd = row - tk * plan.group;
+        const float inv = s.kv - s.n + tk < 0 ? 0.0f : 1.0f / l;
+        const int64_t at = (int64_t)(s.q0 + tk) * a.ld_out + (int64_t)(kvh * plan.group + hd) * D + d0;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                store4(a, at + M * i + G::key(e), f4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]} * inv);
+    }
+}
+
 // ---- the launches -------------------------------------------------------------------------
 
-// Waves and stages of the narrow part, waves of the wide one and their packed rows.  Two
+// Waves and stages of the narrow part, waves of the wide one, its workgroups a CU.  Two
 // stages a wave, so that two and more workgroups share a CU: 48 requests of 60 to 16000 positions
 // (head_dim 128) 52.4 us, with three stages and one workgroup a CU 67; at 64 a third stage is even
 // (47.7 and 48.1 us, 64 requests of 2000).  At 256 two waves, for the same reason: 256 requests
 // of 600 138 us, with four waves 166.
 template <int D> struct Shape8;
-template <> struct Shape8<64> { static constexpr int W = 4, S = 2, LW = 4, LS = 4, NW = 4, M = 32, PER_CU = 2; };
-template <> struct Shape8<128> { static constexpr int W = 4, S = 2, LW = 4, LS = 2, NW = 4, M = 32, PER_CU = 2; };
-template <> struct Shape8<256> { static constexpr int W = 2, S = 2, LW = 2, LS = 2, NW = 8, M = 16, PER_CU = 1; };
+template <> struct Shape8<64> { static constexpr int W = 4, S = 2, LW = 4, LS = 4, NW = 4, PER_CU = 2; };
+template <> struct Shape8<128> { static constexpr int W = 4, S = 2, LW = 4, LS = 2, NW = 4, PER_CU = 2; };
+template <> struct Shape8<256> { static constexpr int W = 2, S = 2, LW = 2, LS = 2, NW = 8, PER_CU = 1; };
 constexpr int kNarrowLeast8 = 4, kBesideLeast8 = 16, kWideLeast8 = 24;
 constexpr int kFewWhole8 = 16, kManyWhole8 = 32, kWideWhole8 = 32;
 template <int D>
 constexpr int narrow8_lds(int w, int s) { return w * s * 2 * kNarrowKeys * D; }
 template <int D>
-constexpr int wide8_lds() { return 4 * kWideKeys * 2 * D; }
+constexpr int wide8_lds() { return D == 256 ? pair8_lds<D, Shape8<D>::NW>() : 4 * kWideKeys * 2 * D; }
 template <int D>
-constexpr int wide8_rows() { return Shape8<D>::M * Shape8<D>::NW; }
+constexpr int wide8_rows() { return 32 * Shape8<D>::NW / (D == 256 ? 2 : 1); }
 template <int D>
 constexpr int wide8_parts() { return 256 * Shape8<D>::PER_CU; }
 
@@ -327,7 +712,10 @@ void rf_paged8_attn_mixed_kernel(const rf_paged_attention a, const rf_paged_cach
     __shared__ __align__(1024) uint8_t lds[NEED > wide8_lds<D>() ? NEED : wide8_lds<D>()];
     const int item = (int)(blockIdx.x + blockIdx.y * gridDim.x);
     if (item < wide.items) {
-        wide_part<D, Shape8<D>::NW, Shape8<D>::M>(a, c, wide, item, lds);
+        if constexpr (D == 256)
+            pair8_part<D, Shape8<D>::NW>(a, c, wide, item, lds);
+        else
+            wide_part<D, Shape8<D>::NW, 32>(a, c, wide, item, lds);
     } else {
         if (threadIdx.x >= 64 * LW) return;      // whole waves, before any barrier
         narrow8_part<D, LW, LS>(a, c, narrow, item - wide.items, lds);
