@@ -13,6 +13,7 @@ typedef int i2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i2* lds_i2;
 typedef __attribute__((address_space(3))) const u32x4* lds_u4;
 typedef __attribute__((address_space(3))) float* lds_f;
+typedef __attribute__((address_space(3))) const int* lds_int;
 
 // A row of D codes in LDS lies as in memory, its 16-byte pieces permuted so that neither
 // K's reads (one piece of 16 rows) nor V's transposing ones (one piece of the rows 8 i .. 8 i + 7
@@ -30,6 +31,11 @@ __device__ __forceinline__ int v_swizzle8(int row) {
 // 16 bytes a lane from each lane's own address into LDS at m0 + 16 lane
 __device__ __forceinline__ void lds_dma16_at(uint32_t lds_dst, uint64_t at) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_dst), "v"(at) : "memory", "m0");
+}
+
+// A byte a lane, as 32 bits at m0 + 4 lane
+__device__ __forceinline__ void lds_dma_byte_at(uint32_t lds_dst, uint64_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_ubyte %1, off" ::"s"(lds_dst), "v"(at) : "memory", "m0");
 }
 
 // ---- few rows -------------------------------------------------------------------------
@@ -295,7 +301,10 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
 // outputs of half of the dims, and they swap weights through LDS, in the registers' order.  So a
 // wave's queries and outputs take 128 registers, two waves fit a SIMD, and an operand that is
 // read from LDS meets 32 rows.  Codes stay codes in LDS and become fp16 on their way into the MFMAs:
-// an operand's conversion is 16 clocks of VALU beside the 32 of its MFMA.
+// an operand's conversion is 16 clocks of VALU beside the 32 of its MFMA.  Three stages of tiles: with two,
+// each turn waited for memory.  A turn of 64 positions takes 5000 clocks where its MFMAs take 2048 and its
+// VALU instructions 2700 a SIMD, in two waves that overlap them in part; a step of three windowed prompts
+// 75 us, with 16 rows a wave over fp16 values in LDS 106.
 //
 // A row's maximum is rounded up to a whole number, so that the two waves' weights come to the
 // larger one by powers of two, exactly.  No weight of a row need be one of fp16's then, so the sum is
@@ -303,11 +312,64 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
 // at most, where a sum of rounded weights would let two comparable ones err by twice that.
 constexpr int kPairRows = 32, kPairStages = 3;
 template <int D, int NW>
-constexpr int pair8_lds() { return 2 * kPairStages * kWideKeys * D + NW * (2 * 2048 + 3 * 4 * kPairRows); }
+constexpr int pair8_lds() { return 2 * kPairStages * kWideKeys * D + NW * (2 * 2048 + 3 * 4 * kPairRows) + 1024; }
 
 // Dims of 4 part + {0 .. 3, 8 .. 11} positions of 16: rows of 16 bytes, the 16 lanes' 8 rows and the
 // next piece's in other banks.
-__device__ __forceinline__ int pair_swizzle(int row) { return 2 * ((row & 3) | ((row >> 1) & 4)); }
+__device__ __forceinline__ uint32_t pair_swizzle(uint32_t row) { return 2 * ((row & 3) | ((row >> 1) & 4)); }
+
+// find_share's items in another order, for up to 64 requests: those that a window makes equally long in the
+// requests' order, then the first (longest) of the others of each request, the second of each, and
+// so on, so that short ones fill the end of a launch.  16 heads on 8, window 1024: three prompts of 600 to
+// 1900 tokens and six single ones 75 us, in the requests' order 83; four of 100 to 3000 71 and 74 (all of
+// them by rank 86: neighbours share K and V in an XCD's L2); eight of 200 to 1000 without a window 115 and 124.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool find_ranked(const rf_paged_attention& a, const rf_paged_cache8& c, const Plan& p, int j,
+                                            Share& s) {
+    const Request r = request_of<ROWS, KEYS>(a, c, p, threadIdx.x & 63);
+    const int share = share_of<ROWS, KEYS>(a, c, p, r);
+    const int parts = max((int)(((unsigned)r.units + share - 1) / (unsigned)share), 1), items = r.tiles * parts;
+    const int slots = parts > 1 ? items : 0, slots_end = wave_scan(slots);
+    // (tiles whose rows all see from position 0 on are the shorter, the earlier they are)
+    const int growing = a.window == 0 ? items : parts > 1 ? 0 : (int)max(min((int64_t)a.window - (r.kv - r.n), (int64_t)r.n), (int64_t)0) * p.group / ROWS;
+    const int equal = items - growing, equal_end = wave_scan(equal), equals = __builtin_amdgcn_readlane(equal_end, 63);
+    int l, at;
+    if (j < equals) {
+        l = __builtin_ctzll(__ballot(equal_end > j));
+        at = j - __builtin_amdgcn_readlane(equal_end - equal, l);
+    } else {
+        j -= equals;
+        const int all = wave_total(growing);
+        if (j >= all) return false;
+        // the rank: the last one with no more items before it, the sum of min(growing, rank)
+        int lo = 0, before = 0;
+        if ((__popcll(__ballot(growing > 0))) == 1) lo = before = j;
+        for (int hi = all; lo < j && hi - lo > 1;) {
+            const int k = (lo + hi) >> 1, n = wave_total(min(growing, k));
+            if (n <= j) {
+                lo = k;
+                before = n;
+            } else {
+                hi = k;
+            }
+        }
+        const uint64_t there = __ballot(growing > lo);
+        const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(there >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)there, 0));
+        l = __builtin_ctzll(__ballot(growing > lo && rank == j - before));
+        at = __builtin_amdgcn_readlane(equal, l) + lo;
+    }
+    auto get = [l](int v) { return __builtin_amdgcn_readlane(v, l); };
+    s.b = l;
+    s.q0 = get(r.q0);
+    s.n = get(r.n);
+    s.kv = get(r.kv);
+    s.tiles = get(r.tiles);
+    s.parts = get(parts);
+    s.slot = get(slots_end - slots);
+    s.part = at / s.tiles;
+    s.tile = s.tiles - 1 - (at - s.part * s.tiles);
+    return true;
+}
 
 template <int D, int NW>
 __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf_paged_cache8& c, const Plan& plan,
@@ -321,17 +383,20 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     // (what a lane works out from this, it works out where it is used: registers are scarce in the loop,
     // and a reload of one waits for the tiles that are on their way)
     auto lane_here = [&] {
-        int l = lane;
+        uint32_t l = (uint32_t)lane;
         asm volatile("" : "+v"(l));
         return l;
     };
     const int nkv = c.num_kv_heads;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     const uint32_t weights0 = lds0 + 2 * kPairStages * MAT, tops0 = weights0 + 2 * NW * 2048, sums0 = tops0 + 2 * NW * 4 * M;
+    const uint32_t bytes0 = sums0 + NW * 4 * M;
 
     Share s;
     const int kvh = item % nkv;
-    if (!find_share<ROWS, kWideKeys>(a, c, plan, item / nkv, false, s)) return;
+    if (!(a.num_seqs <= 64 ? find_ranked<ROWS, kWideKeys>(a, c, plan, item / nkv, s)
+                           : find_share<ROWS, kWideKeys>(a, c, plan, item / nkv, false, s)))
+        return;
     const int rows = s.n * plan.group, r0 = ROWS * s.tile;
     const Span t = span_of(plan, s, r0, min(r0 + ROWS, rows) - 1, a.window);
     const int w0 = r0 + M * (wave >> 1);
@@ -342,17 +407,21 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     const int begin = p0 + s.part * each, end = min(begin + each, p1);
     const int r = min(w0 + col, rows - 1), token = token_of(plan, r), head = r - token * plan.group;
     const int pos = s.kv - s.n + token;
-    // the addresses and exponents (K's, V's << 8) of 64 units, and the pages of the next 64
+    // the addresses of 64 units and the pages of the next 64; their exponents go to LDS, K's 64 and V's, with
+    // the tiles (a load into a register would be waited for at the branch's end, and all tiles with it)
     const Units<rf_paged_cache8> units(a, c, s.b, kvh, t.lo, t.hi);
     const int bsh = block_shift(c);
     bool bad = false;
-    int next = 0, window = -1, k_byte = 0, v_byte = 0;   // the bytes as loaded: they are waited for where they are used
+    int next = 0, window = -1;
     uint64_t address = 0;
     const uint64_t v_from_k = (uint64_t)c.v - (uint64_t)c.k;
     const uint32_t stride = (uint32_t)c.row_stride;
-    auto buffer = [&](int tile) { return (uint32_t)tile % kPairStages * MAT; };
+    auto bytes_at = [&](int tile) { return bytes0 + (uint32_t)(tile & 8) * 64; };
+    // the buffer of the tile after one's, and of the one before
+    auto after = [](uint32_t buf) { return buf == (kPairStages - 1) * MAT ? 0 : buf + MAT; };
+    auto ahead_of = [](uint32_t buf) { return buf == 0 ? (kPairStages - 1) * MAT : buf - MAT; };
     // this wave's rows of a tile of K or V into its buffer; K goes ahead and moves the window
-    auto stage = [&](auto which, int tile) {
+    auto stage = [&](auto which, int tile, uint32_t buf) {
         constexpr bool values = decltype(which)::value;
         if (tile < begin || tile >= end) return;
         const int k0 = kWideKeys * tile;
@@ -361,50 +430,51 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
             const int page = next;
             address = units.address(window + lane, page, bad);
             next = units.page_of(window + 64 + lane);
-            const int64_t at = scale_at(c, (unsigned)page >= (unsigned)c.num_pages ? 0 : page,
-                                        (8 * units.seen(window + lane)) & units.pmask, bsh) + kvh;
-            k_byte = c.k_scale[at];
-            v_byte = c.v_scale[at];
-        }
-        const uint32_t dst = lds0 + (values ? kPairStages * MAT : 0) + buffer(tile);
-        const bool whole = k0 >= t.lo && k0 + kWideKeys <= t.hi;
-        const int ln = lane_here(), dr = ln / 16, ds = ln % 16;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int row0 = RPI * (wave + NW * i), row = row0 + dr;
-            const uint32_t piece = 16u * (uint32_t)(ds ^ (values ? pair_swizzle(row) : k_swizzle8<D>(row)));
-            int unit = 8 * tile + (row0 >> 3);
-            uint32_t off = (uint32_t)((row0 & 7) + dr) * stride;
-            if (!whole) {
-                // positions that no row sees are taken from the nearest one that some row sees
-                const int seen = units.seen(unit);
-                off = (uint32_t)(min(max(k0 + row, t.lo), t.hi - 1) - 8 * seen) * stride;
+            if (wave == 0) {
+                const int64_t at = scale_at(c, (unsigned)page >= (unsigned)c.num_pages ? 0 : page,
+                                            (8 * units.seen(window + lane)) & units.pmask, bsh) + kvh;
+                lds_dma_byte_at(__builtin_amdgcn_readfirstlane(bytes_at(tile)), (uint64_t)(c.k_scale + at));
+                lds_dma_byte_at(__builtin_amdgcn_readfirstlane(bytes_at(tile) + 256), (uint64_t)(c.v_scale + at));
             }
-            const uint64_t at = read_lane(address, unit - window) + (values ? v_from_k : 0);
-            lds_dma16(__builtin_amdgcn_readfirstlane(dst + (uint32_t)row0 * D), off + piece, reinterpret_cast<const uint8_t*>(at));
         }
+        const uint32_t dst = lds0 + (values ? kPairStages * MAT : 0) + buf, ln = lane_here(), dr = ln / 16, ds = ln % 16;
+        auto rows_of = [&](auto all) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int row0 = RPI * (wave + NW * i);
+                const uint32_t row = row0 + dr, piece = 16u * (ds ^ (values ? pair_swizzle(row) : k_swizzle8<D>(row)));
+                const int unit = 8 * tile + (row0 >> 3);
+                uint32_t off = ((row0 & 7) + dr) * stride;
+                // positions that no row sees are taken from the nearest one that some row sees
+                if constexpr (!decltype(all)::value)
+                    off = (uint32_t)(min(max(k0 + (int)row, t.lo), t.hi - 1) - 8 * units.seen(unit)) * stride;
+                const uint64_t at = read_lane(address, unit - window) + (values ? v_from_k : 0);
+                lds_dma16(__builtin_amdgcn_readfirstlane(dst + (uint32_t)row0 * D), off + piece, reinterpret_cast<const uint8_t*>(at));
+            }
+        };
+        if (k0 >= t.lo && k0 + kWideKeys <= t.hi)
+            rows_of(std::true_type());
+        else
+            rows_of(std::false_type());
     };
-    int scales = 0, scales_before = 0;           // the exponents of a tile's units (V's << 8), and of the 64 before
-    auto turn = [&] {
-        scales_before = scales;
-        scales = scale_byte(k_byte) | (scale_byte(v_byte) << 8);
-    };
-    if (begin < end) {
-        next = units.page_of((8 * begin & ~63) + lane);
-        stage(std::false_type(), begin);
-        stage(std::true_type(), begin);
-        turn();
-        stage(std::false_type(), begin + 1);
-    }
-    // the sign and a zero of the scale go to Q, as in wide_part
-    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
-    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
     // dims 32 j + 16 part + {0 .. 7, 8 .. 15} are this lane's of k-steps 2 j and 2 j + 1, as K's 16-byte reads have them
     h8 q[KS];
     const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 16 * part;
 #pragma unroll
+    for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const h8*>(qrow + 32 * (k >> 1) + 8 * (k & 1));
+    uint32_t buf = (uint32_t)(begin + 2) % kPairStages * MAT;    // of the tile before the first
+    if (begin < end) {
+        next = units.page_of((8 * begin & ~63) + lane);
+        stage(std::false_type(), begin, after(buf));
+        stage(std::true_type(), begin, after(buf));
+        stage(std::false_type(), begin + 1, ahead_of(buf));
+    }
+    // the sign and a zero of the scale go to Q, as in wide_part
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+#pragma unroll
     for (int k = 0; k < KS; ++k) {
-        q[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qrow + 32 * (k >> 1) + 8 * (k & 1)) ^ sign);
+        q[k] = __builtin_bit_cast(h8, __builtin_bit_cast(u32x4, q[k]) ^ sign);
         if (a.scale == 0.0f) q[k] *= (_Float16)0;
     }
     // operand addresses: one base, and an xor for each piece
@@ -414,8 +484,8 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     const uint32_t va = lds0 + kPairStages * MAT + (uint32_t)vr * D +
                         16u * (uint32_t)((8 * half + ((lane >> 4) & 1)) ^ pair_swizzle(vr)) + 8u * (uint32_t)(i16 & 1);
     // a wave's weights and maxima of a tile
-    auto weights_at = [&](int wave, int tile, int ln) { return weights0 + (uint32_t)((tile & 1) * NW + wave) * 2048 + 16u * ln; };
-    auto top_at = [&](int wave, int tile, int ln) { return tops0 + (uint32_t)((tile & 1) * NW + wave) * (4 * M) + 4u * (ln % M); };
+    auto weights_at = [&](int wave, int tile, uint32_t ln) { return weights0 + (uint32_t)((tile & 1) * NW + wave) * 2048 + 16u * ln; };
+    auto top_at = [&](int wave, int tile, uint32_t ln) { return tops0 + (uint32_t)((tile & 1) * NW + wave) * (4 * M) + 4u * (ln % M); };
     f16v o[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
@@ -427,10 +497,10 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     h8 p[4];                                     // the weights of this half's positions, and of the other's
 
     // S^T of this wave's half of a tile
-    auto scores = [&](int tile, f16v& x) {
-        uint32_t kt = ka + buffer(tile);
+    auto scores = [&](int tile, uint32_t buf, f16v& x) {
+        uint32_t kt = ka + buf;
         asm("" : "+v"(kt));
-        const float ks = pow2_of(__builtin_amdgcn_ds_bpermute(4 * ((8 * tile & 63) + 4 * half + (lane_here() % M >> 3)), scales) & 0xff);
+        const float ks = pow2_of(scale_byte(*(lds_int)(bytes_at(tile) + 4u * ((8 * tile & 63) + 4 * half + lane_here() % M / 8))));
         auto codes = [&](int j) { return *(lds_u4)(kt ^ (32u * j)); };
         constexpr int AHEAD = 2;
         u32x4 w[AHEAD + 1];
@@ -450,7 +520,7 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     };
     // Both halves' weights of a tile, under one maximum.
     auto meet = [&](int tile) {
-        const int ln = lane_here();
+        const uint32_t ln = lane_here();
         const uint32_t at = weights_at(wave ^ 1, tile, ln);
 #pragma unroll
         for (int i = 0; i < 2; ++i) p[2 + i] = *(lds_h8)(at + 1024u * i);
@@ -508,7 +578,7 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
         l += f[0] + f[1];
     };
     auto give = [&](int tile) {
-        const int ln = lane_here();
+        const uint32_t ln = lane_here();
         const uint32_t at = weights_at(wave, tile, ln);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -517,40 +587,47 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
         }
         if (ln < M) *(lds_f)(top_at(wave, tile, ln)) = own;
     };
-    // O^T += V^T P^T of a tile; beside(n): what is done beside the n-th product
-    auto product = [&](auto mask, int tile, auto beside) {
-        // (the scores are a tile ahead)
-        const int at = 8 * tile & 63, held = at == 56 ? scales_before : scales;
+    // O^T += V^T P^T of a tile, 16 positions at a time, this wave's half first, their codes read a turn
+    // ahead (the first ones by the caller); beside(n): what is done beside the n-th product
+    i2 codes[2][NB];
+    auto read_codes = [&](uint32_t buf, int f) {
+        uint32_t vt = va + buf + (uint32_t)(M * (f < 2 ? half : 1 - half) + 16 * (f & 1)) * D;
+        asm("" : "+v"(vt));
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {            // 16 positions each, this wave's half first
-            const int side = f < 2 ? half : 1 - half;
-            uint32_t vt = va + buffer(tile) + (uint32_t)(M * side + 16 * (f & 1)) * D;
-            asm("" : "+v"(vt));
-            float vs[2];
+        for (int d = 0; d < NB; ++d) codes[f & 1][d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2)(vt ^ (32u * d)));
+    };
+    auto product = [&](auto mask, int tile, uint32_t buf, auto beside) {
+        // the exponents of 16 positions, as read
+        auto bytes_of = [&](int f) {
+            return *(lds_i2)(bytes_at(tile) + 256 + 4u * ((8 * tile & 63) + 4 * (f < 2 ? half : 1 - half) + 2 * (f & 1)));
+        };
+        i2 bytes = bytes_of(0);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                vs[i] = pow2_of(__builtin_amdgcn_readlane(held, at + 4 * side + 2 * (f & 1) + i) >> 8);
-            i2 codes[NB];
-#pragma unroll
-            for (int d = 0; d < NB; ++d) codes[d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2)(vt ^ (32u * d)));
+        for (int f = 0; f < 4; ++f) {
+            const float vs[2] = {pow2_of(scale_byte(bytes[0])), pow2_of(scale_byte(bytes[1]))};
+            if (f < 3) {
+                read_codes(buf, f + 1);
+                bytes = bytes_of(f + 1);
+            }
+            i2 (&now)[NB] = codes[f & 1];
             if constexpr (decltype(mask)::value) {
                 // NaN among values that some rows do not see must not meet their zero weights: zeros
                 // take its place, and the rows that see it get it at the end
                 i2 nan = {0, 0};
 #pragma unroll
-                for (int d = 0; d < NB; ++d) nan |= (codes[d] & 0x7f7f7f7f) + 0x01010101;
+                for (int d = 0; d < NB; ++d) nan |= (now[d] & 0x7f7f7f7f) + 0x01010101;
                 if (__ballot(((nan[0] | nan[1]) & 0x80808080) != 0)) {
                     dirty = true;
 #pragma unroll
                     for (int d = 0; d < NB; ++d) {
-                        const i2 one = (((codes[d] & 0x7f7f7f7f) + 0x01010101) >> 7) & 0x01010101;
-                        codes[d] &= ~((one << 8) - one);
+                        const i2 one = (((now[d] & 0x7f7f7f7f) + 0x01010101) >> 7) & 0x01010101;
+                        now[d] &= ~((one << 8) - one);
                     }
                 }
             }
 #pragma unroll
             for (int d = 0; d < NB; ++d) {
-                const i2 k = codes[d];
+                const i2 k = now[d];
                 const h8 v = join(__builtin_shufflevector(two_of<false>(k[0], vs[0]), two_of<true>(k[0], vs[0]), 0, 1, 2, 3),
                                   __builtin_shufflevector(two_of<false>(k[1], vs[1]), two_of<true>(k[1], vs[1]), 0, 1, 2, 3));
                 o[d] = G::mfma(v, p[f], o[d]);
@@ -575,22 +652,22 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
         else
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();
-        if (tile >= begin && (tile + 1) % 8 == 0) turn();
-        stage(std::true_type(), tile + 2);
-        stage(std::false_type(), tile + 3);
+        stage(std::true_type(), tile + 2, ahead_of(buf));
+        stage(std::false_type(), tile + 3, buf);
     };
     int tile = begin - 1;
     while (true) {
         const int whole = full_end - 1;          // turns from full on have whole tiles on both sides
         const int stop = tile < full && full < whole ? full : end;
 #pragma unroll 1
-        for (; tile < stop; ++tile) {
+        for (; tile < stop; ++tile, buf = after(buf)) {
             start(tile);
             const bool more = tile + 1 >= mine && tile + 1 < mine_end;
-            if (more) scores(tile + 1, x);
+            if (more) scores(tile + 1, after(buf), x);
             if (tile >= mine && tile < mine_end) {
+                read_codes(buf, 0);
                 meet(tile);
-                product(std::true_type(), tile, [](int) {});
+                product(std::true_type(), tile, buf, [](int) {});
             }
             if (more) {
                 maximum(std::true_type(), tile + 1, x);
@@ -601,11 +678,12 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
         }
         if (tile >= end) break;
 #pragma unroll 1
-        for (; tile < whole; ++tile) {
+        for (; tile < whole; ++tile, buf = after(buf)) {
             start(tile);
+            read_codes(buf, 0);
             meet(tile);
-            scores(tile + 1, x);
-            product(std::false_type(), tile, [&](int n) {
+            scores(tile + 1, after(buf), x);
+            product(std::false_type(), tile, buf, [&](int n) {
                 // (the scores have settled beside the first four)
                 if (n == 3) maximum(std::false_type(), tile + 1, x);
                 if (n >= 4 && n < 12) weights(n - 4, x);
