@@ -682,13 +682,17 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
             start(tile);
             read_codes(buf, 0);
             meet(tile);
+            // (a wave in its products goes before the SIMD's other one: 1 to 3 % of a launch)
+            __builtin_amdgcn_s_setprio(2);
             scores(tile + 1, after(buf), x);
+            __builtin_amdgcn_s_setprio(1);
             product(std::false_type(), tile, buf, [&](int n) {
                 // (the scores have settled beside the first four)
                 if (n == 3) maximum(std::false_type(), tile + 1, x);
                 if (n >= 4 && n < 12) weights(n - 4, x);
                 __builtin_amdgcn_sched_barrier(0);
             });
+            __builtin_amdgcn_s_setprio(0);
             give(tile + 1);
         }
     }

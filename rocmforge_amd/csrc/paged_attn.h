@@ -395,7 +395,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
     // Codes come through registers and are written to LDS as the fp16 values that they stand for, each once:
     // fetch a tile's (this wave's share), put them a tile later.
     constexpr int LPC = D / 16, RPC = 64 / LPC, NC = CODES ? kWideKeys / (RPC * NW) : 1;
-    static_assert(!CODES || NC >= 1, "every wave has rows to fetch");
+    static_assert(!CODES || (NC >= 1 && BESIDE), "every wave has rows to fetch, and K runs a tile ahead");
     u32x4 k_codes[NC], v_codes[NC];
     int scales = 0, scales_before = 0;           // a unit's exponents, V's << 8: of this window and of the one before
     const int cr = lane / LPC, cp = lane % LPC;
@@ -465,9 +465,9 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
             put(std::false_type(), begin);
             put(std::true_type(), begin);
             fetch(std::false_type(), begin + 1);
-            if constexpr (BESIDE) put(std::false_type(), begin + 1);
+            put(std::false_type(), begin + 1);
             fetch(std::true_type(), begin + 1);
-            if constexpr (BESIDE) fetch(std::false_type(), begin + 2);
+            fetch(std::false_type(), begin + 2);
         } else {
             stage(std::false_type(), begin);
             stage(std::true_type(), begin);
@@ -649,12 +649,10 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
         if constexpr (CODES) {
             lds_barrier();                       // (this wave's values are written, and the next ones still on their way)
             if (tile < begin) return;
-            if constexpr (!BESIDE) put(std::false_type(), tile + 1);
             put(std::true_type(), tile + 1);
-            if constexpr (BESIDE) put(std::false_type(), tile + 2);
-            if constexpr (!BESIDE) fetch(std::false_type(), tile + 2);
+            put(std::false_type(), tile + 2);
             fetch(std::true_type(), tile + 2);
-            if constexpr (BESIDE) fetch(std::false_type(), tile + 3);
+            fetch(std::false_type(), tile + 3);
             return;
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
