@@ -420,23 +420,24 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     // the buffer of the tile after one's, and of the one before
     auto after = [](uint32_t buf) { return buf == (kPairStages - 1) * MAT ? 0 : buf + MAT; };
     auto ahead_of = [](uint32_t buf) { return buf == 0 ? (kPairStages - 1) * MAT : buf - MAT; };
+    auto move = [&](int tile) {
+        window = 8 * tile & ~63;
+        const int page = next;
+        address = units.address(window + lane, page, bad);
+        next = units.page_of(window + 64 + lane);
+        if (wave == 0) {
+            const int64_t at = scale_at(c, (unsigned)page >= (unsigned)c.num_pages ? 0 : page,
+                                        (8 * units.seen(window + lane)) & units.pmask, bsh) + kvh;
+            lds_dma_byte_at(__builtin_amdgcn_readfirstlane(bytes_at(tile)), (uint64_t)(c.k_scale + at));
+            lds_dma_byte_at(__builtin_amdgcn_readfirstlane(bytes_at(tile) + 256), (uint64_t)(c.v_scale + at));
+        }
+    };
     // this wave's rows of a tile of K or V into its buffer; K goes ahead and moves the window
     auto stage = [&](auto which, int tile, uint32_t buf) {
         constexpr bool values = decltype(which)::value;
         if (tile < begin || tile >= end) return;
         const int k0 = kWideKeys * tile;
-        if (!values && (8 * tile & ~63) != window) {
-            window = 8 * tile & ~63;
-            const int page = next;
-            address = units.address(window + lane, page, bad);
-            next = units.page_of(window + 64 + lane);
-            if (wave == 0) {
-                const int64_t at = scale_at(c, (unsigned)page >= (unsigned)c.num_pages ? 0 : page,
-                                            (8 * units.seen(window + lane)) & units.pmask, bsh) + kvh;
-                lds_dma_byte_at(__builtin_amdgcn_readfirstlane(bytes_at(tile)), (uint64_t)(c.k_scale + at));
-                lds_dma_byte_at(__builtin_amdgcn_readfirstlane(bytes_at(tile) + 256), (uint64_t)(c.v_scale + at));
-            }
-        }
+        if (!values && (8 * tile & ~63) != window) move(tile);
         const uint32_t dst = lds0 + (values ? kPairStages * MAT : 0) + buf, ln = lane_here(), dr = ln / 16, ds = ln % 16;
         auto rows_of = [&](auto all) {
 #pragma unroll
@@ -462,6 +463,23 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     const uint16_t* qrow = a.q + (int64_t)(s.q0 + token) * a.ld_q + (int64_t)(kvh * plan.group + head) * D + 16 * part;
 #pragma unroll
     for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const h8*>(qrow + 32 * (k >> 1) + 8 * (k & 1));
+    // The same where all of the tile is seen, a few instructions: the loop does it beside its products, where it is 2
+    // to 4 % faster than at a turn's start.
+    const int row0 = RPI * wave, unit0 = row0 >> 3;
+    const uint32_t lane_off = ((row0 & 7) + (uint32_t)lane / 16) * stride;
+    const uint32_t k_off = lane_off + 16u * ((uint32_t)lane % 16 ^ k_swizzle8<D>(row0 + lane / 16));
+    const uint32_t v_off = lane_off + 16u * ((uint32_t)lane % 16 ^ pair_swizzle(row0 + lane / 16));
+    static_assert(RPI * NW % 16 == 0, "one offset a lane for all of a wave's rows");
+    auto stage_whole = [&](auto which, int tile, uint32_t buf) {
+        constexpr bool values = decltype(which)::value;
+        if (!values && (8 * tile & ~63) != window) move(tile);
+        const uint32_t dst = lds0 + (values ? kPairStages * MAT : 0) + (uint32_t)row0 * D + buf;
+        const int unit = 8 * tile - window + unit0;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            lds_dma16(__builtin_amdgcn_readfirstlane(dst + (uint32_t)(RPI * NW * i) * D), values ? v_off : k_off,
+                      reinterpret_cast<const uint8_t*>(read_lane(address, unit + RPI * NW / 8 * i) + (values ? v_from_k : 0)));
+    };
     uint32_t buf = (uint32_t)(begin + 2) % kPairStages * MAT;    // of the tile before the first
     if (begin < end) {
         next = units.page_of((8 * begin & ~63) + lane);
@@ -484,8 +502,9 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     const uint32_t va = lds0 + kPairStages * MAT + (uint32_t)vr * D +
                         16u * (uint32_t)((8 * half + ((lane >> 4) & 1)) ^ pair_swizzle(vr)) + 8u * (uint32_t)(i16 & 1);
     // a wave's weights and maxima of a tile
-    auto weights_at = [&](int wave, int tile, uint32_t ln) { return weights0 + (uint32_t)((tile & 1) * NW + wave) * 2048 + 16u * ln; };
-    auto top_at = [&](int wave, int tile, uint32_t ln) { return tops0 + (uint32_t)((tile & 1) * NW + wave) * (4 * M) + 4u * (ln % M); };
+    const uint32_t weights_lane = weights0 + 16u * lane, tops_lane = tops0 + 4u * col;
+    auto weights_at = [&](int wave, int tile) { return weights_lane + (uint32_t)((tile & 1) * NW + wave) * 2048; };
+    auto top_at = [&](int wave, int tile) { return tops_lane + (uint32_t)((tile & 1) * NW + wave) * (4 * M); };
     f16v o[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
@@ -496,11 +515,12 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     bool dirty = false;
     h8 p[4];                                     // the weights of this half's positions, and of the other's
 
+    const uint32_t byte_lane = 4u * (4 * half + col / 8);
     // S^T of this wave's half of a tile
     auto scores = [&](int tile, uint32_t buf, f16v& x) {
         uint32_t kt = ka + buf;
         asm("" : "+v"(kt));
-        const float ks = pow2_of(scale_byte(*(lds_int)(bytes_at(tile) + 4u * ((8 * tile & 63) + 4 * half + lane_here() % M / 8))));
+        const float ks = pow2_of(scale_byte(*(lds_int)(byte_lane + bytes_at(tile) + 4u * (8 * tile & 63))));
         auto codes = [&](int j) { return *(lds_u4)(kt ^ (32u * j)); };
         constexpr int AHEAD = 2;
         u32x4 w[AHEAD + 1];
@@ -520,11 +540,10 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     };
     // Both halves' weights of a tile, under one maximum.
     auto meet = [&](int tile) {
-        const uint32_t ln = lane_here();
-        const uint32_t at = weights_at(wave ^ 1, tile, ln);
+        const uint32_t at = weights_at(wave ^ 1, tile);
 #pragma unroll
         for (int i = 0; i < 2; ++i) p[2 + i] = *(lds_h8)(at + 1024u * i);
-        const float other = *(lds_f)(top_at(wave ^ 1, tile, ln));
+        const float other = *(lds_f)(top_at(wave ^ 1, tile));
         const float most = fmaxf(own, other);
         if (__ballot(most != m || most != own || most != other)) {
             const float f = __builtin_amdgcn_exp2f(m - most), g = __builtin_amdgcn_exp2f(own - most);
@@ -578,14 +597,13 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
         l += f[0] + f[1];
     };
     auto give = [&](int tile) {
-        const uint32_t ln = lane_here();
-        const uint32_t at = weights_at(wave, tile, ln);
+        const uint32_t at = weights_at(wave, tile);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             p[i] = __builtin_bit_cast(h8, w[i]);
             *(lds_h8w)(at + 1024u * i) = p[i];
         }
-        if (ln < M) *(lds_f)(top_at(wave, tile, ln)) = own;
+        if (part == 0) *(lds_f)(top_at(wave, tile)) = own;
     };
     // O^T += V^T P^T of a tile, 16 positions at a time, this wave's half first, their codes read a turn
     // ahead (the first ones by the caller); beside(n): what is done beside the n-th product
@@ -655,6 +673,7 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
         stage(std::true_type(), tile + 2, ahead_of(buf));
         stage(std::false_type(), tile + 3, buf);
     };
+    const int seen_whole = min(end, t.hi / kWideKeys);           // (none of the loop's tiles begins in front of t.lo)
     int tile = begin - 1;
     while (true) {
         const int whole = full_end - 1;          // turns from full on have whole tiles on both sides
@@ -679,7 +698,13 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
         if (tile >= end) break;
 #pragma unroll 1
         for (; tile < whole; ++tile, buf = after(buf)) {
-            start(tile);
+            const bool fast = tile + 3 < seen_whole;
+            if (fast) {
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+                lds_barrier();
+            } else {
+                start(tile);
+            }
             read_codes(buf, 0);
             meet(tile);
             // (a wave in its products goes before the SIMD's other one: 1 to 3 % of a launch)
@@ -687,6 +712,8 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
             scores(tile + 1, after(buf), x);
             __builtin_amdgcn_s_setprio(1);
             product(std::false_type(), tile, buf, [&](int n) {
+                if (n == 0 && fast) stage_whole(std::true_type(), tile + 2, ahead_of(buf));
+                if (n == 2 && fast) stage_whole(std::false_type(), tile + 3, buf);
                 // (the scores have settled beside the first four)
                 if (n == 3) maximum(std::false_type(), tile + 1, x);
                 if (n >= 4 && n < 12) weights(n - 4, x);
