@@ -44,6 +44,40 @@ __device__ __forceinline__ void lds_dma_byte_at(uint32_t lds_dst, uint64_t at) {
 // the part through its own S-stage ring in LDS, codes as they are; they become fp16 in
 // registers, K's under its row's exponent and V's under their keys' (lane 4 i + j of a window
 // of 16 pieces holds address and exponents of piece i's unit j of 8 positions).
+// find_share's items in another order, for 17 to 64 requests: those of the longest parts first, in eighths of
+// a share, so that short ones fill the end of a launch.  48 requests of 60 to 16000 positions 49.1 us, in the
+// requests' order 52.6, 32 of 100 to 8000 24.5 and 27.3; for few requests it is 0.2 us of instructions.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool find_longest(const rf_paged_attention& a, const rf_paged_cache8& c, const Plan& p, int j,
+                                             Share& s) {
+    const Request r = request_of<ROWS, KEYS>(a, c, p, threadIdx.x & 63);
+    const int share = share_of<ROWS, KEYS>(a, c, p, r);
+    const int parts = max((int)(((unsigned)r.units + share - 1) / (unsigned)share), 1), items = r.tiles * parts;
+    const int slots = parts > 1 ? items : 0, slots_end = wave_scan(slots);
+    const int length = (int)min(8ll * r.units / ((int64_t)parts * share), 7ll);
+    for (int k = 7; k >= 0; --k) {
+        const int mine = length == k ? items : 0, end = wave_scan(mine), all = __builtin_amdgcn_readlane(end, 63);
+        if (j >= all) {
+            j -= all;
+            continue;
+        }
+        const int l = __builtin_ctzll(__ballot(end > j));
+        auto get = [l](int v) { return __builtin_amdgcn_readlane(v, l); };
+        s.b = l;
+        s.q0 = get(r.q0);
+        s.n = get(r.n);
+        s.kv = get(r.kv);
+        s.tiles = get(r.tiles);
+        s.parts = get(parts);
+        s.slot = get(slots_end - slots);
+        const int at = j - get(end - mine);
+        s.part = at / s.tiles;
+        s.tile = s.tiles - 1 - (at - s.part * s.tiles);
+        return true;
+    }
+    return false;
+}
+
 template <int D, int W, int S>
 __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const rf_paged_cache8& c, const Plan& plan,
                                              int item, uint8_t* lds) {
@@ -61,7 +95,9 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
 
     Share s;
     const int kvh = item % nkv;
-    if (!find_share<kNarrowRows, kNarrowKeys>(a, c, plan, item / nkv, false, s)) return;
+    if (!(a.num_seqs > 16 && a.num_seqs <= 64 ? find_longest<kNarrowRows, kNarrowKeys>(a, c, plan, item / nkv, s)
+                           : find_share<kNarrowRows, kNarrowKeys>(a, c, plan, item / nkv, false, s)))
+        return;
     const int rows = s.n * plan.group, r0 = kNarrowRows * s.tile;
     const Span t = span_of(plan, s, r0, min(r0 + kNarrowRows, rows) - 1, a.window);
     // the part's pieces
@@ -786,7 +822,7 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
 
 // Waves and stages of the narrow part, waves of the wide one, its workgroups a CU.  Two
 // stages a wave, so that two and more workgroups share a CU: 48 requests of 60 to 16000 positions
-// (head_dim 128) 52.4 us, with three stages and one workgroup a CU 67; at 64 a third stage is even
+// (head_dim 128, in the requests' order) 52.4 us, with three stages and one workgroup a CU 67; at 64 a third stage is even
 // (47.7 and 48.1 us, 64 requests of 2000).  At 256 two waves, for the same reason: 256 requests
 // of 600 138 us, with four waves 166.
 template <int D> struct Shape8;

@@ -103,6 +103,23 @@ def test_many_requests(rf, dev, seqs):
     Case([1] * seqs, kv, 4, 2, 64, seed=1).check()
 
 
+@pytest.mark.parametrize("seqs", [16, 17, 64, 65])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_lengths_of_all_kinds(rf, dev, seqs, d):
+    # parts of many lengths, in whichever order the kernels take them; empty requests among them
+    kv = [(i % 5 > 0) * (1 + (1237 * i * i) % 6000) for i in range(seqs)]
+    Case([min(1, n) for n in kv], kv, 8, 2, d, seed=2).check()
+
+
+@pytest.mark.parametrize("seqs", [1, 5, 64, 65])
+@pytest.mark.parametrize("window", [0, 100, 700])
+def test_prompts_of_all_kinds(rf, dev, seqs, window):
+    # tiles that grow and tiles that a window makes equal, with requests that begin somewhere and at 0
+    new = [(i % 4 < 3) * (1 + (331 * i * i + 200) % 390) for i in range(seqs)]
+    kv = [n + (i % 3) * (i * 97 % 900) for i, n in enumerate(new)]
+    Case(new, kv, 4, 2, 256, window=window, seed=3).check()
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_long_requests_beside_short_ones(rf, dev, d):
     Case([1, 1, 1, 1], [9000, 3, 20000, 250], nh=4, nkv=1, d=d).check()
