@@ -65,8 +65,8 @@ def _memory(n: int, stream):
 def add(step: LoraStep, targets, stream=None) -> None:
     """y = base + scale B (A x) for each target (a LoraTarget, or up to three of them)."""
     targets, block = _targets(targets)
-    on = [b.__dict__["_on"] if "_on" in b.__dict__ else b._device() for b in (step, *targets)]
-    handle = _stream(stream, _one_device(on))
+    on = {b.__dict__["_on"] if "_on" in b.__dict__ else b._device() for b in (step, *targets)}
+    handle = _stream(stream, _one_device(on) if len(on) > 1 else on.pop())
     lib = load()
     memory = None
     if not step.workspace:
@@ -74,5 +74,7 @@ def add(step: LoraStep, targets, stream=None) -> None:
         if n:
             memory = _memory(n, stream)
             step = LoraStep.from_buffer_copy(step)
-            step.workspace, step.workspace_bytes = memory.data_ptr(), n
+            # (past the block's own: a copy keeps no tensors)
+            ctypes.Structure.__setattr__(step, "workspace", memory.data_ptr())
+            ctypes.Structure.__setattr__(step, "workspace_bytes", n)
     _check(lib.rf_lora_add_launch(ctypes.byref(step), block, len(targets), handle), "rf_lora_add_launch")
