@@ -820,15 +820,15 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
 
 // ---- the launches -------------------------------------------------------------------------
 
-// Waves and stages of the narrow part, waves of the wide one, its workgroups a CU.  Two
+// Waves and stages of the narrow part, waves of the wide one.  Two
 // stages a wave, so that two and more workgroups share a CU: 48 requests of 60 to 16000 positions
 // (head_dim 128, in the requests' order) 52.4 us, with three stages and one workgroup a CU 67; at 64 a third stage is even
 // (47.7 and 48.1 us, 64 requests of 2000).  At 256 two waves, for the same reason: 256 requests
 // of 600 138 us, with four waves 166.
 template <int D> struct Shape8;
-template <> struct Shape8<64> { static constexpr int W = 4, S = 2, LW = 4, LS = 4, NW = 4, PER_CU = 2; };
-template <> struct Shape8<128> { static constexpr int W = 4, S = 2, LW = 4, LS = 2, NW = 4, PER_CU = 2; };
-template <> struct Shape8<256> { static constexpr int W = 2, S = 2, LW = 2, LS = 2, NW = 8, PER_CU = 1; };
+template <> struct Shape8<64> { static constexpr int W = 4, S = 2, LW = 4, LS = 4, NW = 4; };
+template <> struct Shape8<128> { static constexpr int W = 4, S = 2, LW = 4, LS = 2, NW = 4; };
+template <> struct Shape8<256> { static constexpr int W = 2, S = 2, LW = 2, LS = 2, NW = 8; };
 constexpr int kNarrowLeast8 = 4, kBesideLeast8 = 16, kWideLeast8 = 24;
 constexpr int kFewWhole8 = 16, kManyWhole8 = 32, kWideWhole8 = 32;
 template <int D>
@@ -837,8 +837,8 @@ template <int D>
 constexpr int wide8_lds() { return D == 256 ? pair8_lds<D, Shape8<D>::NW>() : 4 * kWideKeys * 2 * D; }
 template <int D>
 constexpr int wide8_rows() { return 32 * Shape8<D>::NW / (D == 256 ? 2 : 1); }
-template <int D>
-constexpr int wide8_parts() { return 256 * Shape8<D>::PER_CU; }
+static_assert(wide8_rows<64>() == kWideRows && wide8_rows<128>() == kWideRows && wide8_rows<256>() == kWideRows,
+              "the workspace's tiles");
 
 template <int D>
 __global__ __launch_bounds__(64 * Shape8<D>::W)
@@ -902,7 +902,7 @@ static void attn8_go(const rf_paged_attention& a, const rf_paged_cache8& c, hipS
                                    both ? kBesideLeast8 : kNarrowLeast8);
     Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, aim, narrow_least, inverse(aim), 0, ws};
     const int64_t wide_tiles = (packed / ROWS + std::min(some, packed / kNarrowRows)) * nkv;
-    const int wide_aim = (int)std::max<int64_t>(wide8_parts<D>() - wide_tiles / 4, wide8_parts<D>() / 4);
+    const int wide_aim = (int)std::max<int64_t>(wide_parts<D>() - wide_tiles / 4, wide_parts<D>() / 4);
     Plan wide = {group, inv, kNarrowRows, INT_MAX, wide_aim, least(kWideKeys, kWideWhole8, kWideLeast8), inverse(wide_aim), 0,
                  ws + narrow_bytes<D>() / sizeof(float)};
     // Items: every tile has a part, and there are at most as many parts more as are aimed at (each of

@@ -835,9 +835,16 @@ __device__ __forceinline__ void join_part(const rf_paged_attention& a, const C& 
     }
 }
 
+// Packed rows of a wide workgroup's tile, and the most wide parts that are aimed at: as many as fit the chip at once.
+constexpr int kWideRows = 128;
+template <int D>
+constexpr int wide_parts() { return D == 256 ? 256 : 512; }
+
 // Bytes of the narrow parts of a launch: twice as many as are aimed at; the wide ones' lie behind them.
 template <int D>
 constexpr size_t narrow_bytes() { return (size_t)2 * kNarrowParts * kNarrowRows * (D + 2) * sizeof(float); }
+template <int D>
+constexpr size_t wide_bytes() { return (size_t)2 * wide_parts<D>() * kWideRows * (D + 2) * sizeof(float); }
 
 // ---- what the launchers refuse -------------------------------------------------------------
 

@@ -261,17 +261,17 @@ __device__ __forceinline__ void narrow_part(const rf_paged_attention& a, const r
 // that one's chain of loads runs beside the other's loop, for many tiles and beside wide
 // items (256 requests of 600 positions 148 -> 126 us; one of 2000 9.0 -> 9.5).
 template <int D> struct Shape;
-template <> struct Shape<64> { static constexpr int W = 4, S = 4, LW = 4, LS = 2, NW = 4, M = 32, PER_CU = 2; };
-template <> struct Shape<128> { static constexpr int W = 4, S = 2, LW = 2, LS = 2, NW = 4, M = 32, PER_CU = 2; };
-template <> struct Shape<256> { static constexpr int W = 2, S = 2, LW = 1, LS = 2, NW = 8, M = 16, PER_CU = 1; };
+template <> struct Shape<64> { static constexpr int W = 4, S = 4, LW = 4, LS = 2, NW = 4, M = 32; };
+template <> struct Shape<128> { static constexpr int W = 4, S = 2, LW = 2, LS = 2, NW = 4, M = 32; };
+template <> struct Shape<256> { static constexpr int W = 2, S = 2, LW = 1, LS = 2, NW = 8, M = 16; };
 template <int D>
 constexpr int narrow_lds(int w, int s) { return w * s * 2 * kNarrowKeys * 2 * D; }
 template <int D>
 constexpr int wide_lds() { return 4 * kWideKeys * 2 * D; }
 template <int D>
 constexpr int wide_rows() { return Shape<D>::M * Shape<D>::NW; }
-template <int D>
-constexpr int wide_parts() { return 256 * Shape<D>::PER_CU; }
+static_assert(wide_rows<64>() == kWideRows && wide_rows<128>() == kWideRows && wide_rows<256>() == kWideRows,
+              "the workspace's tiles");
 
 template <int D, bool LIGHT>
 __global__ __launch_bounds__(64 * (LIGHT ? Shape<D>::LW : Shape<D>::W))
@@ -311,16 +311,12 @@ __global__ __launch_bounds__(256) void rf_paged_attn_join_kernel(const rf_paged_
 
 }  // namespace rf
 
-// Bytes of the wide parts of a launch.
-template <int D>
-static constexpr size_t wide_bytes() { return (size_t)2 * rf::wide_parts<D>() * rf::wide_rows<D>() * (D + 2) * sizeof(float); }
-
 extern "C" size_t rf_paged_attention_workspace_bytes(int num_heads, int num_kv_heads, int head_dim) {
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0) return 0;
     switch (head_dim) {
-    case 64: return rf::narrow_bytes<64>() + wide_bytes<64>();
-    case 128: return rf::narrow_bytes<128>() + wide_bytes<128>();
-    case 256: return rf::narrow_bytes<256>() + wide_bytes<256>();
+    case 64: return rf::narrow_bytes<64>() + rf::wide_bytes<64>();
+    case 128: return rf::narrow_bytes<128>() + rf::wide_bytes<128>();
+    case 256: return rf::narrow_bytes<256>() + rf::wide_bytes<256>();
     default: return 0;
     }
 }
