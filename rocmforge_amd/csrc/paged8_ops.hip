@@ -194,7 +194,7 @@ constexpr int kReadRows = 4;                     // at most
 __global__ __launch_bounds__(256) void rf_paged_read8_kernel(const rf_paged_read s, const rf_paged_cache8 c, int per,
                                                             uint32_t inv) {
     __shared__ int64_t codes_at[kReadRows], scales_at[kReadRows];
-    const int tid = threadIdx.x, lane = tid & 63, r0 = per * blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, r0 = per * (int)(blockIdx.x + blockIdx.y * gridDim.x);
     const int bsh = block_shift(c), dsh = __ffs(c.head_dim) - 4;         // pieces of 8 a head
     const int pieces = c.num_kv_heads << dsh;
     if (tid < 64) {
@@ -334,7 +334,8 @@ extern "C" hipError_t rf_paged_read8_launch(const rf_paged_read* read, const rf_
     // few rows in twos (640 rows of 8 heads of 128 3.5 us, in fours 3.7, in sixteens 6.4), many in fours (48
     // ragged requests 210 us, in sixteens 214)
     const int per = s.rows <= 4096 ? 2 : rf::kReadRows;
-    hipLaunchKernelGGL(rf::rf_paged_read8_kernel, dim3((unsigned)((s.rows + per - 1) / per)), dim3(256), 0, stream, s,
-                       *cache, per, inv);
+    const unsigned blocks = (unsigned)((s.rows + per - 1) / per), wide = std::min(blocks, 1u << 20);
+    hipLaunchKernelGGL(rf::rf_paged_read8_kernel, dim3(wide, (blocks + wide - 1) / wide), dim3(256), 0, stream, s, *cache,
+                       per, inv);
     return hipGetLastError();
 }

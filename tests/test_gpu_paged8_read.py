@@ -163,3 +163,22 @@ def test_replays(rf, dev):
             got = got.double()
             # (entries of the tables behind a request's pages name none)
             assert bool(((got == want) | (got.isnan() & want.isnan())).all())
+
+
+def test_more_rows_than_one_dimension_of_a_launch_has(rf, dev):
+    # 2^26 rows and some, all of the same page
+    rows, d = (1 << 26) + 5000, 64
+    p = E.Pages(1, 1024, 1, d)
+    g = P.gen(3)
+    p.hold(*[torch.randn(1, 1024, 1, d, generator=g, device=P.DEV) for _ in range(2)])
+    blocks = -(-rows // 1024)
+    tab, starts = torch.zeros(1, blocks, dtype=torch.int32, device=P.DEV), P.ints([0, rows])
+    out = torch.full((rows, d), 7.0, dtype=torch.float16, device=P.DEV)
+    print(f"[gpu] read8 rows {rows}", flush=True)
+    paged.read8(paged.PagedRead(k=out, block_tables=tab, row_start=starts, ld_out=d, num_seqs=1, max_blocks=blocks,
+                                rows=rows), p.cache())
+    torch.cuda.synchronize()
+    page = p.values()[0].half().view(1024, d)
+    for at in (0, (1 << 24) - 1024, (1 << 26) - 1024, (1 << 26) + 3072):
+        assert torch.equal(out[at:at + 1024], page), at
+    assert torch.equal(out[-(rows % 1024):], page[:rows % 1024])
