@@ -117,15 +117,21 @@ __device__ __forceinline__ bool lora_item(const rf_lora& s, int pieces, LoraItem
 
 // A x over [k0, k1) of the tile's rows into part [wave][row][rank], a share each of the first waves; returns how
 // many.  Few rows: dot products.  A wave takes 256 k of 16 ranks, a lane four of them, so that a row of A is
-// read 512 bytes at a time; the waves are spread over the blocks of ranks, then over k.
-template <bool X16, int RB, int MB, int NW, int HS>
+// read 512 bytes at a time; the waves are spread over the blocks of ranks, then over k.  AHEAD: loads are a turn ahead
+// where there are more than two (64 single tokens on 40 adapters 44.4 -> 42.3 us, 200 90 -> 85; one token of rank 64, of
+// two turns, 14.8 -> 15.3; eight waves do not have the registers).
+template <bool X16, bool AHEAD, int RB, int MB, int NW, int HS>
 __device__ __forceinline__ int lora_dots(const rf_lora& s, const uint16_t* a, const LoraItem<MB>& w, int k0, int k1,
                                          float (*part)[16 * MB][HS]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rank = w.rank;
-    constexpr int R = kFewRows;
     const int ranks = (rank + 15) / 16, slices = min(max(NW / ranks, 1), (k1 - k0 + 255) / 256);
     const int slice = ranks <= NW ? wave / ranks : 0;
     if (slice >= slices) return slices;
+    constexpr int R = kFewRows;
+    struct Turn {
+        h4 v[16];
+        f4 x[R];
+    };
 #pragma unroll 1
     for (int r0 = 16 * (ranks <= NW ? wave - slice * ranks : wave); r0 < rank; r0 += 16 * NW) {
         float acc[R][16];
@@ -133,29 +139,30 @@ __device__ __forceinline__ int lora_dots(const rf_lora& s, const uint16_t* a, co
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[r][i] = 0.0f;
-        for (int kw = k0 + 256 * slice; kw < k1; kw += 256 * slices) {
-            const int k = kw + 4 * lane, kk = min(k, k1 - 4);
-            h4 v[16];
+        // (behind the end loads are of the last elements, and A is zero)
+        auto load = [&](int kw, Turn& t) {
+            const int kk = min(kw + 4 * lane, k1 - 4);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                v[i] = *reinterpret_cast<const h4*>(a + (int64_t)min(r0 + i, rank - 1) * s.in_dim + kk);
-            f4 x[R];
+                t.v[i] = *reinterpret_cast<const h4*>(a + (int64_t)min(r0 + i, rank - 1) * s.in_dim + kk);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const int64_t at = (int64_t)__builtin_amdgcn_readlane((int)w.row[0], r) * s.ld_x + kk;
                 if constexpr (X16) {
                     const h4 y = *reinterpret_cast<const h4*>(static_cast<const uint16_t*>(s.x) + at);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[r][i] = (float)y[i];
+                    for (int i = 0; i < 4; ++i) t.x[r][i] = (float)y[i];
                 } else {
-                    x[r] = *reinterpret_cast<const f4*>(static_cast<const float*>(s.x) + at);
+                    t.x[r] = *reinterpret_cast<const f4*>(static_cast<const float*>(s.x) + at);
                 }
             }
-            if (k >= k1) {
+        };
+        auto multiply = [&](int kw, Turn& t) {
+            if (kw + 4 * lane >= k1) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = h4{0, 0, 0, 0};
+                for (int i = 0; i < 16; ++i) t.v[i] = h4{0, 0, 0, 0};
 #pragma unroll
-                for (int r = 0; r < R; ++r) x[r] = f4{0, 0, 0, 0};
+                for (int r = 0; r < R; ++r) t.x[r] = f4{0, 0, 0, 0};
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
@@ -163,8 +170,33 @@ __device__ __forceinline__ int lora_dots(const rf_lora& s, const uint16_t* a, co
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[r][i] = __builtin_fmaf((float)v[i][e], x[r][e], acc[r][i]);
+                    for (int e = 0; e < 4; ++e) acc[r][i] = __builtin_fmaf((float)t.v[i][e], t.x[r][e], acc[r][i]);
             }
+        };
+        const int by = 256 * slices;
+        int kw = k0 + 256 * slice;
+        Turn t0;
+        if constexpr (AHEAD) {
+            if (kw + 2 * by < k1) {
+                Turn t1;
+                load(kw, t0);
+                __builtin_amdgcn_sched_barrier(0);
+                for (; kw < k1; kw += 2 * by) {
+                    load(kw + by, t1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    multiply(kw, t0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    load(kw + 2 * by, t0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    multiply(kw + by, t1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        for (; kw < k1; kw += by) {
+            load(kw, t0);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(kw, t0);
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -417,7 +449,7 @@ __global__ __launch_bounds__(64 * NW) void rf_lora_whole_kernel(const rf_lora s,
     const int nb0 = w.piece * each, nb1 = min(nb0 + each, blocks);
     if (nb0 >= nb1) return;
     if (w.rank == 0) return lora_copy<NW>(g, w, nb0, nb1);
-    const int slices = lora_dots<X16, RB, 1, NW, HS>(s, g.a + w.id * g.a_stride, w, 0, s.in_dim, part);
+    const int slices = lora_dots<X16, false, RB, 1, NW, HS>(s, g.a + w.id * g.a_stride, w, 0, s.in_dim, part);
     lds_barrier();
     const int r = min((int)threadIdx.x & 15, w.rows - 1);
     lora_up<RB, NW>(s, g, w, nb0, nb1, slices, [&](int k, int j) { return *reinterpret_cast<const f4*>(&part[k][r][j]); });
@@ -438,7 +470,7 @@ __global__ __launch_bounds__(64 * NW) void rf_lora_down_kernel(const rf_lora s, 
         for (int m = 0; m < MB; ++m) rows[16 * m + threadIdx.x] = (int)w.row[m];
     const int k0 = w.piece * each, k1 = min(k0 + each, s.in_dim);
     const uint16_t* a = g.a + w.id * g.a_stride;
-    const int parts = w.rows <= kFewRows ? lora_dots<X16, RB, MB, NW, HS>(s, a, w, k0, k1, part)
+    const int parts = w.rows <= kFewRows ? lora_dots<X16, true, RB, MB, NW, HS>(s, a, w, k0, k1, part)
                                          : lora_down<X16, RB, MB, NW, U, HS>(s, a, w, k0, k1, part);
     lds_barrier();
     float* to = sums + (int64_t)(blockIdx.y * slices + w.piece) * s.rows * (16 * RB);
