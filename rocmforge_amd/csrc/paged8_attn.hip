@@ -824,11 +824,11 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
 // stages a wave, so that two and more workgroups share a CU: 48 requests of 60 to 16000 positions
 // (head_dim 128, in the requests' order) 52.4 us, with three stages and one workgroup a CU 67; at 64 a third stage is even
 // (47.7 and 48.1 us, 64 requests of 2000).  At 256 two waves, for the same reason: 256 requests
-// of 600 138 us, with four waves 166.
+// of 600 138 us, with four waves 166.  HW: waves of a workgroup by itself on its CU, for a few hundred positions.
 template <int D> struct Shape8;
-template <> struct Shape8<64> { static constexpr int W = 4, S = 2, LW = 4, LS = 4, NW = 4; };
-template <> struct Shape8<128> { static constexpr int W = 4, S = 2, LW = 4, LS = 2, NW = 4; };
-template <> struct Shape8<256> { static constexpr int W = 2, S = 2, LW = 2, LS = 2, NW = 8; };
+template <> struct Shape8<64> { static constexpr int W = 4, S = 2, HW = 8, LW = 4, LS = 4, NW = 4; };
+template <> struct Shape8<128> { static constexpr int W = 4, S = 2, HW = 8, LW = 4, LS = 2, NW = 4; };
+template <> struct Shape8<256> { static constexpr int W = 2, S = 2, HW = 4, LW = 2, LS = 2, NW = 8; };
 constexpr int kNarrowLeast8 = 4, kBesideLeast8 = 16, kWideLeast8 = 24;
 constexpr int kFewWhole8 = 16, kManyWhole8 = 32, kWideWhole8 = 32;
 template <int D>
@@ -840,10 +840,10 @@ constexpr int wide8_rows() { return 32 * Shape8<D>::NW / (D == 256 ? 2 : 1); }
 static_assert(wide8_rows<64>() == kWideRows && wide8_rows<128>() == kWideRows && wide8_rows<256>() == kWideRows,
               "the workspace's tiles");
 
-template <int D>
-__global__ __launch_bounds__(64 * Shape8<D>::W)
+template <int D, int W>
+__global__ __launch_bounds__(64 * W)
 void rf_paged8_attn_narrow_kernel(const rf_paged_attention a, const rf_paged_cache8 c, const Plan plan) {
-    constexpr int W = Shape8<D>::W, S = Shape8<D>::S;
+    constexpr int S = Shape8<D>::S;
     __shared__ __align__(1024) uint8_t lds[narrow8_lds<D>(W, S)];
     narrow8_part<D, W, S>(a, c, plan, (int)(blockIdx.x + blockIdx.y * gridDim.x), lds);
 }
@@ -898,7 +898,12 @@ static void attn8_go(const rf_paged_attention& a, const rf_paged_cache8& c, hipS
     // 20 of 4000 49.1 and 44.1, 48 of 60 to 16000 56.9, 52.4 and, at 512, 57.8.
     const int aim = tiles < 64 ? 256 : 400;
     const auto least = [&](int keys, int whole, int cut) { return positions <= whole * keys ? whole : cut; };
-    const int narrow_least = least(kNarrowKeys, both || tiles >= 256 ? kManyWhole8 : kFewWhole8,
+    // Two pieces a wave of a heavy workgroup, three from 64 tiles on: uncut by these, where there are no more tiles than
+    // CUs.  us (head_dim 128), uncut by 8 waves / cut by 4: one request of 100 positions 5.7 / 5.3, of 300 6.8 / 7.4, of 500
+    // 7.8 / 8.7, of 640 9.0 / 8.8, of 900 10.5 / 8.6; 8 of 640 9.7 / 11.2, 24 12.1 / 15.8, but 32 of 500 13.4 / 12.2.
+    const int most = (tiles < 64 ? 2 : 3) * Shape8<D>::HW;
+    const bool heavy = !both && tiles < 256 && positions > 6 * kNarrowKeys && positions <= most * kNarrowKeys;
+    const int narrow_least = least(kNarrowKeys, heavy ? most : both || tiles >= 256 ? kManyWhole8 : kFewWhole8,
                                    both ? kBesideLeast8 : kNarrowLeast8);
     Plan narrow = {group, inv, 0, both ? kNarrowRows : INT_MAX, aim, narrow_least, inverse(aim), 0, ws};
     const int64_t wide_tiles = (packed / ROWS + std::min(some, packed / kNarrowRows)) * nkv;
@@ -923,8 +928,10 @@ static void attn8_go(const rf_paged_attention& a, const rf_paged_cache8& c, hipS
     const dim3 grid(std::min(total, 1u << 20), (total + (1u << 20) - 1) >> 20);
     if (both)
         hipLaunchKernelGGL(rf_paged8_attn_mixed_kernel<D>, grid, dim3(64 * Shape8<D>::NW), 0, stream, a, c, wide, narrow);
+    else if (heavy)
+        hipLaunchKernelGGL((rf_paged8_attn_narrow_kernel<D, Shape8<D>::HW>), grid, dim3(64 * Shape8<D>::HW), 0, stream, a, c, narrow);
     else
-        hipLaunchKernelGGL(rf_paged8_attn_narrow_kernel<D>, grid, dim3(64 * Shape8<D>::W), 0, stream, a, c, narrow);
+        hipLaunchKernelGGL((rf_paged8_attn_narrow_kernel<D, Shape8<D>::W>), grid, dim3(64 * Shape8<D>::W), 0, stream, a, c, narrow);
     const int wide_blocks = (int)wide_joins * (ROWS / kJoinRows);
     if (wide_joins + narrow_joins > 0)
         hipLaunchKernelGGL(rf_paged8_attn_join_kernel<D>, dim3((unsigned)(wide_blocks + narrow_joins)), dim3(256), 0,
