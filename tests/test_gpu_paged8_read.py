@@ -179,6 +179,6 @@ def test_more_rows_than_one_dimension_of_a_launch_has(rf, dev):
                                 rows=rows), p.cache())
     torch.cuda.synchronize()
     page = p.values()[0].half().view(1024, d)
-    for at in (0, (1 << 24) - 1024, (1 << 26) - 1024, (1 << 26) + 3072):
+    for at in (0, (1 << 24) - 1024, (1 << 26) - 1024, (1 << 26) + 2048):
         assert torch.equal(out[at:at + 1024], page), at
     assert torch.equal(out[-(rows % 1024):], page[:rows % 1024])
