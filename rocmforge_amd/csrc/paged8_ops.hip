@@ -11,18 +11,105 @@ namespace rf {
 
 // ---- the rotary step into the pages --------------------------------------------------------
 //
-// A block's exponent needs all its new rows, so a workgroup takes whole runs of rows that
-// share a block: those that start among 16 rows (32 at head_dim 64), up to 15 more with the
-// last one's (a prompt's 16, or 16 requests' single tokens).  D / 8 lanes a row, 8 elements a
-// lane, the rows of a head at once and one head after the other; a lane's four pairs turn by
-// the same angles in all heads, so it takes their cosines once.  A run's largest value meets
-// through LDS.  Where the runs have more rows than the threads take, the last one goes by itself.
+// Queries go a row at a time, their loads two heads ahead (4000 rows of 32 + 16 heads 36 us, 3.9 TB/s; a head ahead,
+// under the barriers of keys and values, 39).  Of keys and values a block's exponent needs all its new rows,
+// so a workgroup takes whole runs of rows that share a block: those that start among 16 rows (32 at head_dim 64), up
+// to 15 more with the last one's (a prompt's 16, or 16 requests' single tokens).  D / 8 lanes a row, 8 elements a
+// lane, the rows of a head at once and one head after the other; a lane's four pairs turn by the same angles in all
+// heads, so it takes their cosines once.  A run's largest value meets through LDS.  Where the runs have more rows than
+// the threads take, the last one goes by itself.
 constexpr int kRunRows = 16;                     // the most rows of a run
 template <int D>
 constexpr int rope8_threads() { return D == 256 ? 512 : 256; }
 template <int D>
 constexpr int start_rows() { return rope8_threads<D>() / (D / 8); }
 
+// A lane's eight elements of a row, of any head: from e0 on and from e1 on four each, which make up pairs.
+template <int D, bool NEOX>
+struct Rope8 {
+    static constexpr int LPH = D / 8;
+    int u, e0, e1;
+    bool turned;
+    float2 cs[4];                                // of its four pairs
+    __device__ __forceinline__ explicit Rope8(const rf_paged_rope& s) : u(threadIdx.x % LPH), turned(u < s.rot_dim / 8) {
+        e0 = NEOX && turned ? 4 * u : 8 * u;
+        e1 = NEOX && turned ? s.rot_dim / 2 + 4 * u : e0 + 4;
+    }
+    __device__ __forceinline__ void angles(const rf_paged_rope& s, int r) {
+        if (!turned) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const double turn = (double)s.positions[r] * s.turns[4 * u + i];
+            float sn, co;
+            sincospif(2.0f * (float)(turn - rint(turn)), &sn, &co);
+            cs[i] = make_float2(co * s.attn_factor, sn * s.attn_factor);
+        }
+    }
+    // (every lane of a row takes the same way, and rows do not share lanes)
+    __device__ __forceinline__ void norm(float (&x)[8], float4 w0, float4 w1, float eps) const {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = __fmaf_rn(x[i], x[i], ss);
+        ss = xor_sum<LPH / 2, 1>(ss);
+        const float inv = 1.0f / sqrtf(ss * (1.0f / D) + eps);
+        const float by[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * by[i];
+    }
+    __device__ __forceinline__ void turn(float (&x)[8]) const {
+        if (!turned) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            constexpr int P = NEOX ? 1 : 2, Q = NEOX ? 4 : 1;
+            const float f = x[P * i], g = x[P * i + Q];
+            x[P * i] = __fmaf_rn(f, cs[i].x, -(g * cs[i].y));
+            x[P * i + Q] = __fmaf_rn(f, cs[i].y, g * cs[i].x);
+        }
+    }
+};
+
+// The query heads [h0, h1) of the workgroup's rows.
+template <int D, bool NEOX>
+__device__ __forceinline__ void rope8_queries(const rf_paged_rope& s, int slots, int h0, int h1) {
+    constexpr int AHEAD = 2;                     // heads whose loads are on their way
+    Rope8<D, NEOX> t(s);
+    const int r = start_rows<D>() * blockIdx.x + threadIdx.x / (D / 8);
+    if (r >= s.rows || (unsigned)s.slots[r] >= (unsigned)slots) return;
+    const float* src = s.q + (int64_t)r * s.ld_q;
+    uint16_t* dst = s.q16 + (int64_t)r * s.ld_q16;
+    float4 a[AHEAD], b[AHEAD];
+    auto load = [&](int h, int k) {
+        const float* from = src + (int64_t)min(h, h1 - 1) * D;
+        a[k] = *reinterpret_cast<const float4*>(from + t.e0);
+        b[k] = *reinterpret_cast<const float4*>(from + t.e1);
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) load(h0 + k, k);
+    float4 w0 = {1, 1, 1, 1}, w1 = w0;           // the norm's weights
+    if (s.q_norm != nullptr) {
+        w0 = *reinterpret_cast<const float4*>(s.q_norm + t.e0);
+        w1 = *reinterpret_cast<const float4*>(s.q_norm + t.e1);
+    }
+    t.angles(s, r);
+    for (int h = h0; h < h1; h += AHEAD)
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (h + k >= h1) return;
+            float x[8] = {a[k].x, a[k].y, a[k].z, a[k].w, b[k].x, b[k].y, b[k].z, b[k].w};
+            load(h + k + AHEAD, k);
+            if (s.q_norm != nullptr) t.norm(x, w0, w1, s.eps);
+            t.turn(x);
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                o[i] = (uint32_t)f16_bits_rn(x[2 * i]) | ((uint32_t)f16_bits_rn(x[2 * i + 1]) << 16);
+            uint16_t* to = dst + (int64_t)(h + k) * D;
+            *reinterpret_cast<uint2*>(to + t.e0) = make_uint2(o[0], o[1]);
+            *reinterpret_cast<uint2*>(to + t.e1) = make_uint2(o[2], o[3]);
+        }
+}
+
+// per: heads a workgroup; the grid's rows are those of q, then of k and v.
 template <int D, bool NEOX>
 __global__ __launch_bounds__(rope8_threads<D>(), 5)
 void rf_paged_rope8_kernel(const rf_paged_rope s, const rf_paged_cache8 c, int per) {
@@ -30,8 +117,13 @@ void rf_paged_rope8_kernel(const rf_paged_rope s, const rf_paged_cache8 c, int p
     static_assert(ROWS >= kRunRows && ROWS + kRunRows < 64, "the threads take a run, a wave's ballot all rows");
     __shared__ float tops[2][ROWS];              // a row's largest finite value
     __shared__ int olds[2][ROWS];                // the exponent before, at a run's first row
-    const int tid = threadIdx.x, lane = tid & 63, u = tid % LPH;
-    const int bsh = block_shift(c), slots = c.num_pages * c.page_size, psh = __ffs(c.page_size) - 1;
+    const int slots = c.num_pages * c.page_size, q_groups = (s.num_heads + per - 1) / per;
+    if ((int)blockIdx.y < q_groups) {
+        const int h0 = blockIdx.y * per;
+        return rope8_queries<D, NEOX>(s, slots, h0, min(h0 + per, s.num_heads));
+    }
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int bsh = block_shift(c), psh = __ffs(c.page_size) - 1;
     const int r0 = ROWS * blockIdx.x;
     // a run: rows one behind the other with rising slots of one block
     const int at = r0 + lane;
@@ -46,10 +138,9 @@ void rf_paged_rope8_kernel(const rf_paged_rope s, const rf_paged_cache8 c, int p
     if (a2 <= a0) return;
     const int a1 = a2 - a0 <= ROWS ? a2 : last;
 
-    const int half = s.rot_dim / 2, heads = s.num_heads + 2 * c.num_kv_heads;
-    const bool turned = u < s.rot_dim / 8;
-    const int e0 = NEOX && turned ? 4 * u : 8 * u, e1 = NEOX && turned ? half + 4 * u : e0 + 4;
-    const int h0 = blockIdx.y * per, h1 = min(h0 + per, heads);
+    Rope8<D, NEOX> t(s);
+    const int u = t.u, nkv = c.num_kv_heads;     // heads: k's, then v's
+    const int h0 = ((int)blockIdx.y - q_groups) * per, h1 = min(h0 + per, 2 * nkv);
     int buf = 0;
     for (int begin = a0, n = a1 - a0; n > 0; begin += n, n = a2 - begin) {
         const int first = r0 + begin;
@@ -58,14 +149,10 @@ void rf_paged_rope8_kernel(const rf_paged_rope s, const rf_paged_cache8 c, int p
         float4 a, b;
         auto load = [&](int h) {
             const int64_t r = first + row;
-            const float* src = h < s.num_heads ? s.q + r * s.ld_q + (int64_t)h * D
-                               : h < s.num_heads + c.num_kv_heads
-                                   ? s.k + r * s.ld_k + (int64_t)(h - s.num_heads) * D
-                                   : s.v + r * s.ld_v + (int64_t)(h - s.num_heads - c.num_kv_heads) * D;
-            a = *reinterpret_cast<const float4*>(src + e0);
-            b = *reinterpret_cast<const float4*>(src + e1);
+            const float* src = h < nkv ? s.k + r * s.ld_k + (int64_t)h * D : s.v + r * s.ld_v + (int64_t)(h - nkv) * D;
+            a = *reinterpret_cast<const float4*>(src + t.e0);
+            b = *reinterpret_cast<const float4*>(src + t.e1);
         };
-        float2 cs[4];
         const int r = first + row, bit = begin + row;
         if (row < n) slot = s.slots[r];
         const bool live = (unsigned)slot < (unsigned)slots;
@@ -74,75 +161,38 @@ void rf_paged_rope8_kernel(const rf_paged_rope s, const rf_paged_cache8 c, int p
             run = 63 - __builtin_clzll(leads & ((2ull << bit) - 1)) - begin;
             end = min(bit + 1 + __builtin_ctzll(leads >> (bit + 1)) - begin, n);
             from = s.slots[first + run] & ((1 << bsh) - 1);
-            if (turned)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const double turn = (double)s.positions[r] * s.turns[4 * u + i];
-                    float sn, co;
-                    sincospif(2.0f * (float)(turn - rint(turn)), &sn, &co);
-                    cs[i] = make_float2(co * s.attn_factor, sn * s.attn_factor);
-                }
+            if (h0 < nkv) t.angles(s, r);
         }
         float4 w0 = {1, 1, 1, 1}, w1 = w0;       // the norm's weights
+        if (s.k_norm != nullptr && h0 < nkv) {
+            w0 = *reinterpret_cast<const float4*>(s.k_norm + t.e0);
+            w1 = *reinterpret_cast<const float4*>(s.k_norm + t.e1);
+        }
         for (int h = h0; h < h1; ++h) {
-            const bool is_q = h < s.num_heads, is_v = h >= s.num_heads + c.num_kv_heads;
-            const int kvh = is_v ? h - s.num_heads - c.num_kv_heads : h - s.num_heads;
-            const float* w = is_v ? nullptr : is_q ? s.q_norm : s.k_norm;
-            if (w != nullptr && (h == h0 || h == s.num_heads)) {
-                w0 = *reinterpret_cast<const float4*>(w + e0);
-                w1 = *reinterpret_cast<const float4*>(w + e1);
-            }
-            uint8_t* codes = (is_v ? c.v : c.k) + (is_q ? 0 : kvh) * c.head_stride;
-            uint8_t* scales = (is_v ? c.v_scale : c.k_scale) + (is_q ? 0 : kvh);
-            float y[8];
+            const bool is_v = h >= nkv;
+            const int kvh = is_v ? h - nkv : h;
+            uint8_t* codes = (is_v ? c.v : c.k) + kvh * c.head_stride;
+            uint8_t* scales = (is_v ? c.v_scale : c.k_scale) + kvh;
+            float x[8];
             if (live) {
-                float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                const float loaded[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = loaded[i];
                 if (h + 1 < h1) load(h + 1);
-                // (every lane of a row takes the same way, and rows do not share lanes)
-                if (w != nullptr) {
-                    float ss = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) ss = __fmaf_rn(x[i], x[i], ss);
-                    ss = xor_sum<LPH / 2, 1>(ss);
-                    const float inv = 1.0f / sqrtf(ss * (1.0f / D) + s.eps);
-                    const float by[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * by[i];
+                if (!is_v) {
+                    if (s.k_norm != nullptr) t.norm(x, w0, w1, s.eps);
+                    t.turn(x);
                 }
-                if (!is_v && turned) {
+                float top = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 t = cs[i];
-                        constexpr int P = NEOX ? 1 : 2, Q = NEOX ? 4 : 1;
-                        const float f = x[P * i], g = x[P * i + Q];
-                        x[P * i] = __fmaf_rn(f, t.x, -(g * t.y));
-                        x[P * i + Q] = __fmaf_rn(f, t.y, g * t.x);
-                    }
-                }
-                if (is_q) {
-                    uint16_t* dst = s.q16 + (int64_t)(first + row) * s.ld_q16 + (int64_t)h * D;
-                    uint32_t o[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        o[i] = (uint32_t)f16_bits_rn(x[2 * i]) | ((uint32_t)f16_bits_rn(x[2 * i + 1]) << 16);
-                    *reinterpret_cast<uint2*>(dst + e0) = make_uint2(o[0], o[1]);
-                    *reinterpret_cast<uint2*>(dst + e1) = make_uint2(o[2], o[3]);
-                } else {
-                    float top = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        y[i] = x[i];
-                        top = fmaxf(top, nan_unless_finite(x[i]) == 0.0f ? fabsf(x[i]) : 0.0f);
-                    }
-                    top = xor_max<LPH / 2, 1>(top);
-                    if (u == 0) {
-                        tops[buf][row] = top;
-                        // (one lane reads it, and writes it again below)
-                        if (run == row) olds[buf][row] = scale_byte(scales[(int64_t)(slot >> bsh) * c.num_kv_heads]);
-                    }
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, nan_unless_finite(x[i]) == 0.0f ? fabsf(x[i]) : 0.0f);
+                top = xor_max<LPH / 2, 1>(top);
+                if (u == 0) {
+                    tops[buf][row] = top;
+                    // (one lane reads it, and writes it again below)
+                    if (run == row) olds[buf][row] = scale_byte(scales[(int64_t)(slot >> bsh) * nkv]);
                 }
             }
-            if (is_q) continue;
             __syncthreads();                     // (of the other buffer's readers all have passed the barrier before)
             if (live) {
                 float top = 0.0f;
@@ -152,9 +202,9 @@ void rf_paged_rope8_kernel(const rf_paged_rope s, const rf_paged_cache8 c, int p
                 const float by = pow2_of(254 - e);
                 uint8_t* dst = codes + (int64_t)(slot >> psh) * c.page_stride +
                                (int64_t)(slot & (c.page_size - 1)) * c.row_stride;
-                const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
-                *reinterpret_cast<uint32_t*>(dst + e0) = codes_of(lo, by);
-                *reinterpret_cast<uint32_t*>(dst + e1) = codes_of(hi, by);
+                const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
+                *reinterpret_cast<uint32_t*>(dst + t.e0) = codes_of(lo, by);
+                *reinterpret_cast<uint32_t*>(dst + t.e1) = codes_of(hi, by);
                 if (run == row) {
                     if (from > 0 && e > old) {
                         // the block's rows before, two at a time (more cost registers, and so the prompts time)
@@ -165,19 +215,19 @@ void rf_paged_rope8_kernel(const rf_paged_rope s, const rf_paged_cache8 c, int p
 #pragma unroll
                             for (int i = 0; i < AT_ONCE; ++i) {
                                 const uint8_t* src = dst - min(i0 + i, from) * c.row_stride;
-                                was[i][0] = *reinterpret_cast<const uint32_t*>(src + e0);
-                                was[i][1] = *reinterpret_cast<const uint32_t*>(src + e1);
+                                was[i][0] = *reinterpret_cast<const uint32_t*>(src + t.e0);
+                                was[i][1] = *reinterpret_cast<const uint32_t*>(src + t.e1);
                             }
 #pragma unroll
                             for (int i = 0; i < AT_ONCE; ++i) {
                                 if (i0 + i > from) continue;
                                 uint8_t* to = dst - (i0 + i) * c.row_stride;
-                                *reinterpret_cast<uint32_t*>(to + e0) = recoded(was[i][0], less);
-                                *reinterpret_cast<uint32_t*>(to + e1) = recoded(was[i][1], less);
+                                *reinterpret_cast<uint32_t*>(to + t.e0) = recoded(was[i][0], less);
+                                *reinterpret_cast<uint32_t*>(to + t.e1) = recoded(was[i][1], less);
                             }
                         }
                     }
-                    if (u == 0) scales[(int64_t)(slot >> bsh) * c.num_kv_heads] = (uint8_t)e;
+                    if (u == 0) scales[(int64_t)(slot >> bsh) * nkv] = (uint8_t)e;
                 }
             }
             buf ^= 1;
@@ -300,11 +350,11 @@ extern "C" hipError_t rf_paged_rope_write8_launch(const rf_paged_rope* step, con
         return hipErrorInvalidValue;
     const int heads = s.num_heads + 2 * cache->num_kv_heads, starts = cache->head_dim == 64 ? rf::start_rows<64>() : rf::start_rows<128>();
     const int chunks = (s.rows + starts - 1) / starts;
-    // as many heads a workgroup as leave sixteen of them a CU, so that cosines are shared: 4000 rows
-    // of 48 heads 36 us, with eight a CU 40, with one head a workgroup 48
+    // as many heads a workgroup as leave some sixteen of them a CU, so that cosines are shared: 4000 rows
+    // of 48 heads and their read back 42.0 us, with eight a CU 46.7; 1500 rows 19.3, with twenty 21.4
     const int64_t most = 16ll * rf::device_cu_count();
-    const int per = (int)std::min<int64_t>(std::max<int64_t>(((int64_t)chunks * heads + most - 1) / most, (heads + 65534) / 65535), heads);
-    const dim3 grid(chunks, (heads + per - 1) / per);
+    const int per = (int)std::min<int64_t>(std::max<int64_t>(((int64_t)chunks * heads + most - 1) / most, (heads + 65532) / 65533), heads);
+    const dim3 grid(chunks, (s.num_heads + per - 1) / per + (2 * cache->num_kv_heads + per - 1) / per);
 #define ROPE_GO(D)                                                                                         \
     if (s.neox)                                                                                            \
         hipLaunchKernelGGL((rf::rf_paged_rope8_kernel<D, true>), grid, dim3(rf::rope8_threads<D>()), 0, stream, s, *cache, per);    \
