@@ -551,7 +551,7 @@ LoraPlan lora_plan(const rf_lora& s, int num_targets) {
     // 32: 512 rows 19.8 / 20.0 / 25.9, 1024 27.7 / 26.1 / 28.9, 2048 49.5 / 43.4 / 46.1, 3059 of 30 requests 76 / 72 / 66
     p.mb = p.rb == 8 || s.rows < 768 ? 1 : s.rows < 2560 ? 2 : 4;
     // (groups of 64 requests are no more than the adapters, and none)
-    const int64_t groups = std::min<int64_t>(s.num_seqs, (int64_t)ceil_div(s.num_seqs, 64) * std::min(64, s.num_adapters + 1));
+    const int64_t groups = std::min<int64_t>(s.num_seqs, (int64_t)ceil_div(s.num_seqs, 64) * (std::min(63, s.num_adapters) + 1));
     const auto tiles = [&](int mb) { return ceil_div(std::min<int64_t>(s.rows, s.rows / (16 * mb) + groups), 8) * 8; };
     p.down = tiles(p.mb);
     p.up = tiles(1);
