@@ -308,6 +308,9 @@ __device__ __forceinline__ int lora_down(const rf_lora& s, const uint16_t* a, co
         __builtin_amdgcn_sched_barrier(0);
         multiply(k + NW, v1);
         __builtin_amdgcn_sched_barrier(0);
+        // (the sums are read behind the loop, 8 wait states after the last product at the earliest: the compiler
+        // left 6 where a branch skips the last block of ranks)
+        asm volatile("s_nop 7");
     }
     // lane: row col, ranks 16 i + 4 quad ..
 #pragma unroll
