@@ -882,10 +882,11 @@ hipError_t rf_paged_attention8_launch(const rf_paged_attention* step, const rf_p
  * and their ranks (q, k and v; gate and up).  a_i[j, k] = a[i * a_stride + j * in_dim + k]
  * (j < max_rank) and b_i[n, j] = b[i * b_stride + n * max_rank + j] are fp16 bits; parts of
  * them behind an adapter's rank are not used, whatever they hold.  ranks are clipped to [0, max_rank].
- * x is fp32, or fp16 bits (x_f16 != 0): fp32 values are taken as two of fp16's (22 bits; beyond
- * 65504 NaN or infinite sums), the inner sums as two of fp16's against the row's largest, products
- * are added in fp32, in an order that goes by the batch.  y may be base itself (with ld_y = ld_base), else they do not overlap;
- * rows past q_start[num_seqs] are left as they were, q_start does not fall.
+ * x is fp32, or fp16 bits (x_f16 != 0): fp32 values are taken whole or as two of fp16's against their
+ * row's largest (22 bits, the smallest step 2^-42 of that one), the inner sums as two of fp16's against theirs
+ * (2^-38), products are added in fp32, in an order that goes by the batch.  Infinities and NaN in a row of x, and
+ * inner sums beyond fp32's range, make the row infinite or NaN where it has an adapter.  y may be base itself
+ * (with ld_y = ld_base), else they do not overlap; rows past q_start[num_seqs] are left as they were, q_start does not fall.
  * in_dim a multiple of 8, max_rank of 8 and at most 128, out_dim, ld_base and ld_y of 4, ld_x (in
  * elements) of 8 (fp16) or 4, a_stride and b_stride of 8; pointers to x, a, b, base and y 16-byte
  * aligned; in_dim, out_dim <= 2^20; rows <= 2^23; num_targets 1 to 3.  targets is read during the call only.
