@@ -891,7 +891,8 @@ hipError_t rf_paged_attention8_launch(const rf_paged_attention* step, const rf_p
  * elements) of 8 (fp16) or 4, a_stride and b_stride of 8; pointers to x, a, b, base and y 16-byte
  * aligned; in_dim, out_dim <= 2^20; rows <= 2^23; num_targets 1 to 3.  targets is read during the call only.
  * workspace: rf_lora_workspace_bytes bytes (it depends on the numbers of both blocks, not on what their
- * buffers hold; 0: none is needed), 16-byte aligned; launches that share one must be stream-ordered. */
+ * buffers hold; 0: none is needed; no less where any of these numbers is larger, so the largest step's serves all),
+ * 16-byte aligned; launches that share one must be stream-ordered. */
 typedef struct rf_lora {
     const void* x;
     const int32_t* adapters;

@@ -587,6 +587,12 @@ struct LoraPlan {
     int slices, each;            // of k
 };
 
+// Tiles of A x have 16 times as many rows.
+int blocks_of_rows(int rows) { return rows < 768 ? 1 : rows < 2560 ? 2 : 4; }
+
+// Workgroups that slices of k are to come to, and the most slices.
+constexpr int kDownAim = 288, kSlices = 8;
+
 LoraPlan lora_plan(const rf_lora& s, int num_targets) {
     LoraPlan p;
     // (a single token, 4096 -> 4096 + 1024 + 1024, rank 16, in a graph 8.3 us for 8.7, and a launch less to issue;
@@ -596,21 +602,27 @@ LoraPlan lora_plan(const rf_lora& s, int num_targets) {
     p.rb = blocks <= 1 ? 1 : blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8;
     // Tiles of more rows read A less often and leave fewer workgroups.  us, 16 / 32 / 64 rows, 12288 -> 4096 of rank
     // 32: 512 rows 19.8 / 20.0 / 25.9, 1024 27.7 / 26.1 / 28.9, 2048 49.5 / 43.4 / 46.1, 3059 of 30 requests 76 / 72 / 66
-    p.mb = p.rb == 8 || s.rows < 768 ? 1 : s.rows < 2560 ? 2 : 4;
+    p.mb = p.rb == 8 ? 1 : blocks_of_rows(s.rows);
     // (groups of 64 requests are no more than the adapters, and none)
     const int64_t groups = std::min<int64_t>(s.num_seqs, (int64_t)ceil_div(s.num_seqs, 64) * (std::min(63, s.num_adapters) + 1));
     const auto tiles = [&](int mb) { return ceil_div(std::min<int64_t>(s.rows, s.rows / (16 * mb) + groups), 8) * 8; };
     p.down = tiles(p.mb);
     p.up = tiles(1);
     // few tiles: k over more workgroups, at least 256 each (16 rows, 12288 -> 4096: 4 slices 17.9 us, 8 14.8)
-    p.slices = std::min(std::max(288 / (p.down * num_targets), 1), 8);
+    p.slices = std::min(std::max(kDownAim / (p.down * num_targets), 1), kSlices);
     p.each = ceil_div(ceil_div(s.in_dim, p.slices), 256) * 256;
     p.slices = ceil_div(s.in_dim, p.each);
     return p;
 }
 
+// No less than num_targets p.slices rows slots, and no less for a larger step, so that the largest one's workspace serves
+// all: there are no fewer tiles than rows / (16 p.mb), and no more slices than these leave of kDownAim.
 size_t lora_bytes(const rf_lora& s, const LoraPlan& p, int num_targets) {
-    return p.whole ? 0 : (size_t)num_targets * p.slices * s.rows * 16 * p.rb * sizeof(float);
+    if (p.whole) return 0;
+    const int64_t rows = (int64_t)num_targets * s.rows;
+    const int64_t slots = std::min<int64_t>(rows * std::min(kSlices, ceil_div(s.in_dim, 256)),
+                                            std::max<int64_t>(rows, kDownAim * 16 * blocks_of_rows(s.rows)));
+    return (size_t)slots * 16 * p.rb * sizeof(float);
 }
 
 }  // namespace

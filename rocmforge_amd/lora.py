@@ -46,7 +46,8 @@ def _targets(targets):
 
 
 def workspace_bytes(step: LoraStep, targets) -> int:
-    """Bytes of a launch's workspace; 0 where it needs none (or is refused)."""
+    """Bytes of a launch's workspace; 0 where it needs none (or is refused).  A server's largest step (rows, requests,
+    targets, ranks, widths) needs the most."""
     targets, block = _targets(targets)
     return int(load().rf_lora_workspace_bytes(ctypes.byref(step), block, len(targets)))
 
