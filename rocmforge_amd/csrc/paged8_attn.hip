@@ -343,9 +343,10 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
 // 75 us, with 16 rows a wave over fp16 values in LDS 106.
 //
 // A row's maximum is rounded up to a whole number, so that the two waves' weights come to the
-// larger one by powers of two, exactly.  No weight of a row need be one of fp16's then, so the sum is
-// of the weights before they are rounded: an output is off by their roundings, 2^-11 of sum w |v|
-// at most, where a sum of rounded weights would let two comparable ones err by twice that.
+// larger one by powers of two, exactly but for those that become subnormal.  No weight of a row need be one of
+// fp16's then, so the sum is of the weights before they are rounded: an output is off by their roundings, 2^-11
+// of sum w |v| at most, where a sum of rounded weights would let two comparable ones err by twice that.  A row of
+// one key has its value all the same: its sum, that one weight, is rounded at the end.
 constexpr int kPairRows = 32, kPairStages = 3;
 template <int D, int NW>
 constexpr int pair8_lds() { return 2 * kPairStages * kWideKeys * D + NW * (2 * 2048 + 3 * 4 * kPairRows) + 1024; }
@@ -789,6 +790,7 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
     if (part == 0) *(lds_f)(sum_at + 4u * M * wave) = l;
     lds_barrier();
     l += *(lds_f)(sum_at + 4u * M * (wave ^ 1));
+    if (pos == 0 || a.window == 1) l = (float)(_Float16)l;
     if (!active || w0 + col >= rows) return;
     const int d0 = D / 2 * half + 4 * part;
     if (s.parts > 1) {

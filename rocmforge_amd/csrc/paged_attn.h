@@ -47,9 +47,10 @@ constexpr float kNone = -3.0e+38f;               // the maximum of no scores
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's maximum is left behind until a score passes it by more than 2^8: most
 // tiles then rescale nothing.  Weights reach 256 (fp16 ends at 65504), and since
-// the sum is of the rounded weights, a row of one key still has it exactly.  Each row
-// renews its own: were a wave's rows renewed together, keys that only some of
-// them see would enter the others' roundings.
+// the sum is of the rounded weights, a row of one key still has it exactly (heads of 256
+// over 8-bit pages, whose sum is not, see to that by themselves).  Each row renews its own:
+// were a wave's rows renewed together, keys that only some of them see would enter the
+// others' roundings.
 constexpr float kLag = 8.0f;
 
 constexpr int kNarrowRows = 16, kNarrowKeys = 32;
