@@ -227,10 +227,10 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
                 top = fmaxf(top, x[b][e]);
             }
         top = xor_butterfly<32, 16>(top, max_raw);
-        const bool up = top > m + kLag;
+        const bool up = top > m + (kLag + kLift);
         if (__ballot(up)) {
-            const float f = up ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
-            m = up ? top : m;
+            const float f = up ? __builtin_amdgcn_exp2f(m - (top - kLift)) : 1.0f;
+            m = up ? top - kLift : m;
             l *= f;
 #pragma unroll
             for (int i = 0; i < NB; ++i) o[i] *= f;
@@ -240,7 +240,7 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int e = 0; e < 4; ++e) p[4 * b + e] = (_Float16)__builtin_amdgcn_exp2f(x[b][e] - m);
-        l = sum8(p, l);
+        l += sum8(p, 0.0f);
         // V^T: lane (dim 16 i + col) takes keys 4 quad + {0 .. 3, 16 .. 19}, as p holds them.  NaN
         // among values that some rows do not see must not meet their zero weights: finite values
         // take its place, and the rows that see it get it at the end.
@@ -584,12 +584,15 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
         const float most = fmaxf(own, other);
         if (__ballot(most != m || most != own || most != other)) {
             const float f = __builtin_amdgcn_exp2f(m - most), g = __builtin_amdgcn_exp2f(own - most);
-            const _Float16 mine = (_Float16)g, others = (_Float16)__builtin_amdgcn_exp2f(other - most);
+            // (in two factors: fp16 ends at 2^-24, and a weight of 2^15 times less than that may count)
+            auto bring = [&](h8* q, float by) {
+                const float some = ceilf(0.5f * by);
+                const _Float16 a = (_Float16)__builtin_amdgcn_exp2f(some), b = (_Float16)__builtin_amdgcn_exp2f(by - some);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                p[i] *= mine;
-                p[2 + i] *= others;
-            }
+                for (int i = 0; i < 2; ++i) q[i] = q[i] * a * b;
+            };
+            bring(p, own - most);
+            bring(p + 2, other - most);
             l *= g;
             m = own = most;
 #pragma unroll
@@ -610,8 +613,8 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, x[e]);
         top = xor_butterfly<32, 32>(top, max_raw) * scale;
-        const bool up = top > m + kLag;
-        own = up ? ceilf(top) : m;
+        const bool up = top > m + (kLag + kLift);
+        own = up ? ceilf(top) - kLift : m;
         if (__ballot(up)) l *= up ? __builtin_amdgcn_exp2f(m - own) : 1.0f;
         // a score times the scale less the maximum in one fma; past 2^23, where the maximum was itself
         // rounded by a half and more, the product is rounded as it was
@@ -625,13 +628,15 @@ __device__ __forceinline__ void pair8_part(const rf_paged_attention& a, const rf
         }
     };
     u32x4 w[2];
+    float sum = 0.0f;                            // of a tile's weights
     auto weights = [&](int n, const f16v& x) {
         float f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) f[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * n + i], mul, -own));
         w[n >> 2][n & 3] = __builtin_bit_cast(uint32_t, h2{(_Float16)f[0], (_Float16)f[1]});
         asm volatile("" : "+v"(w[n >> 2][n & 3]));               // here, not where it is used
-        l += f[0] + f[1];
+        sum = (n == 0 ? 0.0f : sum) + (f[0] + f[1]);
+        if (n == 7) l += sum;
     };
     auto give = [&](int tile) {
         const uint32_t at = weights_at(wave, tile);

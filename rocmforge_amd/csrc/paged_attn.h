@@ -52,6 +52,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // were a wave's rows renewed together, keys that only some of them see would enter the
 // others' roundings.
 constexpr float kLag = 8.0f;
+// Over 8-bit pages a row's maximum, as it is kept, is 2^7 below its largest score, so that weights reach 2^15, have
+// their 11 bits down to 2^-21 and count down to 2^-32 of the largest.  A tile's are added up before they join the sum:
+// what 100000 keys have beside one that leads by e^17 counts.
+constexpr float kLift = 7.0f;
 
 constexpr int kNarrowRows = 16, kNarrowKeys = 32;
 constexpr int kWideKeys = 64;
@@ -326,6 +330,7 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
     constexpr int KS = D / G::DK, NB = D / M, XB = kWideKeys / M, E = G::E, XE = XB * E;
     constexpr bool BESIDE = M == 32;             // the next tile's scores beside a tile's weights
     constexpr bool CODES = std::is_same_v<C, rf_paged_cache8>;
+    constexpr float LIFT = CODES ? kLift : 0.0f;
     static_assert(NI >= 1, "every wave has rows to fetch");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane % M, part = lane / M;   // a lane's packed row, and which keys or dims of it it has
@@ -563,11 +568,11 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
         // exp(x - m) as 2^(x scale - m), one fma: m is a rounded product and the fma's is not, so
         // a row's weights are off by one common factor of 2^(half a step of m).  Far from zero
         // (2^7) scores are rounded as m is, lest the factor leave fp16's range.
-        const bool up = top > m + kLag;
+        const bool up = top > m + (kLag + LIFT);
         float mul = scale;
         if (__ballot(up || far)) {
-            const float f = up ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
-            m = up ? top : m;
+            const float f = up ? __builtin_amdgcn_exp2f(m - (top - LIFT)) : 1.0f;
+            m = up ? top - LIFT : m;
             l *= f;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
@@ -617,11 +622,13 @@ __device__ __forceinline__ void wide_part(const rf_paged_attention& a, const C& 
             for (int two = 0; two < TWOS; ++two) weights(two);
         }
         h8 p[STEPS];
+        float sum = CODES ? 0.0f : l;
 #pragma unroll
         for (int j = 0; j < STEPS; ++j) {
             p[j] = __builtin_bit_cast(h8, w[j]);
-            l = sum8(p[j], l);
+            sum = sum8(p[j], sum);
         }
+        l = CODES ? l + sum : sum;
         // infinities and NaN among values that some rows do not see must not meet their zero
         // weights: finite ones take their place, and the rows that see them get them at the end
         Finite fin;
