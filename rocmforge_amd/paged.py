@@ -205,10 +205,12 @@ def _one_device(indexes):
 def _stream(stream, on):
     """The stream's handle.  on: the tensors' device, None where there are addresses only."""
     import torch
-    if stream is None and torch.cuda.is_initialized():
-        # the handle itself: torch.cuda.current_stream() takes 2.5 us to make an object around it, of a launch's 6.4
+    # the handle itself: torch.cuda.current_stream() takes 2.5 us to make an object around it, of a launch's 6.4 (a call
+    # that torch does not document, so it may be missing)
+    handle = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if stream is None and handle is not None and torch.cuda.is_initialized():
         current = torch.cuda.current_device()
-        stream = torch._C._cuda_getCurrentRawStream(current)
+        stream = handle(current)
     elif stream is None:
         stream = torch.cuda.current_stream()
         current = stream.device_index
