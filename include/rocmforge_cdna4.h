@@ -886,7 +886,8 @@ hipError_t rf_paged_attention8_launch(const rf_paged_attention* step, const rf_p
  * row's largest (22 bits, the smallest step 2^-42 of that one), the inner sums as two of fp16's against theirs
  * (2^-38), products are added in fp32, in an order that goes by the batch.  Infinities and NaN in a row of x, and
  * inner sums beyond fp32's range, make the row infinite or NaN where it has an adapter.  y may be base itself
- * (with ld_y = ld_base), else they do not overlap; rows past q_start[num_seqs] are left as they were, q_start does not fall.
+ * (with ld_y = ld_base), else they do not overlap; y overlaps neither x nor another target's base or y; rows past
+ * q_start[num_seqs] are left as they were, q_start does not fall.
  * in_dim a multiple of 8, max_rank of 8 and at most 128, out_dim, ld_base and ld_y of 4, ld_x (in
  * elements) of 8 (fp16) or 4, a_stride and b_stride of 8; pointers to x, a, b, base and y 16-byte
  * aligned; in_dim, out_dim <= 2^20; rows <= 2^23; num_targets 1 to 3.  targets is read during the call only.

@@ -124,7 +124,7 @@ __device__ __forceinline__ bool lora_item(const rf_lora& s, int pieces, LoraItem
 // read 512 bytes at a time; the waves are spread over the blocks of ranks, then over k.  AHEAD: loads are a turn ahead
 // where there are more than two (64 single tokens on 40 adapters 44.4 -> 42.3 us, 200 90 -> 85; one token of rank 64, of
 // two turns, 14.8 -> 15.3; eight waves do not have the registers).
-template <bool X16, bool AHEAD, int RB, int MB, int NW, int HS>
+template <bool X16, bool AHEAD, int MB, int NW, int HS>
 __device__ __forceinline__ int lora_dots(const rf_lora& s, const uint16_t* a, const LoraItem<MB>& w, int k0, int k1,
                                          float (*part)[16 * MB][HS]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rank = w.rank;
@@ -496,7 +496,7 @@ __global__ __launch_bounds__(64 * NW) void rf_lora_whole_kernel(const rf_lora s,
     const int nb0 = w.piece * each, nb1 = min(nb0 + each, blocks);
     if (nb0 >= nb1) return;
     if (w.rank == 0) return lora_copy<NW>(g, w, nb0, nb1);
-    const int slices = lora_dots<X16, false, RB, 1, NW, HS>(s, g.a + w.id * g.a_stride, w, 0, s.in_dim, part);
+    const int slices = lora_dots<X16, false, 1, NW, HS>(s, g.a + w.id * g.a_stride, w, 0, s.in_dim, part);
     lds_barrier();
     const int r = min((int)threadIdx.x & 15, w.rows - 1);
     lora_up<RB, NW>(s, g, w, nb0, nb1, slices, [&](int k, int j) { return *reinterpret_cast<const f4*>(&part[k][r][j]); });
@@ -517,7 +517,7 @@ __global__ __launch_bounds__(64 * NW) void rf_lora_down_kernel(const rf_lora s, 
         for (int m = 0; m < MB; ++m) rows[16 * m + threadIdx.x] = (int)w.row[m];
     const int k0 = w.piece * each, k1 = min(k0 + each, s.in_dim);
     const uint16_t* a = g.a + w.id * g.a_stride;
-    const int parts = w.rows <= kFewRows ? lora_dots<X16, true, RB, MB, NW, HS>(s, a, w, k0, k1, part)
+    const int parts = w.rows <= kFewRows ? lora_dots<X16, true, MB, NW, HS>(s, a, w, k0, k1, part)
                                          : lora_down<X16, RB, MB, NW, U, HS>(s, a, w, k0, k1, part);
     lds_barrier();
     float* to = sums + (int64_t)(blockIdx.y * slices + w.piece) * s.rows * (16 * RB);

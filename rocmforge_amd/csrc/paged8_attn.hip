@@ -40,10 +40,6 @@ __device__ __forceinline__ void lds_dma_byte_at(uint32_t lds_dst, uint64_t at) {
 
 // ---- few rows -------------------------------------------------------------------------
 //
-// As over fp16 pages (paged_attn.hip): wave w takes the pieces of 32 positions w, w + W, .. of
-// the part through its own S-stage ring in LDS, codes as they are; they become fp16 in
-// registers, K's under its row's exponent and V's under their keys' (lane 4 i + j of a window
-// of 16 pieces holds address and exponents of piece i's unit j of 8 positions).
 // find_share's items in another order, for 17 to 64 requests: those of the longest parts first, in eighths of
 // a share, so that short ones fill the end of a launch.  48 requests of 60 to 16000 positions 49.1 us, in the
 // requests' order 52.6, 32 of 100 to 8000 24.5 and 27.3; for few requests it is 0.2 us of instructions.
@@ -78,6 +74,10 @@ __device__ __forceinline__ bool find_longest(const rf_paged_attention& a, const 
     return false;
 }
 
+// As over fp16 pages (paged_attn.hip): wave w takes the pieces of 32 positions w, w + W, .. of
+// the part through its own S-stage ring in LDS, codes as they are; they become fp16 in
+// registers, K's under its row's exponent and V's under their keys' (lane 4 i + j of a window
+// of 16 pieces holds address and exponents of piece i's unit j of 8 positions).
 template <int D, int W, int S>
 __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const rf_paged_cache8& c, const Plan& plan,
                                              int item, uint8_t* lds) {
