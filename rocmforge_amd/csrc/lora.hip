@@ -122,8 +122,10 @@ __device__ __forceinline__ bool lora_item(const rf_lora& s, int pieces, LoraItem
 // A x over [k0, k1) of the tile's rows into part [wave][row][rank], a share each of the first waves; returns how
 // many.  Few rows: dot products.  A wave takes 256 k of 16 ranks, a lane four of them, so that a row of A is
 // read 512 bytes at a time; the waves are spread over the blocks of ranks, then over k.  AHEAD: loads are a turn ahead
-// where there are more than two (64 single tokens on 40 adapters 44.4 -> 42.3 us, 200 90 -> 85; one token of rank 64, of
-// two turns, 14.8 -> 15.3; eight waves do not have the registers).
+// where there are more than two (64 single tokens on 40 adapters 44.1 -> 42.3 us, 200 90 -> 85, rank 128 70 -> 65; one
+// token of rank 64, of two turns, 14.8 -> 15.3; eight waves do not have the registers).  It takes the kernel's registers
+// to 256 and more, one wave a SIMD, for the tiles of many rows too: prompts of rank 128 178 -> 172 and 72 166 -> 140,
+// rank 32 even, pieces of prompt of up to 200 rows 28.5 -> 29.4.
 template <bool X16, bool AHEAD, int MB, int NW, int HS>
 __device__ __forceinline__ int lora_dots(const rf_lora& s, const uint16_t* a, const LoraItem<MB>& w, int k0, int k1,
                                          float (*part)[16 * MB][HS]) {
@@ -661,7 +663,7 @@ extern "C" hipError_t rf_lora_add_launch(const rf_lora* step, const rf_lora_targ
     float* sums = static_cast<float*>(s.workspace);
     // Pieces of the columns: one workgroup a CU for few tiles (each starts with some 4 us of latencies), two for many,
     // whose ranks differ.  us, 256 / 512 / 768 workgroups: 2 tokens on adapters of up to 64, 4096 -> 2 x 12288, 14.1 /
-    // 15.1 / 18.4, 16 19.1 / 22.6 / 21.9, 64 on 40 adapters 49.3 / 44.1 / 43.5
+    // 15.5 / 19.4, 16 18.7 / 22.7 / 22.7, 64 on 40 adapters 56.6 / 42.3 / 42.5
     const int tiles = p.up * num_targets;
     const int pieces = std::min(ceil_div(tiles < 64 ? 256 : 512, tiles), ceil_div(widest, 64 * NW));
     const dim3 down((unsigned)(p.down * p.slices), num_targets), up((unsigned)(p.up * pieces), num_targets), blk(64 * NW);

@@ -41,7 +41,7 @@ __device__ __forceinline__ void lds_dma_byte_at(uint32_t lds_dst, uint64_t at) {
 // ---- few rows -------------------------------------------------------------------------
 //
 // find_share's items in another order, for 17 to 64 requests: those of the longest parts first, in eighths of
-// a share, so that short ones fill the end of a launch.  48 requests of 60 to 16000 positions 49.1 us, in the
+// a share, so that short ones fill the end of a launch.  48 requests of 60 to 16000 positions 49.2 us, in the
 // requests' order 52.6, 32 of 100 to 8000 24.5 and 27.3; for few requests it is 0.2 us of instructions.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ bool find_longest(const rf_paged_attention& a, const rf_paged_cache8& c, const Plan& p, int j,
@@ -338,9 +338,9 @@ __device__ __forceinline__ void narrow8_part(const rf_paged_attention& a, const 
 // wave's queries and outputs take 128 registers, two waves fit a SIMD, and an operand that is
 // read from LDS meets 32 rows.  Codes stay codes in LDS and become fp16 on their way into the MFMAs:
 // an operand's conversion is 16 clocks of VALU beside the 32 of its MFMA.  Three stages of tiles: with two,
-// each turn waited for memory.  A turn of 64 positions takes 5000 clocks where its MFMAs take 2048 and its
-// VALU instructions 2700 a SIMD, in two waves that overlap them in part; a step of three windowed prompts
-// 75 us, with 16 rows a wave over fp16 values in LDS 106.
+// each turn waited for memory.  A turn of 64 positions takes 2.16 us, some 5000 clocks, where its MFMAs take 2048 and
+// its VALU instructions 2700 a SIMD, in two waves that overlap little; a step of three windowed prompts
+// 70 us, with 16 rows a wave over fp16 values in LDS 106; 512 tokens behind 62800 positions 564 us, 940 TFLOP/s.
 //
 // A row's maximum is rounded up to a whole number, so that the two waves' weights come to the
 // larger one by powers of two, exactly but for those that become subnormal.  No weight of a row need be one of
@@ -358,8 +358,9 @@ __device__ __forceinline__ uint32_t pair_swizzle(uint32_t row) { return 2 * ((ro
 // find_share's items in another order, for up to 64 requests: those that a window makes equally long in the
 // requests' order, then the first (longest) of the others of each request, the second of each, and
 // so on, so that short ones fill the end of a launch.  16 heads on 8, window 1024: three prompts of 600 to
-// 1900 tokens and six single ones 75 us, in the requests' order 83; four of 100 to 3000 71 and 74 (all of
-// them by rank 86: neighbours share K and V in an XCD's L2); eight of 200 to 1000 without a window 115 and 124.
+// 1900 tokens and six single ones 72 us, in the requests' order 80; four of 100 to 3000 69 and 71 (all of
+// them by rank 15 more: neighbours share K and V in an XCD's L2); eight of 200 to 1000 behind up to 6000 positions
+// without a window 135 and 144, but eight fresh ones 64.5 and 61.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ bool find_ranked(const rf_paged_attention& a, const rf_paged_cache8& c, const Plan& p, int j,
                                             Share& s) {
