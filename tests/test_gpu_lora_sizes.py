@@ -83,3 +83,25 @@ def test_a_row_is_the_same_size_in_any_company(rf, dev):
     alone.check()
     want, bound = alone.want(0)
     assert bool(((c.y[0][7:8].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("new", [[5], [40], [17, 30, 6], [800], [2600]])
+@pytest.mark.parametrize("max_rank", [16, 32, 64, 128])
+@pytest.mark.parametrize("looked_at", [False, True])
+def test_values_that_do_not_fit_the_first_ones(rf, dev, new, max_rank, looked_at):
+    # 10^3 to 10^30 times the others, in some rows, far behind where a wave begins; rows without one keep their bits
+    c = Case(new, (max_rank, max_rank - 9, 7), max_rank, k=12288, widths=(72,))
+    n, dims = sum(new), torch.arange(700, 12288, 1333, device=P.DEV)
+    if not looked_at:
+        c.a[0][:, :, dims] = 0.0
+    c.run()
+    want = c.y[0][:n].clone()
+    rows = torch.arange(1, n, 3, device=P.DEV)
+    size = torch.pow(10.0, 3 + (rows * 7 % 28 if looked_at else rows % 4).double()).float()
+    c.x[rows, dims[rows % len(dims)]] = size
+    c.run()
+    value, bound = c.want(0)
+    assert bool(((c.y[0].double() - value).abs() <= bound)[:n].all())
+    others = torch.ones(n, dtype=torch.bool, device=P.DEV)
+    others[rows] = False
+    assert torch.equal(c.y[0][:n][others], want[others])
